@@ -328,7 +328,7 @@ def run(state):
             return y
         return tuple(t.detach() for t in y) + torch.autograd.grad(y, (q, k), (state["dq"], state["dk"]))
     q, k, v = state["q"], state["k"], state["v"]
-    o = fa.flash_attention_v100(q, k, v, score_cap=case["cap"] or None, distance_slopes=state["slopes"], key_ranges=state["ranges"])
+    o = fa.flash_attention_v100_with_rules(q, k, v, score_cap=case["cap"] or None, distance_slopes=state["slopes"], key_ranges=state["ranges"])
     if not case["train"]:
         return (o,)
     return (o.detach(),) + torch.autograd.grad(o, (q, k, v), state["do"])
