@@ -94,10 +94,53 @@ BwdWorkspace bwd_workspace_layout(const fa_b200_params& p, int variant, bool inl
 // What AUTO resolves to besides the public variants: the pair instances of the tensor-core kernels.
 constexpr int kVariantPair = 16;
 
+// ---- key ranges (key_ranges.cu) ------------------------------------------------
+// A plan's regions, int32, one after the other, each for all batch entries:
+//   rows     [B][nq_pad]        int2  first, end of a row ((0, 0): sees nothing; so the padding rows)
+//   q_tiles  [B][nq_pad / 128]  int4  of a tile's rows: least first and largest end of those that see keys (0, 0: none),
+//                                     largest first, least end of all rows below Nq (2^31 - 1, 0 if one sees nothing)
+//   q_parts  [B][nq_pad / 16]   int2  the same hull for 16 rows
+//   k_tiles  [B][nk_pad / 128]  int2  first and end of the query tiles whose hull meets the key tile ((0, 0): none)
+//   origin   [B]                      position of row 0
+struct RangesLayout {
+    int64_t q_tiles, q_parts, k_tiles, origin, total;          // in int32; rows are at 0
+    int nq_pad, nk_pad;
+};
+static inline __host__ __device__ RangesLayout ranges_layout(int64_t B, int Nq, int Nk) {
+    RangesLayout l;
+    l.nq_pad = (int)(((int64_t)Nq + 127) / 128 * 128);
+    l.nk_pad = (int)(((int64_t)Nk + 127) / 128 * 128);
+    l.q_tiles = B * l.nq_pad * 2;
+    l.q_parts = l.q_tiles + B * (l.nq_pad / 128) * 4;
+    l.k_tiles = l.q_parts + B * (l.nq_pad / 16) * 2;
+    l.origin = l.k_tiles + B * (l.nk_pad / 128) * 2;
+    l.total = l.origin + (B + 3) / 4 * 4;
+    return l;
+}
+// The rules of a call as its kernels read them (rows = nullptr: none).  Strides over the batch, 0 where one plan serves all.
+struct Rules {
+    const int2* rows; const int4* q_tiles; const int2* q_parts; const int2* k_tiles; const int32_t* origin;
+    int64_t rows_b, q_tiles_b, q_parts_b, k_tiles_b, origin_b;
+    const float* slopes;           // optional, one per head
+    float cap;                     // 0: none
+};
+static inline Rules make_rules(const fa_b200_rules& r, int Nq, int Nk) {
+    const RangesLayout l = ranges_layout(r.plan_batch, Nq, Nk);
+    const int32_t* base = (const int32_t*)r.plan;
+    const bool shared = r.plan_batch == 1;
+    Rules u;
+    u.rows = (const int2*)base; u.q_tiles = (const int4*)(base + l.q_tiles); u.q_parts = (const int2*)(base + l.q_parts);
+    u.k_tiles = (const int2*)(base + l.k_tiles); u.origin = base + l.origin;
+    u.rows_b = shared ? 0 : l.nq_pad; u.q_tiles_b = shared ? 0 : l.nq_pad / 128; u.q_parts_b = shared ? 0 : l.nq_pad / 16;
+    u.k_tiles_b = shared ? 0 : l.nk_pad / 128; u.origin_b = shared ? 0 : 1;
+    u.slopes = r.slopes; u.cap = r.score_cap;
+    return u;
+}
+
 // ---- kernel families ---------------------------------------------------------
 // CUDA-core tiles (simt_kernels.cu)
-int simt_fwd(const fa_b200_params& p);
-int simt_bwd(const fa_b200_params& p, const BwdWorkspace& ws);
+int simt_fwd(const fa_b200_params& p, const Rules* rules = nullptr);
+int simt_bwd(const fa_b200_params& p, const BwdWorkspace& ws, const Rules* rules = nullptr);
 bool simt_supports(const fa_b200_params& p);
 
 // TMA + tcgen05 (fwd_sm100.cu, bwd_sm100.cu)

@@ -355,6 +355,87 @@ int fa_b200_bwd_with_scratch(const fa_b200_params* p, void* scratch, size_t scra
     return variant != FA_B200_VARIANT_SIMT ? sm100_bwd(*p, ws) : simt_bwd(*p, ws);
 }
 
+// ---- calls with rules: capped scores, distances, a range of keys for each row ----
+}  // extern "C"
+
+namespace {
+int validate_rules(const fa_b200_params* p, const fa_b200_rules* r) {
+    if (!r) { set_error("rules is null"); return FA_EINVAL; }
+    if (r->struct_bytes != sizeof(fa_b200_rules)) {
+        set_error("struct_bytes %zu does not match this library's fa_b200_rules (%zu bytes)", r->struct_bytes, sizeof(fa_b200_rules));
+        return FA_EINVAL;
+    }
+    if (p->causal || p->causal_shift || p->bias.ptr || p->d_scores || p->kv_lengths || p->dropout_p != 0.f || p->rng_heads) {
+        set_error("a call with rules has no causal mask, bias, key counts or dropout of its own");
+        return FA_EINVAL;
+    }
+    if (!(r->score_cap >= 0.f) || r->score_cap > 1e30f) { set_error("score_cap must be 0 or positive and finite"); return FA_EINVAL; }
+    if (r->score_cap > 0.f && !(p->scale * p->scale < 1e30f * r->score_cap)) { set_error("scale is too large for the cap"); return FA_EINVAL; }
+    if (p->B > 0 && p->Nq > 0) {
+        if (r->plan_batch != 1 && r->plan_batch != p->B) { set_error("the plan is for a batch of %d, the call has %d", r->plan_batch, p->B); return FA_EINVAL; }
+        if (!r->plan) { set_error("the plan is null"); return FA_EINVAL; }
+        if (((uintptr_t)r->plan & 15u) != 0) { set_error("the plan must be 16-byte aligned"); return FA_EALIGN; }
+    }
+    return FA_OK;
+}
+// Kernel family of a call with rules.
+int choose_rules_variant(const fa_b200_params& p, bool backward, int* variant) {
+    (void)backward;
+    if (!simt_supports(p)) { set_error("no kernel covers D=%d with rules", p.D); return FA_EUNSUPPORTED; }
+    *variant = FA_B200_VARIANT_SIMT;
+    return FA_OK;
+}
+}  // namespace
+
+extern "C" {
+
+size_t fa_b200_fwd_rules_workspace_bytes(const fa_b200_params* p) {
+    if (!p || p->struct_bytes != sizeof(fa_b200_params)) return 0;
+    return 0;
+}
+
+int fa_b200_fwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r, void* workspace, size_t workspace_bytes) {
+    int rc = validate_common(p, false);
+    if (rc || (rc = validate_rules(p, r))) return rc;
+    if ((rc = refuse_after_timeout(p, "fa_b200_fwd_with_rules"))) return rc;
+    if (p->B == 0 || p->Nq == 0) return FA_OK;
+    if (p->Nk == 0) { set_error("Nk = 0: there are no keys"); return FA_EINVAL; }
+    int variant;
+    if ((rc = choose_rules_variant(*p, false, &variant))) return rc;
+    GuardDevice g(p->device);
+    if (!g.ok) { set_error("cudaSetDevice(%d) failed", p->device); return FA_ECUDA; }
+    const Rules u = make_rules(*r, p->Nq, p->Nk);
+    (void)workspace; (void)workspace_bytes;
+    return simt_fwd(*p, &u);
+}
+
+size_t fa_b200_bwd_rules_workspace_bytes(const fa_b200_params* p) {
+    if (!p || p->struct_bytes != sizeof(fa_b200_params)) return 0;
+    if (p->B <= 0 || p->Nq <= 0 || p->H <= 0 || p->Hkv <= 0 || p->D <= 0) return 256;
+    return bwd_workspace_layout(*p, FA_B200_VARIANT_SIMT).total;
+}
+
+int fa_b200_bwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r) {
+    int rc = validate_common(p, true);
+    if (rc || (rc = validate_rules(p, r))) return rc;
+    if ((rc = refuse_after_timeout(p, "fa_b200_bwd_with_rules"))) return rc;
+    if (p->B == 0 || (p->Nq == 0 && p->Nk == 0)) return FA_OK;
+    if (p->Nk == 0) { set_error("Nk = 0: there are no keys"); return FA_EINVAL; }
+    GuardDevice g(p->device);
+    if (!g.ok) { set_error("cudaSetDevice(%d) failed", p->device); return FA_ECUDA; }
+    if (p->Nq == 0) return zero_dk_dv(p);
+    int variant;
+    if ((rc = choose_rules_variant(*p, true, &variant))) return rc;
+    const BwdWorkspace ws = bwd_workspace_layout(*p, variant);
+    if (!p->workspace || p->workspace_bytes < ws.total) {
+        set_error("backward needs %zu bytes of workspace, got %zu", ws.total, p->workspace ? p->workspace_bytes : (size_t)0);
+        return FA_EWORKSPACE;
+    }
+    if (((uintptr_t)p->workspace & 255u) != 0) { set_error("workspace must be 256-byte aligned"); return FA_EALIGN; }
+    const Rules u = make_rules(*r, p->Nq, p->Nk);
+    return simt_bwd(*p, ws, &u);
+}
+
 // ---------------------------------------------------------------------------
 // Backward without a caller-supplied workspace.
 //

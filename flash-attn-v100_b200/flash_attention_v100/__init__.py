@@ -13,6 +13,7 @@ from .interface import (
     flash_attention_v100,
     flash_attention_v100_causal,
     flash_attention_v100_with_dropout,
+    flash_attention_v100_with_rules,
     flash_attention_v100_multi_gpu,
     FlashAttentionV100Manager,
     get_flash_attention_manager,
@@ -29,6 +30,8 @@ from .ops.attention import (
     kernel_variant,
 )
 from .ops.host_pipeline import HostAttentionStep
+from .ops.key_ranges import KeyRanges, build_key_ranges
+from .ops.rotary import rotary_embedding, rotary_frequencies
 from .modules import EnhancedMultiHeadAttention
 from .ops.sequence_parallel import flash_attention_v100_sequence_parallel
 
@@ -64,5 +67,6 @@ __all__ = [
     "FlashAttentionV100Manager", "get_flash_attention_manager", "flash_attention_performance_mode",
     "flash_attention_memory_mode", "get_enhanced_config", "plan_shards", "set_dropout_seed",
     "kernel_variant", "HostAttentionStep", "EnhancedMultiHeadAttention",
-    "flash_attention_v100_sequence_parallel",
+    "flash_attention_v100_sequence_parallel", "flash_attention_v100_with_rules", "KeyRanges", "build_key_ranges", "rotary_embedding",
+    "rotary_frequencies",
 ]

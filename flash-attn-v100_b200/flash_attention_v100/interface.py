@@ -20,6 +20,8 @@ import torch.distributed as dist
 
 from .config import get_enhanced_config
 from .ops.attention import FlashAttentionV100Function, native_call
+from .ops.key_ranges import KeyRanges, build_key_ranges
+from .ops.rules import RuledAttentionFunction, check_rules
 from .utils import validate_inputs as _validate_inputs
 
 log = logging.getLogger("flash_attention_v100")
@@ -446,6 +448,63 @@ def flash_attention_v100_with_dropout(q, k, v, dropout_p: float, **kwargs):
     return flash_attention_v100(q, k, v, dropout_p=dropout_p, **kwargs)
 
 
+def flash_attention_v100_with_rules(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    causal: bool = False,
+    scale: Optional[float] = None,
+    *,
+    score_cap: Optional[float] = None,
+    distance_slopes: Optional[torch.Tensor] = None,
+    key_ranges: Optional[KeyRanges] = None,
+    key_lengths: Optional[torch.Tensor] = None,
+    causal_alignment: str = "top_left",
+    return_softmax_lse: bool = False,
+    enable_profiling: bool = False,
+) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Attention whose scores are capped, moved by distances, or limited to a range of keys for each query; forward and
+    backward.  No counterpart in the reference.
+
+        s = scale * q.k;  x = score_cap * tanh(s / score_cap) - distance_slopes[h] * |position_i - j|
+        o = softmax(x over the keys j query i sees) v
+
+    Args:
+        q, k, v, scale, return_softmax_lse, enable_profiling: as flash_attention_v100's; grouped heads, every dtype and
+            head size it takes.  fp16 and bf16 with a head size that is a multiple of 8 run on the tensor cores, others on
+            the CUDA cores
+        score_cap: positive; None leaves the scores as they are
+        distance_slopes: (num_heads,) floating point, no gradient
+        key_ranges: which keys each query sees (build_key_ranges): packed documents, prefixes, windows, ragged caches; built
+            once, read by every layer.  Takes the place of causal, key_lengths and causal_alignment.  A query that sees
+            nothing has an output of zeros, an lse of -inf and no gradient.  position_i counts its query offsets
+        causal, key_lengths, causal_alignment: without key_ranges, as flash_attention_v100's (counts below 1 hide all keys
+            of an entry); ranges for them are built by the call.  position_i is i, with the bottom-right alignment i + Nk - Nq
+
+    Keys and values behind an entry's counts (or outside every range) may be unwritten memory in a call without gradients; in
+    a training step they have to be numbers.  Gradients are bit-reproducible.  One GPU: that of the tensors.
+    """
+    q, k, v, scale = _validate_inputs(q, k, v, scale)
+    if key_ranges is not None and (causal or key_lengths is not None):
+        raise ValueError("key_ranges say which keys are seen: causal and key_lengths cannot be combined with them")
+    shift = _causal_shift(causal, causal_alignment, q.shape[1], k.shape[1], key_lengths)
+    cap, slopes = check_rules(q, k, score_cap, distance_slopes, key_ranges)
+    manager = get_flash_attention_manager()
+    profile = manager.enable_profiling or enable_profiling
+    if profile:
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record(torch.cuda.current_stream(q.device))
+    if key_ranges is None:
+        key_ranges = build_key_ranges(q.shape[1], k.shape[1], batch=1 if key_lengths is None else q.shape[0], causal=causal,
+                                      key_lengths=key_lengths, query_offsets=shift, device=q.device)
+    o, lse = RuledAttentionFunction.apply(q, k, v, scale, cap, slopes, key_ranges.plan, key_ranges.batch)
+    if profile:
+        end.record(torch.cuda.current_stream(q.device))
+        end.synchronize()
+        _record_performance(manager, start.elapsed_time(end), q.shape, k.shape[1], causal)
+    return (o, lse) if return_softmax_lse else o
+
+
 def flash_attention_v100_multi_gpu(q, k, v, **kwargs):
     """Reference interface.py:633-640."""
     return flash_attention_v100(q, k, v, enable_multi_gpu=True, **kwargs)
@@ -472,6 +531,6 @@ def flash_attention_memory_mode():
 
 __all__ = [
     "flash_attention_v100", "flash_attention_v100_causal", "flash_attention_v100_with_dropout",
-    "flash_attention_v100_multi_gpu", "FlashAttentionV100Manager", "get_flash_attention_manager",
+    "flash_attention_v100_with_rules", "flash_attention_v100_multi_gpu", "FlashAttentionV100Manager", "get_flash_attention_manager",
     "flash_attention_performance_mode", "flash_attention_memory_mode", "plan_shards",
 ]

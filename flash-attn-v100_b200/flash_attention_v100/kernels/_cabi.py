@@ -30,6 +30,8 @@ EXPORTS = (
     "fa_b200_copy_rows", "fa_b200_selftest_wait_timeout", "fa_b200_dropout_bits_bytes",
     "fa_b200_fwd_with_workspace", "fa_b200_fwd_workspace_bytes", "fa_b200_bwd_with_scratch", "fa_b200_bwd_scratch_bytes",
     "fa_b200_key_order", "fa_b200_permute_rows",
+    "fa_b200_key_ranges_bytes", "fa_b200_key_ranges", "fa_b200_fwd_with_rules", "fa_b200_fwd_rules_workspace_bytes",
+    "fa_b200_bwd_with_rules", "fa_b200_bwd_rules_workspace_bytes", "fa_b200_rotary",
 )
 
 
@@ -72,6 +74,41 @@ class CombineParams(ctypes.Structure):
         ("dtype", ctypes.c_int32), ("first", ctypes.c_int32), ("device", ctypes.c_int32),
         ("reserved", ctypes.c_int32), ("stream", ctypes.c_void_p),
         ("acc_stride_b", ctypes.c_int64), ("lse_stride_b", ctypes.c_int64), ("lse_stride_h", ctypes.c_int64),
+    ]
+
+
+class RangesParams(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", ctypes.c_size_t),
+        ("plan", ctypes.c_void_p), ("plan_bytes", ctypes.c_size_t),
+        ("positions", ctypes.c_void_p), ("rows", ctypes.c_void_p),
+        ("document_offsets", ctypes.c_void_p), ("prefix_lengths", ctypes.c_void_p),
+        ("key_lengths", ctypes.c_void_p), ("query_offsets", ctypes.c_void_p),
+        ("offsets_stride_b", ctypes.c_int64), ("prefix_stride_b", ctypes.c_int64),
+        ("n_documents", ctypes.c_int32), ("query_offset", ctypes.c_int32),
+        ("causal", ctypes.c_int32), ("window", ctypes.c_int32),
+        ("B", ctypes.c_int32), ("Nq", ctypes.c_int32), ("Nk", ctypes.c_int32), ("device", ctypes.c_int32),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class RuleParams(ctypes.Structure):
+    _fields_ = [("struct_bytes", ctypes.c_size_t), ("plan", ctypes.c_void_p), ("plan_batch", ctypes.c_int32),
+                ("score_cap", ctypes.c_float), ("slopes", ctypes.c_void_p)]
+
+
+class RotaryParams(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", ctypes.c_size_t),
+        ("x", Tensor4 * 2), ("y", Tensor4 * 2), ("heads", ctypes.c_int32 * 2),
+        ("positions", ctypes.c_void_p),
+        ("positions_stride_b", ctypes.c_int64), ("positions_stride_n", ctypes.c_int64), ("position0", ctypes.c_int64),
+        ("inv_freq", ctypes.c_void_p),
+        ("positions_64bit", ctypes.c_int32),
+        ("B", ctypes.c_int32), ("N", ctypes.c_int32), ("D", ctypes.c_int32), ("half", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("factor", ctypes.c_float), ("dtype", ctypes.c_int32), ("device", ctypes.c_int32),
+        ("stream", ctypes.c_void_p),
     ]
 
 
@@ -137,6 +174,21 @@ def load():
         lib.fa_b200_permute_rows.argtypes = [ctypes.c_void_p] * 5 + [ctypes.c_int, ctypes.c_int, ctypes.c_size_t, ctypes.c_int,
                                                                      ctypes.c_int, ctypes.c_void_p]
         lib.fa_b200_permute_rows.restype = ctypes.c_int
+        rp = ctypes.POINTER(RuleParams)
+        lib.fa_b200_key_ranges_bytes.argtypes = [ctypes.c_int] * 3
+        lib.fa_b200_key_ranges_bytes.restype = ctypes.c_size_t
+        lib.fa_b200_key_ranges.argtypes = [ctypes.POINTER(RangesParams)]
+        lib.fa_b200_key_ranges.restype = ctypes.c_int
+        lib.fa_b200_fwd_with_rules.argtypes = [pp, rp, ctypes.c_void_p, ctypes.c_size_t]
+        lib.fa_b200_fwd_with_rules.restype = ctypes.c_int
+        lib.fa_b200_fwd_rules_workspace_bytes.argtypes = [pp]
+        lib.fa_b200_fwd_rules_workspace_bytes.restype = ctypes.c_size_t
+        lib.fa_b200_bwd_with_rules.argtypes = [pp, rp]
+        lib.fa_b200_bwd_with_rules.restype = ctypes.c_int
+        lib.fa_b200_bwd_rules_workspace_bytes.argtypes = [pp]
+        lib.fa_b200_bwd_rules_workspace_bytes.restype = ctypes.c_size_t
+        lib.fa_b200_rotary.argtypes = [ctypes.POINTER(RotaryParams)]
+        lib.fa_b200_rotary.restype = ctypes.c_int
         lib.fa_b200_selftest_wait_timeout.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
         lib.fa_b200_selftest_wait_timeout.restype = ctypes.c_int
         lib.fa_b200_tile_config.argtypes = [ctypes.c_int] * 4 + [ctypes.POINTER(Tile)]

@@ -21,6 +21,8 @@ from .memory import (
 )
 
 from .host_pipeline import HostAttentionStep, chunk_bounds, plan_chunks
+from .key_ranges import KeyRanges, build_key_ranges
+from .rotary import rotary_embedding, rotary_frequencies
 from .sequence_parallel import (
     flash_attention_v100_sequence_parallel,
     ring_schedule,
@@ -37,4 +39,5 @@ __all__ = [
     "get_memory_statistics", "backward_workspace_bytes",
     "HostAttentionStep", "chunk_bounds", "plan_chunks",
     "flash_attention_v100_sequence_parallel", "ring_schedule", "zigzag_split", "zigzag_merge",
+    "KeyRanges", "build_key_ranges", "rotary_embedding", "rotary_frequencies",
 ]

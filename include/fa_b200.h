@@ -317,6 +317,96 @@ int fa_b200_key_order(const uint8_t* mask, int64_t mask_stride_b, int B, int N, 
 int fa_b200_permute_rows(const void* src0, const void* src1, void* dst0, void* dst1, const int32_t* order, int B, int N,
                          size_t row_bytes, int scatter, int device, void* stream);
 
+/*
+ * Key ranges: which keys each query sees, as one interval [first, end) per row, built on the GPU from lengths and kept
+ * for as many attention calls as there are layers.  Documents packed into a row, a prefix all of a document's rows see,
+ * a sliding window, causal masks and caches of ragged lengths are all such intervals.  No counterpart in the reference,
+ * which expands masks to a dense bias (examples/basic_usage.py:228-250).
+ *
+ * Row i of batch entry b stands at position t = i + query_offset + query_offsets[b].
+ *   document    the m with document_offsets[b][m] <= t < document_offsets[b][m + 1] (ascending; none: the row sees
+ *               nothing); without documents one that starts at 0 and has no end
+ *   first       the document's start, with a window at least t - window + 1
+ *   end         the document's end, at most Nk and key_lengths[b]; causal: at most t + 1, or, where it is more, the
+ *               document's start + prefix_lengths[b][m]; a window without causal: at most t + window
+ *   position    t - the document's start (0 for a row of no document)
+ * A row with first >= end sees nothing and is stored as (0, 0).  With `rows` the intervals are given instead (clipped to
+ * [0, Nk]), the fields above but query_offset(s), which count distances, are ignored, and positions are t.
+ *
+ * Everything is on `device`; the plan is overwritten whole by each build, which may be captured into a graph.
+ */
+typedef struct fa_b200_ranges_params {
+    size_t         struct_bytes;       /* = sizeof(fa_b200_ranges_params); checked */
+    void*          plan;               /* output, fa_b200_key_ranges_bytes(B, Nq, Nk) bytes, 16-byte aligned.  It begins with
+                                          the rows: int32 pairs (first, end), Nq rounded up to 128 of them a batch entry */
+    size_t         plan_bytes;
+    int32_t*       positions;          /* optional output, (B, Nq) int32 */
+    const int32_t* rows;               /* optional (B, Nq) pairs, dense */
+    const int32_t* document_offsets;   /* optional, n_documents + 1 a batch entry, offsets_stride_b apart (0: shared) */
+    const int32_t* prefix_lengths;     /* optional, n_documents a batch entry (one without documents); causal only */
+    const int32_t* key_lengths;        /* optional, B */
+    const int32_t* query_offsets;      /* optional, B */
+    int64_t        offsets_stride_b, prefix_stride_b;
+    int32_t        n_documents, query_offset;
+    int32_t        causal, window;     /* window 0: none */
+    int32_t        B, Nq, Nk, device;
+    void*          stream;             /* cudaStream_t */
+} fa_b200_ranges_params;
+
+size_t fa_b200_key_ranges_bytes(int B, int Nq, int Nk);
+int fa_b200_key_ranges(const fa_b200_ranges_params* p);
+
+/*
+ * Attention whose scores are bent, moved or hidden by rule:
+ *   x = cap tanh(scale q.k / cap) - slope_h |position - key|    for the keys of the row's range, -inf elsewhere
+ * with softmax, output, lse and gradients of x.  A row that sees nothing has an output of zeros, an lse of -inf and no
+ * gradient.  Positions are those of the plan's query offsets.  In fa_b200_params causal, causal_shift, bias, kv_lengths,
+ * d_scores, dropout_p and the rng_* fields have to be zero; the plan says what they would.
+ * Keys and values that no row of a call's batch entry sees may hold anything in a forward (an unwritten cache); in a
+ * backward, and where other rows see them, they have to be numbers.
+ * No counterpart in the reference.
+ */
+typedef struct fa_b200_rules {
+    size_t         struct_bytes;       /* = sizeof(fa_b200_rules); checked */
+    const void*    plan;               /* fa_b200_key_ranges' */
+    int32_t        plan_batch;         /* batch entries it was built for: B, or 1 for all */
+    float          score_cap;          /* 0: none */
+    const float*   slopes;             /* optional, H */
+} fa_b200_rules;
+
+/* Forward; scratch as for fa_b200_fwd_with_workspace. */
+int fa_b200_fwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r, void* workspace, size_t workspace_bytes);
+size_t fa_b200_fwd_rules_workspace_bytes(const fa_b200_params* p);
+/* Backward, deterministic; p->workspace holds at least fa_b200_bwd_rules_workspace_bytes(p) bytes. */
+int fa_b200_bwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r);
+size_t fa_b200_bwd_rules_workspace_bytes(const fa_b200_params* p);
+
+/*
+ * Rotary positions: of every head of x, columns are taken in pairs (u, w), the i-th turned by position * inv_freq[i]:
+ *   u' = f (u cos - w sin),  w' = f (w cos + u sin)         f = factor
+ * interleaved: pair i is columns 2i, 2i + 1; else columns i and i + half.  Columns from 2 * half on are copied.
+ * `inverse`: turned back (the gradient of the turn, with the same factor).  One or two (B, N, H, D) tensors a call, for
+ * instance q and k; x and y may be the same memory, not otherwise overlapping.  Angles are reduced in 64 bits.
+ * No counterpart in the reference.
+ */
+typedef struct fa_b200_rotary_params {
+    size_t         struct_bytes;       /* = sizeof(fa_b200_rotary_params); checked */
+    fa_b200_tensor x[2], y[2];         /* x[1].ptr = NULL: one tensor */
+    int32_t        heads[2];
+    const void*    positions;          /* (B, N) int32 or int64, strides in elements (0: shared); NULL: position0 + n */
+    int64_t        positions_stride_b, positions_stride_n;
+    int64_t        position0;
+    const double*  inv_freq;           /* half */
+    int32_t        positions_64bit;
+    int32_t        B, N, D, half;
+    int32_t        interleaved, inverse;
+    float          factor;
+    int32_t        dtype, device;
+    void*          stream;             /* cudaStream_t */
+} fa_b200_rotary_params;
+
+int fa_b200_rotary(const fa_b200_rotary_params* p);
+
 /* Bytes of scratch fa_b200_bwd needs for these sizes (delta, fp32 dQ
  * accumulator, ...).  Counterpart of the 'delta' entry of
  * ops/memory.py:653-760 allocate_attention_workspace_enhanced. */

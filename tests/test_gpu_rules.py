@@ -1,0 +1,299 @@
+"""flash_attention_v100_with_rules against its definition in 64 bits: outputs, log-sum-exps and every gradient, at the tolerances
+of the package's other attention calls (relative L2 2e-3 for fp16 and bf16, 1e-5 for fp32)."""
+import pytest
+import torch
+
+import flash_attention_v100 as fa
+from flash_attention_v100.testing import TOLERANCE
+from rules_helpers import attention64, rel, rotary64, visible
+
+pytestmark = pytest.mark.gpu
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _inputs(B, Nq, Nk, H, Hkv, D, dtype, device, std=1.0, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    q, k, v, d = (torch.randn(B, n, h, D, generator=g) for n, h in ((Nq, H), (Nk, Hkv), (Nk, Hkv), (Nq, H)))
+    return [(t * s).to(dtype).to(device) for t, s in ((q, std), (k, 1.0), (v, 1.0), (d, 1.0))]
+
+
+def _ranges(Nq, Nk, B, host, device):
+    t = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32, device=device)
+    starts = host.get("starts", 0)
+    r = fa.build_key_ranges(Nq, Nk, batch=B, causal=host.get("causal", False), window=host.get("window"), document_offsets=t(host.get("offsets")),
+                            prefix_lengths=t(host.get("prefixes")), key_lengths=t(host.get("lengths")),
+                            query_offsets=t(starts) if isinstance(starts, list) else starts, device=device)
+    see = torch.stack([visible(Nq, Nk, b, **host) for b in range(B)])
+    at = torch.stack([torch.arange(Nq) + (starts[b] if isinstance(starts, list) else starts) for b in range(B)])
+    return r, see, at
+
+
+def _slopes(H, device):
+    return (2.0 ** (-8.0 * torch.arange(1, H + 1) / H)).to(device)
+
+
+def _check(got, want, dtype, names):
+    for n, a, w in zip(names, got, want):
+        assert torch.equal(torch.isfinite(a).cpu(), torch.isfinite(w).cpu()), n
+        fine = torch.isfinite(w)
+        assert rel(a[fine], w[fine]) <= TOLERANCE[dtype], (n, rel(a[fine], w[fine]))
+
+
+def _step(q, k, v, g, **rules):
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    o, lse = fa.flash_attention_v100_with_rules(q, k, v, return_softmax_lse=True, **rules)
+    grads = torch.autograd.grad(o, (q, k, v), g)
+    return (o.detach(), lse.detach()) + grads
+
+
+MASKS = {
+    "none": (200, 300, 2, {}),
+    "causal": (333, 333, 1, dict(causal=True)),
+    "one": (1, 1, 2, dict(causal=True)),
+    "documents": (400, 400, 2, dict(causal=True, offsets=[[0, 1, 130, 131, 390], [7, 7, 7, 300, 400]])),
+    "documents-full": (300, 300, 1, dict(offsets=[[0, 100, 250]])),
+    "prefix": (300, 300, 2, dict(causal=True, offsets=[[0, 140, 300], [0, 10, 200]], prefixes=[[20, 1000], [0, 190]])),
+    "window": (400, 400, 1, dict(causal=True, window=77)),
+    "window-both": (270, 270, 1, dict(window=33)),
+    "lengths": (130, 200, 3, dict(lengths=[0, 200, 77])),
+    "cache": (5, 700, 3, dict(causal=True, lengths=[5, 700, 260], starts=[0, 695, 255])),
+    "far-window": (3, 900, 2, dict(causal=True, window=100, lengths=[900, 850], starts=[897, 847])),
+}
+
+
+@pytest.mark.parametrize("rule", ["ranges", "cap", "slopes", "both"])
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("dtype,H,Hkv,D", [("bf16", 4, 2, 64), ("bf16", 2, 2, 128), ("fp16", 4, 1, 64), ("fp16", 3, 3, 80), ("fp32", 2, 1, 64), ("bf16", 2, 1, 33)])
+def test_step(device, dtype, H, Hkv, D, mask, rule):
+    Nq, Nk, B, host = MASKS[mask]
+    t = TYPES[dtype]
+    q, k, v, g = _inputs(B, Nq, Nk, H, Hkv, D, t, device, std=2.0)
+    ranges, see, at = _ranges(Nq, Nk, B, host, device)
+    cap = 5.0 if rule in ("cap", "both") else None
+    slopes = _slopes(H, device) if rule in ("slopes", "both") else None
+    want = attention64(q, k, v, see, at, D ** -0.5, cap, slopes, grad=g)
+    got = _step(q, k, v, g, score_cap=cap, distance_slopes=slopes, key_ranges=ranges)
+    _check(got, want, t, ("o", "lse", "dq", "dk", "dv"))
+    with torch.no_grad():
+        o, lse = fa.flash_attention_v100_with_rules(q, k, v, score_cap=cap, distance_slopes=slopes, key_ranges=ranges, return_softmax_lse=True)
+    _check((o, lse), want, t, ("o", "lse"))
+    # rows and keys that see nothing or that nobody sees: zeros, not small numbers
+    rows, keys = ~see.any(dim=2), ~see.any(dim=1)
+    assert (got[0].cpu()[rows] == 0).all() and (got[2].cpu()[rows] == 0).all()
+    assert (got[3].cpu()[keys] == 0).all() and (got[4].cpu()[keys] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [0.01, 1.0, 30.0, 1e4])
+@pytest.mark.parametrize("std", [0.01, 3.0, 40.0])
+def test_caps_and_scores_of_any_size(device, dtype, cap, std):
+    """Scores from thousandths of a cap to hundreds of it.  Scores of a spread s give outputs whose distance from the formula
+    grows with s times the score's rounding (2^-24 of a sum of D products whose terms are below 4 s): at most 1e-6 (1 + s)."""
+    t = TYPES[dtype]
+    q, k, v, g = _inputs(1, 200, 200, 2, 2, 64, t, device, std=std)
+    ranges, see, at = _ranges(200, 200, 1, dict(causal=True), device)
+    want = attention64(q, k, v, see, at, 0.125, cap, None, grad=g)
+    got = _step(q, k, v, g, scale=0.125, score_cap=cap, key_ranges=ranges)
+    for n, a, w in zip(("o", "lse", "dv"), (got[0], got[1], got[4]), (want[0], want[1], want[4])):
+        assert rel(a, w) <= TOLERANCE[t] + 1e-6 * (1 + std), (n, rel(a, w))
+    # dQ and dK: in a saturated score (1 - tanh^2) is the difference of 1 and a number rounded to 2^-24; what is left has that
+    # absolute error, so gradients far below the scale |dO| |V| |K| are compared on that scale
+    for n, a, w, x in (("dq", got[2], want[2], k), ("dk", got[3], want[3], q)):
+        scale = 0.125 * 64 * x.double().abs().max().item()
+        assert (a.double() - w).norm() <= (TOLERANCE[t] + 1e-6 * (1 + std)) * w.norm() + 2.0 ** -20 * scale * w.numel() ** 0.5, n
+
+
+def test_without_ranges_the_calls_own_masks(device):
+    """causal, key_lengths and the alignment build the ranges of the call; without any rule the result is the plain call's."""
+    q, k, v, g = _inputs(2, 100, 260, 4, 2, 64, torch.bfloat16, device)
+    for mask, host in [(dict(), {}), (dict(causal=True), dict(causal=True)), (dict(causal=True, causal_alignment="bottom_right"), dict(causal=True, starts=160)),
+                       (dict(key_lengths=torch.tensor([260, 31], device=device)), dict(lengths=[260, 31])),
+                       (dict(causal=True, key_lengths=torch.tensor([90, 31], device=device)), dict(causal=True, lengths=[90, 31]))]:
+        see = torch.stack([visible(100, 260, b, **host) for b in range(2)])
+        at = (torch.arange(100) + host.get("starts", 0)).expand(2, 100)
+        slopes = _slopes(4, device)
+        want = attention64(q, k, v, see, at, 0.125, 9.0, slopes, grad=g)
+        _check(_step(q, k, v, g, score_cap=9.0, distance_slopes=slopes, **mask), want, torch.bfloat16, ("o", "lse", "dq", "dk", "dv"))
+        plain = fa.flash_attention_v100(q, k, v, return_softmax_lse=True, **mask)
+        ruled = fa.flash_attention_v100_with_rules(q, k, v, return_softmax_lse=True, **mask)
+        assert rel(ruled[0], plain[0]) <= 2 * TOLERANCE[torch.bfloat16] and rel(ruled[1], plain[1]) <= 1e-5
+
+
+def test_one_plan_for_any_batch(device):
+    q, k, v, g = _inputs(3, 150, 150, 2, 2, 64, torch.float16, device)
+    host = dict(causal=True, offsets=[0, 60, 150])
+    r = fa.build_key_ranges(150, 150, causal=True, document_offsets=torch.tensor([0, 60, 150], dtype=torch.int32, device=device))
+    see = torch.stack([visible(150, 150, b, **host) for b in range(3)])
+    want = attention64(q, k, v, see, torch.arange(150).expand(3, 150), 0.125, None, _slopes(2, device), grad=g)
+    _check(_step(q, k, v, g, distance_slopes=_slopes(2, device), key_ranges=r), want, torch.float16, ("o", "lse", "dq", "dk", "dv"))
+
+
+def test_rows_of_any_order(device):
+    """Ranges given by hand: neither sorted nor overlapping, whole tiles that see nothing among them."""
+    g0 = torch.Generator().manual_seed(5)
+    first = torch.randint(0, 500, (2, 600), generator=g0)
+    rows = torch.stack([first, first + torch.randint(0, 120, (2, 600), generator=g0)], dim=2)
+    rows[0, 128:256] = 0
+    rows[1, :, 1] = rows[1, :, 1].clamp(max=300)
+    rows[1, 400:] = torch.tensor([250, 251])
+    r = fa.build_key_ranges(600, 512, batch=2, rows=rows.to(torch.int32).to(device))
+    j = torch.arange(512)
+    see = (j >= rows[..., :1]) & (j < rows[..., 1:])
+    for dtype, D in ((torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)):
+        q, k, v, g = _inputs(2, 600, 512, 2, 1, D, dtype, device)
+        want = attention64(q, k, v, see, torch.arange(600).expand(2, 600), D ** -0.5, 8.0, None, grad=g)
+        _check(_step(q, k, v, g, score_cap=8.0, key_ranges=r), want, dtype, ("o", "lse", "dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Nq,H,Hkv,D", [(1, 8, 8, 64), (1, 32, 4, 128), (1, 6, 2, 80), (4, 8, 2, 128), (130, 4, 1, 64), (300, 2, 2, 128)])
+def test_caches_of_ragged_lengths(device, dtype, Nq, H, Hkv, D):
+    """New tokens at the end of caches, what lies behind each cache unwritten memory."""
+    t = TYPES[dtype]
+    lengths = [Nq, 1500, 128 + Nq, 777, 1024]
+    B, Nk = len(lengths), 1500
+    q, k, v, _ = _inputs(B, Nq, Nk, H, Hkv, D, t, device, std=2.0)
+    k2, v2 = k.clone(), v.clone()
+    for b, n in enumerate(lengths):
+        k2[b, n:], v2[b, n:] = float("nan"), float("inf")
+    starts = [n - Nq for n in lengths]
+    for window in (None, 200):
+        ranges, see, at = _ranges(Nq, Nk, B, dict(causal=True, window=window, lengths=lengths, starts=starts), device)
+        slopes = _slopes(H, device)
+        want = attention64(q, k, v, see, at, D ** -0.5, 20.0, slopes)
+        with torch.no_grad():
+            got = fa.flash_attention_v100_with_rules(q, k2, v2, score_cap=20.0, distance_slopes=slopes, key_ranges=ranges, return_softmax_lse=True)
+        _check(got, want, t, ("o", "lse"))
+
+
+def test_bit_reproducible_and_on_another_stream(device):
+    q, k, v, g = _inputs(2, 500, 500, 4, 2, 128, torch.bfloat16, device)
+    ranges, _, _ = _ranges(500, 500, 2, dict(causal=True, offsets=[[0, 200, 500], [0, 1, 480]]), device)
+    rules = dict(score_cap=10.0, distance_slopes=_slopes(4, device), key_ranges=ranges)
+    a = _step(q, k, v, g, **rules)
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(side):
+        b = _step(q, k, v, g, **rules)
+    side.synchronize()
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+
+
+def test_views(device):
+    """Slices of a fused projection, unaligned rows, a head dimension that is not contiguous, an expanded gradient."""
+    ranges, see, at = _ranges(200, 200, 2, dict(causal=True, offsets=[[0, 90, 200], [0, 10, 150]]), device)
+    qkv = torch.randn(2, 200, 8, 64, device=device).bfloat16()
+    g = torch.randn(2, 200, 4, 64, device=device).bfloat16()
+    views = {
+        "fused": (qkv[:, :, :4], qkv[:, :, 4:6], qkv[:, :, 6:]),
+        "odd": tuple(torch.randn(2, 200, h, 65, device=device).bfloat16()[..., 1:] for h in (4, 2, 2)),
+        "permuted": tuple(torch.randn(2, 64, h, 200, device=device).bfloat16().permute(0, 3, 2, 1) for h in (4, 2, 2)),
+    }
+    for name, (q, k, v) in views.items():
+        q, k, v = (x.detach() for x in (q, k, v))
+        want = attention64(q, k, v, see, at, 0.125, 7.0, None, grad=g)
+        _check(_step(q, k, v, g, score_cap=7.0, key_ranges=ranges), want, torch.bfloat16, ("o", "lse", "dq", "dk", "dv"))
+    q = views["fused"][0].detach().requires_grad_(True)
+    o = fa.flash_attention_v100_with_rules(q, k, v, score_cap=7.0, key_ranges=ranges)
+    d, = torch.autograd.grad(o.float().sum(), q)
+    one = torch.ones_like(g)
+    want = attention64(q.detach(), k, v, see, at, 0.125, 7.0, None, grad=one)
+    assert rel(d, want[2]) <= TOLERANCE[torch.bfloat16] * 2       # (dO = 1: dP - delta cancels to a tenth of its terms)
+
+
+def test_no_keys_and_no_queries(device):
+    x = lambda n: torch.randn(2, n, 2, 64, device=device).half().requires_grad_(True)
+    q, k, v = x(5), x(0), x(0)
+    o, lse = fa.flash_attention_v100_with_rules(q, k, v, score_cap=3.0, return_softmax_lse=True)
+    assert (o == 0).all() and (lse == float("-inf")).all()
+    o.sum().backward()
+    assert (q.grad == 0).all() and k.grad.shape == k.shape
+    q, k, v = x(0), x(5), x(5)
+    o = fa.flash_attention_v100_with_rules(q, k, v, causal=True, score_cap=3.0)
+    o.sum().backward()
+    assert o.shape == (2, 0, 2, 64) and (k.grad == 0).all() and (v.grad == 0).all()
+
+
+def test_refusals(device):
+    q = torch.zeros(2, 8, 4, 64, device=device).half()
+    r = fa.build_key_ranges(8, 8, causal=True, device=device)
+    call = fa.flash_attention_v100_with_rules
+    for match, f in [
+        ("positive", lambda: call(q, q, q, score_cap=0.0)), ("positive", lambda: call(q, q, q, score_cap=float("inf"))),
+        ("shape", lambda: call(q, q, q, distance_slopes=torch.ones(3, device=device))),
+        ("same device", lambda: call(q, q, q, distance_slopes=torch.ones(4))),
+        ("no gradient", lambda: call(q, q, q, distance_slopes=torch.ones(4, device=device, requires_grad=True))),
+        ("cannot be combined", lambda: call(q, q, q, causal=True, key_ranges=r)),
+        ("cannot be combined", lambda: call(q, q, q, key_lengths=torch.ones(2, device=device), key_ranges=r)),
+        ("are for", lambda: call(q, q[:, :4], q[:, :4], key_ranges=r)),
+        ("are for", lambda: call(q, q, q, key_ranges=fa.build_key_ranges(8, 8, batch=3, device=device))),
+        ("maximum 128", lambda: call(*(torch.zeros(1, 4, 1, 136, device=device).half(),) * 3, score_cap=1.0)),
+    ]:
+        with pytest.raises(ValueError, match=match):
+            f()
+    with pytest.raises(TypeError):
+        call(q, q, q, key_ranges=torch.zeros(2, 8, 2, device=device))
+
+
+def test_ranges_changed_behind_the_forward_are_noticed(device):
+    q, k, v, g = _inputs(1, 64, 64, 1, 1, 64, torch.float16, device)
+    r = fa.build_key_ranges(64, 64, causal=True, device=device)
+    q.requires_grad_(True)
+    o = fa.flash_attention_v100_with_rules(q, k, v, key_ranges=r)
+    fa.build_key_ranges(64, 64, window=3, device=device, out=r)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.backward(g)
+
+
+def test_a_packed_training_step(device):
+    """The operators together: ranges of packed documents, q and k turned by the positions within them, attention over the
+    ranges, gradients back to q, k and v; every document as if it were alone."""
+    B, N, H, Hkv, D = 2, 300, 4, 2, 64
+    q, k, v, g = _inputs(B, N, N, H, Hkv, D, torch.bfloat16, device)
+    offsets = [[0, 100, 260, 300], [0, 17, 17, 250]]
+    r, see, at = _ranges(N, N, B, dict(causal=True, offsets=offsets), device)
+    f = fa.rotary_frequencies(D, device=device)[0]
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    qr, kr = fa.rotary_embedding(q, k, inv_freq=f, positions=r.positions)
+    o = fa.flash_attention_v100_with_rules(qr, kr, v, score_cap=30.0, key_ranges=r)
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), g)
+    within = r.positions
+    with torch.no_grad():
+        q64, k64 = (rotary64(t, within, f, False) for t in (q, k))
+        want = attention64(q64, k64, v, see, at, D ** -0.5, 30.0, None, grad=g)
+        want = (want[0], rotary64(want[2], within, f, False, inverse=True), rotary64(want[3], within, f, False, inverse=True), want[4])
+    # q and k are rounded to bf16 once more on the way, and so are their gradients: 2^-8 / sqrt(3) each, independent
+    for n, a, w in zip(("o", "dq", "dk", "dv"), (o, dq, dk, dv), want):
+        assert rel(a, w) <= 4 * 2.0 ** -8 / 3 ** 0.5, (n, rel(a, w))
+
+
+def test_a_decoding_step_in_a_graph(device):
+    """Ranges, rotary and attention of one new token, captured once and replayed as the caches grow."""
+    B, Nk, H, Hkv, D = 3, 600, 8, 2, 128
+    q, k, v, _ = _inputs(B, 1, Nk, H, Hkv, D, torch.bfloat16, device)
+    f = fa.rotary_frequencies(D, device=device)[0]
+    lengths = torch.tensor([1, 130, 599], dtype=torch.int32, device=device)
+    slopes = _slopes(H, device)
+
+    def step(r=None):
+        r = fa.build_key_ranges(1, Nk, batch=B, causal=True, key_lengths=lengths, query_offsets=lengths - 1, out=r)
+        qr = fa.rotary_embedding(q, inv_freq=f, positions=r.positions)
+        return r, fa.flash_attention_v100_with_rules(qr, k, v, score_cap=25.0, distance_slopes=slopes, key_ranges=r)
+
+    with torch.no_grad():
+        r, _ = step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            _, o = step(r)
+        for new in ([1, 130, 599], [2, 131, 600], [300, 128, 5]):
+            lengths.copy_(torch.tensor(new, dtype=torch.int32))
+            graph.replay()
+            see = torch.stack([visible(1, Nk, b, causal=True, lengths=new, starts=[n - 1 for n in new]) for b in range(B)])
+            at = torch.tensor(new).view(B, 1) - 1
+            qr = rotary64(q, at.to(device), f, False).to(torch.bfloat16)
+            want = attention64(qr, k, v, see, at, D ** -0.5, 25.0, slopes)[0]
+            assert rel(o, want) <= 2 * TOLERANCE[torch.bfloat16]      # (q's rounding may fall on the other side)
