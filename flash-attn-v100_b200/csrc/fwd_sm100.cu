@@ -45,6 +45,7 @@
 #include "sm100_ptx.cuh"
 #include "tma_host.cuh"
 #include "tile_config.cuh"
+#include "score_rules.cuh"
 #include <type_traits>
 
 namespace fa {
@@ -156,14 +157,18 @@ struct FwdArgs {
     float4* part_o;                // [2 * gridDim.x slots][D / 4][part_rows], sums not yet divided
     float2* part_ml;               // [2 * gridDim.x slots][part_rows]: maximum (log2 units), row sum (< 0: no block visited)
     int4* part_meta;               // [gridDim.x]: batch, column, pair, number of ranges (0: none starts here)
+    // Calls with rules (RULES != 0):
+    Rules rules;
+    float cap_in, cap_out;         // u = S * cap_in, x = tanh(u) * cap_out (log2 units)
+    int cols_per_group;            // whole pairs: (batch, head) columns per group of work items
 };
 
-// A stretch of work: key blocks [j0, j1) of a pair.  n[t]: blocks the pair's tile t has in all
-// (0: no rows); count(t): how many of them lie in this stretch.
+// A stretch of work: key blocks [j0, j1) of a pair.  n[t]: behind the last block of the pair's tile t
+// (0: no rows); count(t): how many of them lie in this stretch.  With rules a pair's blocks begin at jb, not at 0.
 struct Stretch {
-    int pair, h, b, nk, j0, j1, n[2];
+    int pair, h, b, nk, j0, j1, n[2], jb;
     __device__ __forceinline__ int count(int t) const { const int e = n[t] < j1 ? n[t] : j1; return e > j0 ? e - j0 : 0; }
-    __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 >= n[0] && j1 >= n[1]; }
+    __device__ __forceinline__ bool whole() const { return j0 == jb && j1 >= n[0] && j1 >= n[1]; }
 };
 
 // key blocks tile t of a pair of tiles with q_per_tile queries visits
@@ -173,7 +178,56 @@ __device__ __forceinline__ int num_blocks(const FwdArgs& a, int q_per_tile, int 
     if (a.causal && row0 + q_per_tile + a.shift < kv_end) kv_end = row0 + q_per_tile + a.shift;
     return (row0 < a.Nq) ? (kv_end + kBlockN - 1) / kBlockN : 0;
 }
-__device__ __forceinline__ int pair_blocks(const FwdArgs& a, int pair, int nk) {
+// Rules: the keys [x, y) that rows of tile t of a pair see, from the plan's hulls of 128 or (packed tiles) 16 rows.
+__device__ __forceinline__ int2 tile_hull(const FwdArgs& a, int b, int q_per_tile, int pair, int t) {
+    const int row0 = (pair * 2 + t) * q_per_tile;
+    if (row0 >= a.Nq) return make_int2(0, 0);
+    if (q_per_tile == kBlockM) {
+        const int4 h = a.rules.q_tiles[b * a.rules.q_tiles_b + row0 / 128];
+        return make_int2(max(h.x, 0), min(h.y, a.Nk));
+    }
+    const int last = (row0 + q_per_tile < a.Nq ? row0 + q_per_tile : a.Nq) - 1;
+    int2 r = make_int2(0x7fffffff, 0);
+    for (int i = row0 / 16; i <= last / 16; ++i) {
+        const int2 h = a.rules.q_parts[b * a.rules.q_parts_b + i];
+        if (h.y > 0) { r.x = min(r.x, h.x); r.y = max(r.y, h.y); }
+    }
+    return r.y > 0 ? make_int2(max(r.x, 0), min(r.y, a.Nk)) : make_int2(0, 0);
+}
+// A tile whose rows see nothing walks one block, which gives them their zeros.
+__device__ __forceinline__ void ruled_blocks(const FwdArgs& a, int b, int q_per_tile, int pair, int (&n)[2], int& jb) {
+    int lo[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int2 h = tile_hull(a, b, q_per_tile, pair, t);
+        const bool sees = h.y > h.x;
+        lo[t] = sees ? h.x / kBlockN : 0x7fffffff;
+        n[t] = sees ? (h.y + kBlockN - 1) / kBlockN : 0;
+    }
+    jb = min(lo[0], lo[1]);
+    if (jb == 0x7fffffff) jb = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+        if (n[t] == 0 && (pair * 2 + t) * q_per_tile < a.Nq) n[t] = jb + 1;
+}
+template <int RULES>
+__device__ __forceinline__ void stretch_blocks(const FwdArgs& a, int q_per_tile, Stretch& s) {
+    s.jb = 0;
+    if constexpr (RULES != 0) {
+        s.nk = a.Nk;
+        ruled_blocks(a, s.b, q_per_tile, s.pair, s.n, s.jb);
+    } else {
+        s.nk = kv_len_of(a.kv_len, s.b, a.Nk);
+        s.n[0] = num_blocks(a, q_per_tile, s.pair, 0, s.nk); s.n[1] = num_blocks(a, q_per_tile, s.pair, 1, s.nk);
+    }
+}
+template <int RULES>
+__device__ __forceinline__ int pair_blocks(const FwdArgs& a, int b, int pair, int nk) {
+    if constexpr (RULES != 0) {
+        int n[2], jb;
+        ruled_blocks(a, b, a.q_per_tile, pair, n, jb);
+        return (n[0] > n[1] ? n[0] : n[1]) - jb;
+    }
     const int n0 = num_blocks(a, a.q_per_tile, pair, 0, nk), n1 = num_blocks(a, a.q_per_tile, pair, 1, nk);
     return n0 > n1 ? n0 : n1;
 }
@@ -210,28 +264,28 @@ __device__ __forceinline__ int warp_find(int n, int lane, int& target, Cost cost
 template <int SCHED> __device__ __forceinline__ int start_cost(const FwdArgs& a) { return SCHED == 2 ? a.start_cost : 0; }
 template <int SCHED>
 __device__ __forceinline__ int take_units(const FwdArgs& a, int at, int units, Stretch& s) {
-    const int n = s.n[0] > s.n[1] ? s.n[0] : s.n[1], c0 = start_cost<SCHED>(a);
-    s.j0 = max(at - c0, 0);
-    s.j1 = min(n, at + units - c0);
+    const int n = (s.n[0] > s.n[1] ? s.n[0] : s.n[1]) - s.jb, c0 = start_cost<SCHED>(a);
+    s.j0 = s.jb + max(at - c0, 0);
+    s.j1 = s.jb + min(n, at + units - c0);
     const int left = at + units - c0 - n;
     return left > c0 ? left : 0;
 }
 // One warp: the costs are the pairs' units; with per-batch key counts a batch entry has a total of its own.
-template <int SCHED>
+template <int SCHED, int RULES>
 __device__ __forceinline__ void find_range(const FwdArgs& a, int lane, volatile RangeStart* out) {
     const int c0 = start_cost<SCHED>(a);
     auto column = [&](int b) {                       // units of one (batch, column): serial, every lane its own b
         const int nk = kv_len_of(a.kv_len, b, a.Nk);
         int sum = 0;
-        for (int pr = 0; pr < a.n_pairs; ++pr) sum += pair_blocks(a, pr, nk) + c0;
+        for (int pr = 0; pr < a.n_pairs; ++pr) sum += pair_blocks<RULES>(a, b, pr, nk) + c0;
         return sum;
     };
     int total = 0, col = 0;
-    if (a.kv_len) {
+    if (RULES || a.kv_len) {
         for (int b = lane; b < a.B; b += 32) total += a.heads * column(b);
         total = __shfl_sync(0xffffffffu, warp_scan(total, lane), 31);
     } else {
-        for (int pr = lane; pr < a.n_pairs; pr += 32) col += pair_blocks(a, pr, a.Nk) + c0;
+        for (int pr = lane; pr < a.n_pairs; pr += 32) col += pair_blocks<RULES>(a, 0, pr, a.Nk) + c0;
         col = __shfl_sync(0xffffffffu, warp_scan(col, lane), 31);
         total = a.B * a.heads * col;
     }
@@ -240,7 +294,7 @@ __device__ __forceinline__ void find_range(const FwdArgs& a, int lane, volatile 
     const int first = range_begin((int)blockIdx.x, ctas, total);
     const int units = range_begin((int)blockIdx.x + 1, ctas, total) - first;
     int at = first, b;
-    if (a.kv_len) {
+    if (RULES || a.kv_len) {
         b = warp_find(a.B, lane, at, [&](int i) { return a.heads * column(i); });
         col = column(b);
     } else {
@@ -250,18 +304,18 @@ __device__ __forceinline__ void find_range(const FwdArgs& a, int lane, volatile 
     const int h = at / col;
     at -= h * col;
     const int nk = kv_len_of(a.kv_len, b, a.Nk);
-    const int pair = warp_find(a.n_pairs, lane, at, [&](int i) { return pair_blocks(a, i, nk) + c0; });
+    const int pair = warp_find(a.n_pairs, lane, at, [&](int i) { return pair_blocks<RULES>(a, b, i, nk) + c0; });
     if (lane == 0) {
         out->b = b; out->h = h; out->pair = pair; out->at = at; out->units = at + units > c0 ? units : 0; out->total = total; out->ctas = ctas;
     }
 }
 
 // A role's walk over the CTA's work; every role runs one of its own and sees the same stretches:
-//     for (WorkLoop<SCHED> wl(a, range); wl.more(a); wl.advance()) for (u = 0; u < wl.kSub; ++u) if (wl.get(a, u, st)) ...
+//     for (WorkLoop<SCHED, RULES> wl(a, range); wl.more(a); wl.advance()) for (u = 0; u < wl.kSub; ++u) if (wl.get(a, u, st)) ...
 // Two walks and not one with a switch, because the softmax threads have no register to spare: one walk for
 // both made the kernel of whole pairs spill more and cost it 1-2 % (B4 N4096 H32 D128).
-template <int SCHED> struct WorkLoop;
-template <> struct WorkLoop<0> {       // whole pairs, round robin
+template <int SCHED, int RULES> struct WorkLoop;
+template <> struct WorkLoop<0, 0> {       // whole pairs, round robin
     static constexpr int kSub = 2;     // causal: a pair and its mirror
     int w;
     __device__ __forceinline__ WorkLoop(const FwdArgs&, const volatile RangeStart*) : w(blockIdx.x) {}
@@ -281,14 +335,35 @@ template <> struct WorkLoop<0> {       // whole pairs, round robin
         s.pair = pair;
         s.h = bh % a.H;
         s.b = bh / a.H;
-        s.nk = kv_len_of(a.kv_len, s.b, a.Nk);
-        s.n[0] = num_blocks(a, kBlockM, pair, 0, s.nk); s.n[1] = num_blocks(a, kBlockM, pair, 1, s.nk);
+        stretch_blocks<0>(a, kBlockM, s);
         s.j0 = 0;
         s.j1 = s.n[0] > s.n[1] ? s.n[0] : s.n[1];
         return true;
     }
 };
-template <int SCHED> struct WorkLoop {       // split schedule: the CTA's range of units
+// Whole pairs with rules: what a pair costs is on the device.  In groups of columns whose K and V stay in L2, the last pair of
+// all columns first, which under a causal mask is the longest, then the one before it.
+template <int RULES> struct WorkLoop<0, RULES> {
+    static constexpr int kSub = 1;
+    int w;
+    __device__ __forceinline__ WorkLoop(const FwdArgs&, const volatile RangeStart*) : w(blockIdx.x) {}
+    __device__ __forceinline__ bool more(const FwdArgs& a) const { return w < a.n_items; }
+    __device__ __forceinline__ void advance() { w += gridDim.x; }
+    __device__ __forceinline__ bool get(const FwdArgs& a, int, Stretch& s) const {
+        const int cols = a.B * a.H, per_group = a.cols_per_group * a.n_pairs;
+        const int group = w / per_group, at = w - group * per_group;
+        const int here = min(a.cols_per_group, cols - group * a.cols_per_group);
+        const int col = group * a.cols_per_group + at % here;
+        s.pair = a.n_pairs - 1 - at / here;
+        s.h = col % a.H;
+        s.b = col / a.H;
+        stretch_blocks<RULES>(a, kBlockM, s);
+        s.j0 = s.jb;
+        s.j1 = s.n[0] > s.n[1] ? s.n[0] : s.n[1];
+        return true;
+    }
+};
+template <int SCHED, int RULES> struct WorkLoop {       // split schedule: the CTA's range of units
     static constexpr int kSub = 1;
     int b, h, pair, at, units;
     __device__ __forceinline__ WorkLoop(const FwdArgs&, const volatile RangeStart* r)
@@ -297,8 +372,7 @@ template <int SCHED> struct WorkLoop {       // split schedule: the CTA's range 
     __device__ __forceinline__ void advance() {}
     __device__ __forceinline__ bool get(const FwdArgs& a, int, Stretch& s) {
         s.pair = pair; s.h = h; s.b = b;
-        s.nk = kv_len_of(a.kv_len, b, a.Nk);
-        s.n[0] = num_blocks(a, a.q_per_tile, pair, 0, s.nk); s.n[1] = num_blocks(a, a.q_per_tile, pair, 1, s.nk);
+        stretch_blocks<RULES>(a, a.q_per_tile, s);
         units = take_units<SCHED>(a, at, units, s);
         at = 0;
         if (++pair == a.n_pairs) { pair = 0; if (++h == a.heads) { h = 0; ++b; } }
@@ -310,12 +384,12 @@ template <int SCHED> struct WorkLoop {       // split schedule: the CTA's range 
 // the epilogue reads the stretch again, so that no register holds them while a block's 128 scores are worked on.
 // Held in registers, the D = 128 kernel spilled 424 bytes instead of 60 and the chunk below took 152 us instead of 112.
 struct WalkRecord { int b, h, pair, at, units, cur_pair, cur_h, cur_b, cur_j0, cur_j1; };
-template <int SCHED> struct SoftmaxLoop;
-template <> struct SoftmaxLoop<0> : WorkLoop<0> {
-    __device__ __forceinline__ SoftmaxLoop(const FwdArgs& a, const volatile RangeStart* r, volatile WalkRecord*) : WorkLoop<0>(a, r) {}
+template <int SCHED, int RULES> struct SoftmaxLoop;
+template <int RULES> struct SoftmaxLoop<0, RULES> : WorkLoop<0, RULES> {
+    __device__ __forceinline__ SoftmaxLoop(const FwdArgs& a, const volatile RangeStart* r, volatile WalkRecord*) : WorkLoop<0, RULES>(a, r) {}
     __device__ __forceinline__ void again(const FwdArgs&, Stretch&) const {}
 };
-template <int SCHED> struct SoftmaxLoop {
+template <int SCHED, int RULES> struct SoftmaxLoop {
     static constexpr int kSub = 1;
     volatile WalkRecord* rec;
     __device__ __forceinline__ SoftmaxLoop(const FwdArgs&, const volatile RangeStart* r, volatile WalkRecord* w) : rec(w) {
@@ -328,8 +402,7 @@ template <int SCHED> struct SoftmaxLoop {
         int b = rec->b, h = rec->h, pair = rec->pair;
         const int at = rec->at, units = rec->units;
         s.pair = pair; s.h = h; s.b = b;
-        s.nk = kv_len_of(a.kv_len, b, a.Nk);
-        s.n[0] = num_blocks(a, a.q_per_tile, pair, 0, s.nk); s.n[1] = num_blocks(a, a.q_per_tile, pair, 1, s.nk);
+        stretch_blocks<RULES>(a, a.q_per_tile, s);
         const int left = take_units<SCHED>(a, at, units, s);
         if (++pair == a.n_pairs) { pair = 0; if (++h == a.heads) { h = 0; ++b; } }
         __syncwarp();                                  // every lane has read
@@ -340,8 +413,7 @@ template <int SCHED> struct SoftmaxLoop {
     }
     __device__ __forceinline__ void again(const FwdArgs& a, Stretch& s) const {
         s.pair = rec->cur_pair; s.h = rec->cur_h; s.b = rec->cur_b; s.j0 = rec->cur_j0; s.j1 = rec->cur_j1;
-        s.nk = kv_len_of(a.kv_len, s.b, a.Nk);
-        s.n[0] = num_blocks(a, a.q_per_tile, s.pair, 0, s.nk); s.n[1] = num_blocks(a, a.q_per_tile, s.pair, 1, s.nk);
+        stretch_blocks<RULES>(a, a.q_per_tile, s);
     }
 };
 
@@ -356,12 +428,19 @@ __device__ __noinline__ float exact_log(float x) { return (float)log((double)x);
 // DROP: 0 no dropout; 1 the keep bits are drawn here, by the softmax threads (no workspace);
 // 2 they are loaded from the workspace, where dropout_bits_kernel has written the call's bits.
 // SCHED: see FwdCfg.
-template <int D, bool BF16, int DROP, int PREC, int SCHED>
+// RULES: 0 none; calls with rules (fa_b200_rules): 1 ranges and distances, 2 a score cap as well.  As PREC = 0, with any head
+// size that is a multiple of 8 as in the pair instances.  A score becomes x, in log2 units, where the others have the raw
+// product: the cap's tanh in place (score_rules.cuh), the distance behind it, -inf outside the row's range.  Rows of V that
+// no row of the pair sees are set to zeros in shared memory by warps 10-11, because 0 times unwritten memory is no zero.
+template <int D, bool BF16, int DROP, int PREC, int SCHED, int RULES = 0>
 __global__ void __launch_bounds__(kThreads, 1)
 fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_bias, const FwdArgs a) {
     using Cfg = FwdCfg<D, PREC, SCHED>;
     constexpr bool FREE = SCHED != 0, TWIN = SCHED == 2;
+    constexpr bool RULED = RULES != 0, ANY_D = PREC != 0 || RULED;
+    constexpr bool NOTHING = FREE || RULED;     // a row may have seen nothing yet
+    static_assert(!RULED || (PREC == 0 && DROP == 0), "rules come without bias and dropout");
     constexpr int ST = Cfg::kStages;
     constexpr int TILE = Cfg::kTileBytes;
     // tcgen05.mma kind::f16 wants A and B in one format (an fp16 A next to a bf16 B raises an
@@ -369,6 +448,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     // With P as a pair (PREC = 1) P_hi + P_lo come in V's own format and nothing is converted.
     constexpr bool CONV = BF16 && PREC == 0;
     constexpr bool P_BF16 = BF16 && PREC != 0;
+    constexpr bool V_PASS = CONV || RULED;      // warps 10-11 pass each V tile on
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -404,7 +484,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         prefetch_tensormap(&map_k);
         prefetch_tensormap(&map_v);
     }
-    if (FREE && warp == 11) find_range<SCHED>(a, lane, range);
+    if (FREE && warp == 11) find_range<SCHED, RULES>(a, lane, range);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
@@ -421,7 +501,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             int q_loads[2] = {0, 0};
             bool ok = true;
             const uint32_t q_bytes = FREE ? (uint32_t)(Cfg::kNBox * 128 * pack * q_per_tile) : TILE;
-            for (WorkLoop<SCHED> wl(a, range); wl.more(a) && ok; wl.advance()) {
+            for (WorkLoop<SCHED, RULES> wl(a, range); wl.more(a) && ok; wl.advance()) {
                 for (int u = 0; u < wl.kSub && ok; ++u) {
                     Stretch st;
                     if (!wl.get(a, u, st)) continue;
@@ -485,7 +565,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (elect_one()) {
             constexpr uint32_t idesc_s = make_idesc_f16(BF16, BF16, kBlockM, kBlockN, false, false);
             // P, V: fp16, or as a pair the inputs' format and the head size in whole groups of 16 columns
-            const uint32_t idesc_pv = PREC ? make_idesc_f16(P_BF16, P_BF16, kBlockM, (a.d + 15) & ~15, false, true)
+            const uint32_t idesc_pv = ANY_D ? make_idesc_f16(P_BF16, P_BF16, kBlockM, (a.d + 15) & ~15, false, true)
                                            : make_idesc_f16(false, false, kBlockM, D, false, true);
             const uint32_t sQ_u = smem_u32(sQ), sK_u = smem_u32(sK), sV_u = smem_u32(sV);
 
@@ -501,7 +581,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     const uint32_t off = ((uint32_t)(kk >> 2) * kBoxBytes + (uint32_t)(kk & 3) * 32u) >> 4;
-                    if (PREC == 0 || kk * 16 < a.d) mma_ss_f16(d, a0 + off, b0 + off, idesc_s, kk > 0);
+                    if (!ANY_D || kk * 16 < a.d) mma_ss_f16(d, a0 + off, b0 + off, idesc_s, kk > 0);
                 }
             };
             // one 64-key half (hf = 0, 1) of O_t += P_t V_j
@@ -527,7 +607,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             int q_uses[2] = {0, 0};         // pairs that used tile t (Q_full phase)
             int p_waits[2] = {0, 0};        // P_t hand-offs so far (P_full phase)
             bool ok = true;
-            for (WorkLoop<SCHED> wl(a, range); TWIN && wl.more(a) && ok; wl.advance()) {
+            for (WorkLoop<SCHED, RULES> wl(a, range); TWIN && wl.more(a) && ok; wl.advance()) {
                 Stretch st;
                 wl.get(a, 0, st);
                 // one tile: block j of the stretch belongs to accumulator set j & 1
@@ -543,7 +623,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
                         const uint32_t off = ((uint32_t)(kk >> 2) * kBoxBytes + (uint32_t)(kk & 3) * 32u) >> 4;
-                        mma_ss_f16(d, dQ + off, b0 + off, idesc_s, kk > 0);
+                        if (!RULED || kk * 16 < a.d) mma_ss_f16(d, dQ + off, b0 + off, idesc_s, kk > 0);
                     }
                     mma_commit(&bars[Cfg::kSFull + (j & 1)]);
                     mma_commit(&bars[Cfg::kKEmpty + c % ST]);
@@ -554,7 +634,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 if (ok && nb > 1) ok = s_block(1);
                 for (int j = 0; j < nb && ok; ++j) {
                     const int t = j & 1, c = kvc + j, vs = c % ST;
-                    ok = mbar_wait(&bars[(CONV ? Cfg::kVConv : Cfg::kVFull) + vs], (uint32_t)(c / ST) & 1u, abort_flag);
+                    ok = mbar_wait(&bars[(V_PASS ? Cfg::kVConv : Cfg::kVFull) + vs], (uint32_t)(c / ST) & 1u, abort_flag);
                     if (ok) ok = mbar_wait(&bars[Cfg::kPHalf + t], (uint32_t)p_waits[t] & 1u, abort_flag);
                     if (!ok) break;
                     tc_fence_after_sync();
@@ -570,7 +650,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
                 kvc += nb;
             }
-            for (WorkLoop<SCHED> wl(a, range); !TWIN && wl.more(a) && ok; wl.advance()) {
+            for (WorkLoop<SCHED, RULES> wl(a, range); !TWIN && wl.more(a) && ok; wl.advance()) {
                 for (int u = 0; u < wl.kSub && ok; ++u) {
                     Stretch st;
                     if (!wl.get(a, u, st)) continue;
@@ -600,7 +680,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         const int ks = (kvc + j + 1) % ST;
                         const uint32_t kph = (uint32_t)((kvc + j + 1) / ST) & 1u;
                         bool k_ready = false;
-                        ok = mbar_wait(&bars[(CONV ? Cfg::kVConv : Cfg::kVFull) + vs], vph, abort_flag);
+                        ok = mbar_wait(&bars[(V_PASS ? Cfg::kVConv : Cfg::kVFull) + vs], vph, abort_flag);
                         if (!ok) break;
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
@@ -637,23 +717,35 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
         }
         __syncwarp();
-      } else if (CONV) {
-        // ------------------------------------------------------------ warps 10-11: V_j bf16 -> fp16
+      } else if (V_PASS) {
+        // ------------------------------------------------------------ warps 10-11: V_j bf16 -> fp16; rules: unseen rows to zeros
         // the same walk as the producer's; a tile is touched between its arrival (V_full) and its
         // first reader (the PV MMAs wait for V_conv instead of V_full)
         const int ct = (warp - 10) * 32 + lane;
         int kvc = 0;
         bool ok = true;
-        for (WorkLoop<SCHED> wl(a, range); wl.more(a) && ok; wl.advance()) {
+        for (WorkLoop<SCHED, RULES> wl(a, range); wl.more(a) && ok; wl.advance()) {
             for (int u = 0; u < wl.kSub && ok; ++u) {
                 Stretch st;
                 if (!wl.get(a, u, st)) continue;
+                int2 seen = make_int2(0, 0);                // keys that rows of the pair see
+                if constexpr (RULED) {
+                    const int2 h0 = tile_hull(a, st.b, q_per_tile, st.pair, 0), h1 = tile_hull(a, st.b, q_per_tile, st.pair, 1);
+                    seen = h0.y == 0 ? h1 : (h1.y == 0 ? h0 : make_int2(min(h0.x, h1.x), max(h0.y, h1.y)));
+                }
                 for (int j = st.j0; j < st.j1; ++j, ++kvc) {
                     const int sidx = kvc % ST;
                     ok = mbar_wait(&bars[Cfg::kVFull + sidx], (uint32_t)(kvc / ST) & 1u, abort_flag);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    convert_tile_bf16_to_f16<false>(sV + sidx * TILE, TILE, ct, 64, 1.f);
+                    if constexpr (CONV) convert_tile_bf16_to_f16<false>(sV + sidx * TILE, TILE, ct, 64, 1.f);
+                    if (RULED && (j * kBlockN < seen.x || j * kBlockN + kBlockN > seen.y)) {
+                        // (the pieces a thread has converted are its own to clear)
+                        for (int at = ct; at < TILE / 16; at += 64) {
+                            const int key = j * kBlockN + ((at >> 3) & (kBlockN - 1));
+                            if (key < seen.x || key >= seen.y) *reinterpret_cast<uint4*>(sV + sidx * TILE + at * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    }
                     fence_proxy_async_smem();           // generic-proxy writes -> visible to the MMA's reads
                     mbar_arrive_warp(&bars[Cfg::kVConv + sidx]);
                 }
@@ -667,7 +759,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             int slot = 0, done = 0;
             uint32_t ph = 1u;                   // the slots start empty
             bool ok = true;
-            for (WorkLoop<SCHED> wl(a, range); wl.more(a) && ok; wl.advance()) {
+            for (WorkLoop<SCHED, RULES> wl(a, range); wl.more(a) && ok; wl.advance()) {
                 for (int u = 0; u < wl.kSub && ok; ++u) {
                     Stretch st;
                     if (!wl.get(a, u, st)) continue;
@@ -710,7 +802,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         bool ok = true;
 
         if (FREE && threadIdx.x == 0) a.part_meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-        for (SoftmaxLoop<SCHED> wl(a, range, walk); wl.more(a) && ok; wl.advance()) {
+        for (SoftmaxLoop<SCHED, RULES> wl(a, range, walk); wl.more(a) && ok; wl.advance()) {
             for (int u = 0; u < wl.kSub && ok; ++u) {
                 Stretch st;
                 if (!wl.get(a, u, st)) continue;
@@ -724,9 +816,9 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 auto row_ok = [&] { return i < a.Nq && (!FREE || r < pack * q_per_tile); };
                 if (FREE && !st.whole()) {
                     // the slot my row's partial goes to: a range's first stretch takes slot 0 unless it starts a pair
-                    const int64_t slot = 2 * (int64_t)blockIdx.x + (st.j0 == 0 ? 1 : 0);
+                    const int64_t slot = 2 * (int64_t)blockIdx.x + (st.j0 == st.jb ? 1 : 0);
                     if (!TWIN && n == st.j0 && row_ok()) a.part_ml[slot * a.part_rows + t * kBlockM + r] = make_float2(-INFINITY, -1.f);
-                    if (threadIdx.x == 0 && st.j0 == 0) {
+                    if (threadIdx.x == 0 && st.j0 == st.jb) {
                         // the pair starts here and goes on in the ranges of the CTAs behind this one
                         const int total = range->total, ctas = range->ctas;
                         const int full = st.n[0] > st.n[1] ? st.n[0] : st.n[1];
@@ -742,6 +834,17 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 const bool idle = TWIN && __all_sync(0xffffffffu, !row_ok());
                 const uint32_t bh = dropout_column(a.rng, st.b, h);
                 float m = -INFINITY, l = 0.f;
+                // rules: my row's keys and position, and what a key's distance takes off in log2 units
+                [[maybe_unused]] int2 keys = make_int2(0, 0);
+                [[maybe_unused]] int at = 0;
+                [[maybe_unused]] float slope = 0.f;
+                if constexpr (RULED) {
+                    if (row_ok()) {
+                        keys = a.rules.rows[st.b * a.rules.rows_b + i];
+                        if (a.rules.slopes) slope = a.rules.slopes[h] * kLog2e;
+                    }
+                    at = i + a.rules.origin[st.b * a.rules.origin_b];
+                }
                 // my row of the bias (a row beyond Nq, whose results nobody keeps, reads the last one)
                 const float* brow = nullptr;
                 if (PREC == 1 && a.bias)
@@ -815,7 +918,68 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         }
                     }
                     if (PREC == 2 && !ok) break;
-                    const bool need_mask = (a.causal && col0 + kBlockN - 1 > tile * q_per_tile + a.shift) || (col0 + kBlockN > nk);
+                    if constexpr (RULES == 2) {
+                        // u = S scale / cap, tanh(u) in its place
+                        const uint64_t in2 = f2_pack(a.cap_in, a.cap_in);
+                        float z0 = 0.f, z1 = 0.f;
+#pragma unroll
+                        for (int c = 0; c < 128; c += 4) {
+                            const uint64_t ua = f2_mul(f2_pack(SF(c), SF(c + 1)), in2), ub = f2_mul(f2_pack(SF(c + 2), SF(c + 3)), in2);
+                            const uint64_t za = f2_mul(ua, ua), zb = f2_mul(ub, ub);
+                            float x0, x1, x2, x3;
+                            f2_unpack(za, x0, x1);
+                            f2_unpack(zb, x2, x3);
+                            z0 = max3(z0, x0, x1);
+                            z1 = max3(z1, x2, x3);
+                            f2_unpack(f2_tanh_poly(ua, za), x0, x1);
+                            f2_unpack(f2_tanh_poly(ub, zb), x2, x3);
+                            SSET(c, x0); SSET(c + 1, x1); SSET(c + 2, x2); SSET(c + 3, x3);
+                        }
+                        if (__any_sync(0xffffffffu, fmaxf(z0, z1) > kTanhPolyMax * kTanhPolyMax)) {
+                            // some score beyond the polynomial: the block's scores again
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) tmem_ld_32x32(tS + c * 32, sr[c]);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int c = 0; c < 128; ++c) SSET(c, tanh_any(SF(c) * a.cap_in));
+                        }
+                    }
+                    if constexpr (RULED) {
+                        if (a.rules.slopes) {
+                            // x = S scale - slope |position - key|, whole numbers that fp32 holds exactly up to 2^24
+                            const float from = (float)(at - col0), mul = RULES == 2 ? a.cap_out : a.scale_log2;
+                            const uint64_t mul2 = f2_pack(mul, mul), step2 = f2_pack(-2.f, -2.f);
+                            uint64_t d2 = f2_pack(from, from - 1.f);
+                            if (__any_sync(0xffffffffu, at < min(col0 + kBlockN, keys.y) - 1)) {        // keys ahead of a row
+#pragma unroll
+                                for (int c = 0; c < 128; c += 2) {
+                                    float d0, d1, x0, x1;
+                                    f2_unpack(d2, d0, d1);
+                                    f2_unpack(f2_mul(f2_pack(SF(c), SF(c + 1)), mul2), x0, x1);
+                                    SSET(c, fmaf(-slope, fabsf(d0), x0));
+                                    SSET(c + 1, fmaf(-slope, fabsf(d1), x1));
+                                    d2 = f2_add(d2, step2);
+                                }
+                            } else {
+                                const uint64_t slope2 = f2_pack(-slope, -slope);
+#pragma unroll
+                                for (int c = 0; c < 128; c += 2) {
+                                    float x0, x1;
+                                    f2_unpack(f2_fma(d2, slope2, f2_mul(f2_pack(SF(c), SF(c + 1)), mul2)), x0, x1);
+                                    SSET(c, x0);
+                                    SSET(c + 1, x1);
+                                    d2 = f2_add(d2, step2);
+                                }
+                            }
+                        }
+                        const int lo = keys.x - col0, hi = keys.y - col0;             // the columns my row sees
+                        if (__any_sync(0xffffffffu, lo > 0 || hi < kBlockN)) {
+#pragma unroll
+                            for (int c = 0; c < 128; ++c)
+                                if (c < lo || c >= hi) SSET(c, -INFINITY);
+                        }
+                    }
+                    const bool need_mask = !RULED && ((a.causal && col0 + kBlockN - 1 > tile * q_per_tile + a.shift) || (col0 + kBlockN > nk));
                     if (need_mask) {
                         // my row sees the block's first `seen` columns: keys below the count, at most i + shift
                         int seen = nk - col0;
@@ -831,13 +995,14 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         if (c + 4 < 128) { mx2 = max3(mx2, SF(c + 4), SF(c + 5)); mx3 = max3(mx3, SF(c + 6), SF(c + 7)); }
                     }
                     // with a bias the scores are x already, without one x = S scale is left to the FMA that takes the maximum off
-                    const float to_x = PREC == 0 ? a.scale_log2 : (PREC == 1 && !a.bias ? a.scale : 1.f);
+                    const float to_x = RULED ? (a.rules.slopes ? 1.f : (RULES == 2 ? a.cap_out : a.scale_log2)) :
+                                       PREC == 0 ? a.scale_log2 : (PREC == 1 && !a.bias ? a.scale : 1.f);
                     const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * to_x;
                     const float m_new = fmaxf(m, mx);
                     const bool grow = (m_new - m) > (PREC ? kRescaleThreshold * kLn2 : kRescaleThreshold);   // first block: inf > 8
                     if (__any_sync(0xffffffffu, grow)) {
                         // 0 on the first block; a row may have seen nothing but -inf so far (a bias; a stretch of a pair)
-                        const float alpha = ((PREC || FREE) && m_new == -INFINITY) ? 0.f : ex2(PREC ? (m - m_new) * kLog2e : m - m_new);
+                        const float alpha = ((PREC || NOTHING) && m_new == -INFINITY) ? 0.f : ex2(PREC ? (m - m_new) * kLog2e : m - m_new);
                         m = m_new;
                         l *= alpha;
                         if (j > first) {
@@ -906,8 +1071,8 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     // dropout P is packed to 16 bits as it is produced and each 64-key half is
                     // stored to TMEM as soon as it is complete, so conversion and store latency
                     // overlap the exponentials of the other half.
-                    const float ms = kPShift - (FREE && m == -INFINITY ? 0.f : m);     // nothing seen yet: P = 0
-                    const uint64_t c2 = f2_pack(a.scale_log2, a.scale_log2), nm2 = f2_pack(ms, ms);
+                    const float ms = kPShift - (NOTHING && m == -INFINITY ? 0.f : m);     // nothing seen yet: P = 0
+                    const uint64_t c2 = RULED ? f2_pack(to_x, to_x) : f2_pack(a.scale_log2, a.scale_log2), nm2 = f2_pack(ms, ms);
                     uint32_t pk[32];
 #pragma unroll
                     for (int c = 0; c < 128; c += 4) {
@@ -1036,7 +1201,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 };
                 if (FREE && !st.whole()) {
                     // a part of the pair's keys: the sums as they are, four columns of neighbouring rows side by side
-                    const int64_t slot = 2 * (int64_t)blockIdx.x + (st.j0 == 0 ? 1 : 0);
+                    const int64_t slot = 2 * (int64_t)blockIdx.x + (st.j0 == st.jb ? 1 : 0);
                     const int pr = t * kBlockM + r;
                     if (row_ok()) a.part_ml[slot * a.part_rows + pr] = make_float2(m, l);
                     float4* po = a.part_o + slot * (int64_t)(D / 4) * a.part_rows + pr;
@@ -1054,7 +1219,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     }
                     continue;
                 }
-                const float inv = a.inv_keep / l;
+                const float inv = RULED && m == -INFINITY ? 0.f : a.inv_keep / l;       // (0: a row that sees nothing)
                 T16* orow = reinterpret_cast<T16*>(a.o) + (int64_t)st.b * a.o_sb + (int64_t)i * a.o_sn +
                             (int64_t)h * a.o_sh;
                 T16* lrow = a.o_lo ? reinterpret_cast<T16*>(a.o_lo) + (int64_t)st.b * a.l_sb + (int64_t)i * a.l_sn +
@@ -1066,7 +1231,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     if (row_ok()) {
 #pragma unroll
                         for (int g = 0; g < 4; ++g) {
-                            if (PREC != 0 && c0 + g * 8 >= a.d) break;
+                            if (ANY_D && c0 + g * 8 >= a.d) break;
                             uint4 v4;
                             v4.x = pack2<BF16>(__uint_as_float(orr[g * 8 + 0]) * inv, __uint_as_float(orr[g * 8 + 1]) * inv);
                             v4.y = pack2<BF16>(__uint_as_float(orr[g * 8 + 2]) * inv, __uint_as_float(orr[g * 8 + 3]) * inv);
@@ -1110,7 +1275,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 // cut has two parts at least, and where those lie does not depend on which pair it is, so the first two parts' rows are
 // under way together with the record that says so (one bf16 query for each of 32 sequences of up to 4096 keys, 32 heads on 8:
 // 11.3 -> 9.4 us, the call 82.1 -> 79.7; 700 queries on 8892 keys: 15.4 -> 13.9, 108.7 -> 107.7).
-template <int D, bool BF16>
+template <int D, bool BF16, bool RULED = false>
 __global__ void __launch_bounds__(256) fwd_merge_kernel(const FwdArgs a) {
     using T16 = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     grid_dependency_wait();
@@ -1167,12 +1332,13 @@ __global__ void __launch_bounds__(256) fwd_merge_kernel(const FwdArgs a) {
         const float4* po = a.part_o + slot * (int64_t)(D / 4) * a.part_rows + rr;
         add(a.part_ml[slot * a.part_rows + rr], [&](int g, int y) { return po[(int64_t)((g * 8 + warp) * 2 + y) * a.part_rows]; });
     }
-    const float inv = a.inv_keep / l;
+    const float inv = RULED && m == -INFINITY ? 0.f : a.inv_keep / l;
     T16* orow = reinterpret_cast<T16*>(a.o) + (int64_t)b * a.o_sb + (int64_t)i * a.o_sn + (int64_t)h * a.o_sh;
     T16* lrow = a.o_lo ? reinterpret_cast<T16*>(a.o_lo) + (int64_t)b * a.l_sb + (int64_t)i * a.l_sn + (int64_t)h * a.l_sh : nullptr;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
         const int c0 = (g * 8 + warp) * 8;
+        if (RULED && c0 >= a.d) break;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -1238,7 +1404,7 @@ constexpr int kMergeUnits = 4;
 // of 2048-4096 keys, H32 Hkv8 D128 84 -> 82.  Without counts pairs are alike, and in the kernel of several tiles the
 // walk with starts took registers from the softmax (700 queries on 8892 keys 93 -> 100 us).
 constexpr int kLongRange = 8;
-FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free) {
+FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, bool ruled = false) {
     FwdPlan pl;
     memset(&pl, 0, sizeof(pl));
     auto pairs_of = [&](int qpt) { return (int)(((int64_t)p.Nq + 2 * qpt - 1) / (2 * qpt)); };
@@ -1257,11 +1423,11 @@ FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free) {
     const int64_t total = (int64_t)p.B * pl.heads * col;
     pl.ctas = (int)(total < sms ? total : sms);
     int64_t ranges = (total + pl.ctas - 1) / pl.ctas;
-    const bool one_tile = p.Nq <= pl.q_per_tile;
-    if (p.kv_lengths && one_tile) ranges = (3 * ranges + 3) / 4;
+    const bool one_tile = p.Nq <= pl.q_per_tile, counts = p.kv_lengths || ruled;
+    if (counts && one_tile) ranges = (3 * ranges + 3) / 4;
     if (total < (1 << 28) && whole * 9 > (ranges + kMergeUnits) * 10) {
         pl.sched = one_tile ? 2 : 1;
-        pl.start_cost = p.kv_lengths && one_tile && ranges >= kLongRange ? 3 : 0;
+        pl.start_cost = counts && one_tile && ranges >= kLongRange ? 3 : 0;
         const int tiles = (int)(((int64_t)p.Nq + pl.q_per_tile - 1) / pl.q_per_tile);
         const int rows = tiles > 1 ? 2 * kBlockM : p.Nq * pl.pack;
         pl.part_rows = (int)align_up((size_t)rows, 32);
@@ -1274,13 +1440,14 @@ FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free) {
     return plan_schedule(p, D, sms, false);
 }
 
-template <int D, bool BF16, int PREC>
-int launch(const fa_b200_params& p, void* ws, size_t ws_bytes) {
+// `rules`: RULES != 0 instances only.
+template <int D, bool BF16, int PREC, int RULES = 0>
+int launch(const fa_b200_params& p, void* ws, size_t ws_bytes, const Rules* rules = nullptr) {
     const int d = p.D;
     const int sms = sm_count(p.device);
     if (sms <= 0) { set_error("cannot read the SM count of device %d", p.device); return FA_ECUDA; }
-    FwdPlan plan = plan_schedule(p, D, sms, ws != nullptr);
-    if (ws_bytes < plan.bytes || ((uintptr_t)ws & 255u) != 0) plan = plan_schedule(p, D, sms, false);
+    FwdPlan plan = plan_schedule(p, D, sms, ws != nullptr, RULES != 0);
+    if (ws_bytes < plan.bytes || ((uintptr_t)ws & 255u) != 0) plan = plan_schedule(p, D, sms, false, RULES != 0);
     const CUtensorMapDataType dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap mq, mk, mv;
     int r;
@@ -1298,6 +1465,16 @@ int launch(const fa_b200_params& p, void* ws, size_t ws_bytes) {
         return FA_ECUDA;
     }
     FwdArgs a;
+    a.rules = Rules{};
+    a.cap_in = a.cap_out = 0.f;
+    a.cols_per_group = 1;
+    if constexpr (RULES != 0) {
+        a.rules = *rules;
+        if (RULES == 2) { a.cap_in = (float)((double)p.scale / rules->cap); a.cap_out = rules->cap * kLog2e; }
+        const int64_t col_bytes = 2 * (int64_t)p.Nk * D * 2 / (p.H / p.Hkv);
+        const int64_t g = (int64_t)tile::kFwdGroupBytes / (col_bytes > 0 ? col_bytes : 1), cols = (int64_t)p.B * p.H;
+        a.cols_per_group = (int)(g < 1 ? 1 : (g > cols ? cols : g));
+    }
     a.bias_b = bias_b; a.bias_h = bias_h;
     a.o = p.o.ptr;
     a.o_sb = p.o.stride_b; a.o_sn = p.o.stride_n; a.o_sh = p.o.stride_h;
@@ -1347,12 +1524,13 @@ int launch(const fa_b200_params& p, void* ws, size_t ws_bytes) {
         a.mq = (const uint4*)p.dropout_bits;
         drop = 2;
     }
-    auto kernel = drop == 2 ? fwd_sm100_kernel<D, BF16, 2, PREC, 0> : fwd_sm100_kernel<D, BF16, 0, PREC, 0>;
-    if constexpr (PREC != 2) if (drop == 1) kernel = fwd_sm100_kernel<D, BF16, 1, PREC, 0>;      // bias_is_staged()
+    auto kernel = fwd_sm100_kernel<D, BF16, 0, PREC, 0, RULES>;
+    if constexpr (RULES == 0) if (drop == 2) kernel = fwd_sm100_kernel<D, BF16, 2, PREC, 0>;
+    if constexpr (PREC != 2 && RULES == 0) if (drop == 1) kernel = fwd_sm100_kernel<D, BF16, 1, PREC, 0>;      // bias_is_staged()
     int smem = FwdCfg<D, PREC, 0>::kSmemBytes;
     if constexpr (PREC == 0) {
-        if (plan.sched == 1) kernel = fwd_sm100_kernel<D, BF16, 0, PREC, 1>;
-        if (plan.sched == 2) { kernel = fwd_sm100_kernel<D, BF16, 0, PREC, 2>; smem = FwdCfg<D, PREC, 2>::kSmemBytes; }
+        if (plan.sched == 1) kernel = fwd_sm100_kernel<D, BF16, 0, PREC, 1, RULES>;
+        if (plan.sched == 2) { kernel = fwd_sm100_kernel<D, BF16, 0, PREC, 2, RULES>; smem = FwdCfg<D, PREC, 2>::kSmemBytes; }
     }
     {
         static std::mutex mu;
@@ -1372,13 +1550,27 @@ int launch(const fa_b200_params& p, void* ws, size_t ws_bytes) {
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        FA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fwd_merge_kernel<D, BF16>, a));
+        FA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fwd_merge_kernel<D, BF16, RULES != 0>, a));
     }
     return FA_OK;
 }
 
 
-#ifndef FA_PAIR_INSTANCES
+#if defined(FA_RULES_INSTANCES)
+}  // namespace
+
+template <int RULES>
+int fwd_by_type(const fa_b200_params& p, const Rules& rules, void* ws, size_t ws_bytes) {
+    if (p.dtype == FA_B200_BF16) return p.D > 64 ? launch<128, true, 0, RULES>(p, ws, ws_bytes, &rules) : launch<64, true, 0, RULES>(p, ws, ws_bytes, &rules);
+    return p.D > 64 ? launch<128, false, 0, RULES>(p, ws, ws_bytes, &rules) : launch<64, false, 0, RULES>(p, ws, ws_bytes, &rules);
+}
+int sm100_rules_fwd(const fa_b200_params& p, const Rules& rules, void* ws, size_t ws_bytes) {
+    return rules.cap > 0.f ? fwd_by_type<2>(p, rules, ws, ws_bytes) : fwd_by_type<1>(p, rules, ws, ws_bytes);
+}
+size_t sm100_rules_fwd_workspace_bytes(const fa_b200_params& p) {
+    return plan_schedule(p, p.D > 64 ? 128 : 64, sm_count(p.device), true, true).bytes;
+}
+#elif !defined(FA_PAIR_INSTANCES)
 bool tensor_ok(const fa_b200_tensor& t, int64_t B, int64_t N, int64_t H) {
     if (((uintptr_t)t.ptr & 15u) != 0) return false;
     if (H > 1 && (t.stride_h % 8) != 0) return false;

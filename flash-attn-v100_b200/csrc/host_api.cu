@@ -380,7 +380,12 @@ int validate_rules(const fa_b200_params* p, const fa_b200_rules* r) {
 }
 // Kernel family of a call with rules.
 int choose_rules_variant(const fa_b200_params& p, bool backward, int* variant) {
-    (void)backward;
+    const char* why = "";
+    const bool tc = !backward && sm100_pair_supports(p, backward, &why);
+    if (p.variant == FA_B200_VARIANT_TCGEN05 || p.variant == FA_B200_VARIANT_TCGEN05_2PASS) {
+        if (!tc) { set_error("tcgen05 kernels do not cover this call: %s", why); return FA_EUNSUPPORTED; }
+    }
+    if (p.variant != FA_B200_VARIANT_SIMT && tc) { *variant = FA_B200_VARIANT_TCGEN05_2PASS; return FA_OK; }
     if (!simt_supports(p)) { set_error("no kernel covers D=%d with rules", p.D); return FA_EUNSUPPORTED; }
     *variant = FA_B200_VARIANT_SIMT;
     return FA_OK;
@@ -391,7 +396,10 @@ extern "C" {
 
 size_t fa_b200_fwd_rules_workspace_bytes(const fa_b200_params* p) {
     if (!p || p->struct_bytes != sizeof(fa_b200_params)) return 0;
-    return 0;
+    if (p->B <= 0 || p->Nq <= 0 || p->Nk <= 0 || p->H <= 0 || p->Hkv <= 0 || p->D <= 0 || p->H % p->Hkv != 0) return 0;
+    int variant;
+    if (choose_rules_variant(*p, false, &variant) != FA_OK || variant == FA_B200_VARIANT_SIMT) return 0;
+    return sm100_rules_fwd_workspace_bytes(*p);
 }
 
 int fa_b200_fwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r, void* workspace, size_t workspace_bytes) {
@@ -405,8 +413,7 @@ int fa_b200_fwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r, void
     GuardDevice g(p->device);
     if (!g.ok) { set_error("cudaSetDevice(%d) failed", p->device); return FA_ECUDA; }
     const Rules u = make_rules(*r, p->Nq, p->Nk);
-    (void)workspace; (void)workspace_bytes;
-    return simt_fwd(*p, &u);
+    return variant != FA_B200_VARIANT_SIMT ? sm100_rules_fwd(*p, u, workspace, workspace_bytes) : simt_fwd(*p, &u);
 }
 
 size_t fa_b200_bwd_rules_workspace_bytes(const fa_b200_params* p) {

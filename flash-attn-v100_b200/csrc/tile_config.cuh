@@ -28,6 +28,8 @@ constexpr int kFwdRegsOther = 88;
 // gradients the same.
 constexpr int fwd_poly_period(int D) { return D == 64 ? 4 : 2; }
 constexpr int kFwdHalfSignalAt = 16;    // first half of P handed over after this many of the second half's exps
+// calls with rules: (batch, head) columns per group of work items such that a group's K and V fit this budget
+constexpr long long kFwdGroupBytes = 64ll << 20;
 constexpr float kFwdRescaleLog2 = 8.f;  // the running maximum is refreshed when it grows by more than 2^8
 
 // ---- backward (bwd_sm100.cu) --------------------------------------------------------------------
