@@ -74,6 +74,7 @@
 #include "sm100_ptx.cuh"
 #include "tma_host.cuh"
 #include "tile_config.cuh"
+#include "score_rules.cuh"
 #include <type_traits>
 
 namespace fa {
@@ -199,6 +200,9 @@ struct BwdArgs {
     int ds_vec;                    // rows of d_scores can be written as float4
     int ds_staged;                 // PREC = 2: d_scores leaves by TMA
     float* d_scores;               // optional dense (B, H, Nq, Nk) gradient of the scores (written by MODE 1)
+    // Calls with rules (RULES != 0):
+    Rules rules;
+    float cap_in, cap_out;         // u = S * cap_in, x = tanh(u) * cap_out (log2 units)
 };
 
 __device__ __forceinline__ void bulk_load_1d(void* smem_dst, const void* gsrc, uint32_t bytes, uint64_t* bar) {
@@ -321,7 +325,7 @@ struct BwdItem {
     int head_kv, pad;
 };
 static_assert(sizeof(BwdItem) == 48, "kCtlBytes");
-template <bool KS, bool FUSED, bool DS>
+template <bool KS, bool FUSED, bool DS, int RULES>
 __device__ __forceinline__ BwdItem make_item(const BwdArgs& a, const CtaWork& cw) {
     BwdItem m;
     m.b = cw.b;
@@ -336,18 +340,30 @@ __device__ __forceinline__ BwdItem make_item(const BwdArgs& a, const CtaWork& cw
         const int nq_tiles = (a.Nq + kTile - 1) / kTile;
         m.n_per_head = nq_tiles > m.it0 ? nq_tiles - m.it0 : 0;
         if (m.tile * kTile >= m.nk) m.n_per_head = 0;   // a tile of padding keys: dK = dV = 0
+        if (RULES) {
+            // the query tiles whose ranges meet the key tile, and those between
+            const int2 seen = a.rules.k_tiles[m.b * a.rules.k_tiles_b + m.tile];
+            m.it0 = max(seen.x, 0);
+            m.n_per_head = max(min(seen.y, nq_tiles) - m.it0, 0);
+        }
         m.n_iter = m.n_per_head * a.group;
         // The fused kernel without a causal mask starts each key tile's walk at a different query tile, so that the CTAs
         // of one head, which run at the same time, add to different dQ tiles (under a causal mask the walks are
         // staggered already).
         if (FUSED && !a.causal && m.n_per_head > 0) m.rot = m.tile % m.n_per_head;
     } else {
-        m.tile = a.causal ? (int)gridDim.x - 1 - cw.tile_rank : cw.tile_rank;     // query tile, heavy first
+        m.tile = a.causal || RULES ? (int)gridDim.x - 1 - cw.tile_rank : cw.tile_rank;     // query tile, heavy first
         m.head_kv = cw.head / a.group;
         m.it0 = 0;
         int kv_end = m.nk;
         if (a.causal && m.tile * kTile + kTile + a.shift < kv_end) kv_end = m.tile * kTile + kTile + a.shift;
+        if (RULES) {
+            const int4 hull = a.rules.q_tiles[m.b * a.rules.q_tiles_b + m.tile];
+            kv_end = min(hull.y, a.Nk);
+            m.it0 = max(hull.x, 0) / kTile;
+        }
         m.n_per_head = kv_end > 0 ? (kv_end + kTile - 1) / kTile : 0;
+        if (RULES) m.n_per_head = max(m.n_per_head - m.it0, 0);
         // d(loss)/d(scores) wanted: the steps are walked twice (comment at `sum_p2` below)
         m.n_iter = DS ? 2 * m.n_per_head : m.n_per_head;
     }
@@ -361,7 +377,10 @@ __device__ __forceinline__ BwdItem make_item(const BwdArgs& a, const CtaWork& cw
 // DS (pairs, MODE 1): the call wants d(loss)/d(scores).  An instance of its own: as branches its code cost the kernel of
 // calls that do not want it 13 of 66 us (B4 N1024 H16 D96 causal).  Two walks over the keys take 95 us where one took 71
 // (B8 N512 H12 D64 bf16); see `sum_p2` for what they give.
-template <int D, bool BF16, int MODE, int NWG, int DROP, bool INLINE, int PREC, bool DS>
+// RULES: 0 none; calls with rules (fa_b200_rules): 1 ranges and distances, 2 a score cap as well.  As PREC = 0, with any head
+// size that is a multiple of 8.  Blocks walk the tiles their ranges meet; a tile that some row does not see whole is masked
+// key by key.  The cap's derivative, 1 - tanh^2, goes to P when P has been handed to its MMA: what dS is then made of.
+template <int D, bool BF16, int MODE, int NWG, int DROP, bool INLINE, int PREC, bool DS, int RULES = 0>
 __global__ void __launch_bounds__(128 * NWG + kExtraThreads, 1)
 bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
                  const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_w,
@@ -374,6 +393,8 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     constexpr bool CONV = BF16 && PREC == 0;    // every MMA runs f16 x f16: bf16 tiles are converted
     constexpr bool P_BF16 = BF16 && PREC != 0;  // ... except that pairs of bf16 need no conversion
     static_assert(PREC == 0 || (MODE != 2 && !INLINE), "the pair instances are the two-pass form");
+    constexpr bool RULED = RULES != 0, ANY_D = PREC != 0 || RULED;
+    static_assert(!RULED || (PREC == 0 && DROP == 0 && MODE != 2 && !INLINE && !DS), "rules come without bias and dropout, in two passes");
     constexpr bool STREAM_CONV = CONV && INLINE;             // ... the streamed ones by warps 18 and 19
     constexpr bool XY_CONV = CONV && (KS || INLINE);         // ... the stationary ones (X; key-stationary also Y), too
     constexpr bool ROWFORM = CONV && !INLINE;                // staged vectors are in the row form (see DoForm)
@@ -500,7 +521,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             int xy_issued[2] = {0, 0};
             bool ok = true;
             CtaWork w = cta_work(a.cols_per_group, blockIdx);
-            BwdItem m = make_item<KS, FUSED, DS>(a, w);
+            BwdItem m = make_item<KS, FUSED, DS, RULES>(a, w);
             auto publish = [&](int k) {
                 const int slot = k & 1;
                 float2 rg = make_float2(0.f, 0.f);
@@ -527,7 +548,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 for (int it = 0; it < m.n_iter; ++it) {
                     int head_u, row_u;
                     if (KS) { head_u = m.head_x * a.group + hg; row_u = q_tile_of(m.it0, m.n_per_head, m.rot, qi) * kTile; }
-                    else    { head_u = m.head_kv; row_u = k_tile_of(m.n_per_head, it) * kTile; }
+                    else    { head_u = m.head_kv; row_u = ((RULED ? m.it0 : 0) + k_tile_of(m.n_per_head, it)) * kTile; }
                     ok = mbar_wait(&bars[Cfg::kUEmpty + us], (uph & 1u) ^ 1u, abort_flag);
                     if (!ok) break;
                     mbar_expect_tx(&bars[Cfg::kUFull + us], TILE);
@@ -582,7 +603,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 uint3 block;
                 const bool another = clc_answer_block(clc_answer, block);
                 fence_proxy_async_smem();            // read before the next answer is written
-                if (another) m = make_item<KS, FUSED, DS>(a, cta_work(a.cols_per_group, block));
+                if (another) m = make_item<KS, FUSED, DS, RULES>(a, cta_work(a.cols_per_group, block));
                 else m.n_iter = -1;
                 publish(k + 1);
                 if (!another) break;
@@ -609,7 +630,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             constexpr bool T1_BF16 = BF16 && !CONV, T2_BF16 = BF16 && !(CONV && KS);
             constexpr uint32_t idesc_t1 = make_idesc_f16(T1_BF16, T1_BF16, kTile, kTile, false, false);
             constexpr uint32_t idesc_t2 = make_idesc_f16(T2_BF16, T2_BF16, kTile, kTile, false, false);
-            const uint32_t idesc_acc = PREC ? make_idesc_f16(P_BF16, P_BF16, kTile, (a.d + 15) & ~15, false, true)
+            const uint32_t idesc_acc = ANY_D ? make_idesc_f16(P_BF16, P_BF16, kTile, (a.d + 15) & ~15, false, true)
                                             : make_idesc_f16(false, false, kTile, D, false, true);
             constexpr int kUReady = STREAM_CONV ? Cfg::kUConv : Cfg::kUFull;
             constexpr int kWReady = (STREAM_CONV && KS) ? Cfg::kWConv : Cfg::kWFull;
@@ -627,7 +648,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     const uint32_t off = ((uint32_t)(kk >> 2) * kBoxBytes + (uint32_t)(kk & 3) * 32u) >> 4;
-                    if (PREC == 0 || kk * 16 < a.d) mma_ss_f16(d_tmem, a0 + off, b0 + off, idesc_t, kk > 0);
+                    if (!ANY_D || kk * 16 < a.d) mma_ss_f16(d_tmem, a0 + off, b0 + off, idesc_t, kk > 0);
                 }
             };
             // acc (+)= A[TMEM] * B[smem tile, MN-major], restricted to the first (hf = 0) or second 16 columns of
@@ -992,6 +1013,17 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         [[maybe_unused]] float* ds_row = DS
             ? a.d_scores + (((int64_t)b * a.H + head_x) * a.Nq + row_g) * (int64_t)a.Nk : nullptr;
         [[maybe_unused]] const float ds_mul = sc.ds_mul;
+        // rules: position of row 0; query-stationary: my row's keys, what a key's distance takes off in log2 units
+        [[maybe_unused]] int origin = 0;
+        [[maybe_unused]] int2 keys = make_int2(0, 0);
+        [[maybe_unused]] float row_slope = 0.f;
+        if constexpr (RULED) {
+            origin = a.rules.origin[b * a.rules.origin_b];
+            if (!KS) {
+                if (row_g < a.Nq) keys = a.rules.rows[b * a.rules.rows_b + row_g];
+                if (a.rules.slopes) row_slope = -a.rules.slopes[head_x] * kLog2e;
+            }
+        }
         // fused kernel: add the dQ tile of step `jt` (queries on the TMEM lanes, my D / NWG columns)
         // to the fp32 sums in global memory; the order of additions across CTAs is not fixed
         auto drain_dq = [&](int jt, int q_tile, int head_q) -> bool {
@@ -1026,7 +1058,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         int prev_tile = 0, prev_head = 0;   // query tile and head of the previous step
         for (const int g0 = g, g_end = g + n_iter; g < g_end && ok; ++g) {
             const int it = g - g0;          // (query-stationary)
-            const int strm_tile = (KS) ? q_tile_of(it0, n_per_head, rot, qi) : k_tile_of(n_per_head, it);     // query tile (0) / key tile (1)
+            const int strm_tile = (KS) ? q_tile_of(it0, n_per_head, rot, qi) : (RULED ? it0 : 0) + k_tile_of(n_per_head, it);     // query tile (0) / key tile (1)
             const int col_g0 = strm_tile * kTile + cb;                          // global index of my first column
             const int head_q = (KS) ? head_x * a.group + hg : head_x;
             const uint32_t bh = dropout_column(a.rng, b, head_q);
@@ -1101,6 +1133,25 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 #pragma unroll
                     for (int k = 0; k < 2; ++k) kwr[h][k] = w[16 * h + 8 * k];
             }
+            // rules: whether some query of the step does not see my whole key tile, and then, for my eight query columns, the
+            // tile's rows they see: first and end of columns 8j + 2lq + {0, 1}, a byte each (128: none)
+            [[maybe_unused]] bool partial = false;
+            [[maybe_unused]] uint32_t sees[4];
+            [[maybe_unused]] float slope = 0.f;
+            if constexpr (RULED) {
+                const int4 hull = a.rules.q_tiles[b * a.rules.q_tiles_b + strm_tile];
+                if (a.rules.slopes) slope = -a.rules.slopes[head_q] * kLog2e;
+                partial = hull.z > tile * kTile || hull.w < tile * kTile + kTile;
+                if (partial) {
+                    const int4* rows = reinterpret_cast<const int4*>(a.rules.rows + b * a.rules.rows_b + col_g0 + 2 * lq);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int4 x = rows[4 * j];
+                        auto in_tile = [&](int key) { return (uint32_t)min(max(key - tile * kTile, 0), kTile); };
+                        sees[j] = in_tile(x.x) | in_tile(x.y) << 8 | in_tile(x.z) << 16 | in_tile(x.w) << 24;
+                    }
+                }
+            }
             ok = mbar_wait(&bars[Cfg::kT1Full], (uint32_t)g & 1u, abort_flag);
             if (ok) ok = mbar_wait(&bars[Cfg::kVFull + (g & 1)], (uint32_t)(g >> 1) & 1u, abort_flag);
             if (PREC == 2 && ok) ok = mbar_wait(&bars[Cfg::kBiasFull], (uint32_t)g & 1u, abort_flag);
@@ -1135,7 +1186,36 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                                 kbits |= (((uint32_t)mbuf[col * 8 + (row >> 4)] >> (row & 15)) & 1u) << (16 * h + 4 * j + 2 * k + e);
                             }
             }
-            const float sc1 = PREC ? a.score_scale : a.scale_log2;
+            if constexpr (RULES == 2) {
+                // tanh(u) in the place of u = S scale / cap
+                const uint64_t in2 = f2_pack(a.cap_in, a.cap_in);
+                float top = 0.f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int c = 0; c < 16; c += 2) {
+                        const uint64_t u = f2_mul(f2_pack(__uint_as_float(pf[h][c]), __uint_as_float(pf[h][c + 1])), in2), z = f2_mul(u, u);
+                        float x0, x1;
+                        f2_unpack(z, x0, x1);
+                        top = max3(top, x0, x1);
+                        f2_unpack(f2_tanh_poly(u, z), x0, x1);
+                        pf[h][c] = __float_as_uint(x0);
+                        pf[h][c + 1] = __float_as_uint(x1);
+                    }
+                if (__any_sync(0xffffffffu, top > kTanhPolyMax * kTanhPolyMax)) {
+                    tmem_ld_16x256b_x4(tT1 + t_lo, pf[0]);
+                    tmem_ld_16x256b_x4(tT1 + t_hi, pf[1]);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) pf[h][c] = __float_as_uint(tanh_any(__uint_as_float(pf[h][c]) * a.cap_in));
+                }
+            }
+            // position less key of element (j, h, k, e): `apart` + 8j + e - 16h - 8k
+            [[maybe_unused]] const float apart = (float)(origin + col_g0 + 2 * lq - (tile * kTile + rbase));
+            [[maybe_unused]] const bool ahead = origin + strm_tile * kTile < tile * kTile + kTile - 1;    // some key is behind its query
+            const float sc1 = RULES == 2 ? a.cap_out : (PREC ? a.score_scale : a.scale_log2);
             const uint64_t sc2 = f2_pack(sc1, sc1);
             // key row > query column + shift is hidden: only tiles the mask's edge crosses need the test
             const bool diag = a.causal && strm_tile * kTile + a.shift < tile * kTile + kTile - 1;
@@ -1191,13 +1271,40 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                             if (PREC == 2 || (PREC == 1 && a.bias)) x = f2_add(x, L);
                             if (P_BF16)    x = f2_mul(x, f2_pack(kLog2e, kLog2e));
                             else if (PREC) x = f2_fma(x, f2_pack(kLog2e, kLog2e), f2_pack(kPShift, kPShift));
+                            if (RULED && a.rules.slopes) {
+                                const float away = (float)(8 * j - 16 * h - 8 * k);
+                                uint64_t d2 = f2_add(f2_pack(apart, apart), f2_pack(away, away + 1.f));
+                                if (ahead) {
+                                    float d0, d1;
+                                    f2_unpack(d2, d0, d1);
+                                    d2 = f2_pack(fabsf(d0), fabsf(d1));
+                                }
+                                x = f2_fma(d2, f2_pack(slope, slope), x);
+                            }
                             f2_unpack(x, x0, x1);
+                            if constexpr (RULED) {
+                                float p0 = ex2(x0), p1 = ex2(x1);
+                                if (partial) {
+                                    const uint32_t key = (uint32_t)(rbase + 16 * h + 8 * k), w = sees[j];
+                                    if (key < (w & 0xFFu) || key >= (w >> 8 & 0xFFu)) p0 = 0.f;
+                                    if (key < (w >> 16 & 0xFFu) || key >= w >> 24) p1 = 0.f;
+                                }
+                                pk[h][2 * jj + k] = pack2<false>(p0, p1);
+                                if (RULES == 2) {
+                                    // the part of the score's gradient that gets through the cap
+                                    const uint64_t t2 = f2_pack(__uint_as_float(pf[h][i0]), __uint_as_float(pf[h][i0 + 1])), p2 = f2_pack(p0, p1);
+                                    f2_unpack(f2_fma(f2_mul(p2, t2), f2_mul(t2, f2_pack(-1.f, -1.f)), p2), p0, p1);
+                                }
+                                pf[h][i0] = __float_as_uint(p0);
+                                pf[h][i0 + 1] = __float_as_uint(p1);
+                                continue;
+                            }
                             pf[h][i0] = __float_as_uint(ex2(x0));
                             pf[h][i0 + 1] = __float_as_uint(ex2(x1));
                         }
                 }
                 if (PREC == 2 && hf == 1) mbar_arrive_read_done(&bars[Cfg::kBiasEmpty]);
-                if (diag || tail) {
+                if (!RULED && (diag || tail)) {
                     // one branch for the whole half: the diagonal tile and a tile with padding keys are rare
 #pragma unroll
                     for (int jj = 0; jj < 2; ++jj)
@@ -1212,7 +1319,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                             }
                 }
 #pragma unroll
-                for (int jj = 0; jj < 2; ++jj)
+                for (int jj = 0; jj < (RULED ? 0 : 2); ++jj)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -1385,6 +1492,42 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 tmem_wait_st();
             } else {
                 const uint64_t neg2 = f2_pack(my_nlse2, my_nlse2);
+                [[maybe_unused]] const uint64_t mul2 = RULES == 2 ? f2_pack(a.cap_out, a.cap_out) : sc2;
+                if constexpr (RULES == 2) {
+                    // u = S scale / cap, then its tanh, in place (S itself may be overwritten in tensor memory by now)
+                    const uint64_t in2 = f2_pack(a.cap_in, a.cap_in);
+                    float top = 0.f;
+#pragma unroll
+                    for (int c = 0; c < CPT; c += 2) {
+                        const uint64_t u = f2_mul(f2_pack(PF(c), PF(c + 1)), in2);
+                        float x0, x1, u0, u1;
+                        f2_unpack(f2_mul(u, u), x0, x1);
+                        top = max3(top, x0, x1);
+                        f2_unpack(u, u0, u1);
+                        PSET(c, u0);
+                        PSET(c + 1, u1);
+                    }
+                    if (__any_sync(0xffffffffu, top > kTanhPolyMax * kTanhPolyMax)) {
+#pragma unroll
+                        for (int c = 0; c < CPT; ++c) PSET(c, tanh_any(PF(c)));
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < CPT; c += 2) {
+                            const uint64_t u = f2_pack(PF(c), PF(c + 1));
+                            float x0, x1;
+                            f2_unpack(f2_tanh_poly(u, f2_mul(u, u)), x0, x1);
+                            PSET(c, x0);
+                            PSET(c + 1, x1);
+                        }
+                    }
+                }
+                [[maybe_unused]] uint64_t d2 = 0ull;
+                [[maybe_unused]] bool ahead = false;
+                if constexpr (RULED) {
+                    const int from = origin + row_g - col_g0;
+                    d2 = f2_pack((float)from, (float)from - 1.f);
+                    ahead = __any_sync(0xffffffffu, from < min(CPT, keys.y - col_g0) - 1);
+                }
                 [[maybe_unused]] const uint64_t scn2 = f2_pack(a.score_scale, a.score_scale), log2e2 = f2_pack(kLog2e, kLog2e), up2 = f2_pack(p_mul, p_mul);
                 [[maybe_unused]] float4 bv = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -1423,6 +1566,31 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                         PSET(c + 1, x1);
                         continue;
                     }
+                    if constexpr (RULED) {
+                        const uint64_t t2 = f2_pack(PF(c), PF(c + 1));
+                        uint64_t x = f2_fma(t2, mul2, neg2);
+                        if (a.rules.slopes) {
+                            uint64_t by = d2;
+                            if (ahead) {
+                                float d0, d1;
+                                f2_unpack(d2, d0, d1);
+                                by = f2_pack(fabsf(d0), fabsf(d1));
+                            }
+                            x = f2_fma(by, f2_pack(row_slope, row_slope), x);
+                            d2 = f2_add(d2, f2_pack(-2.f, -2.f));
+                        }
+                        f2_unpack(x, x0, x1);
+                        x0 = ex2(x0);
+                        x1 = ex2(x1);
+                        if (RULES == 2) {
+                            // (dS needs P and the cap's derivative as a product only)
+                            const uint64_t p2 = f2_pack(x0, x1);
+                            f2_unpack(f2_fma(f2_mul(p2, t2), f2_mul(t2, f2_pack(-1.f, -1.f)), p2), x0, x1);
+                        }
+                        PSET(c, x0);
+                        PSET(c + 1, x1);
+                        continue;
+                    }
                     f2_unpack(f2_fma(f2_pack(PF(c), PF(c + 1)), sc2, neg2), x0, x1);
                     // a quarter of the exponentials as a polynomial on the FMA pipes (this kernel keeps the
                     // special-function unit busiest; measured 0.7 % over the backward, half: 0.2 %)
@@ -1437,8 +1605,17 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                     }
                 }
                 if (PREC == 2 && (!DS || !a.ds_staged || summing)) mbar_arrive_read_done(&bars[Cfg::kBiasEmpty]);
+                if constexpr (RULED) {
+                    const int lo = keys.x - col_g0, hi = keys.y - col_g0;             // the columns my row sees
+                    if (__any_sync(0xffffffffu, lo > 0 || hi < CPT)) {
+#pragma unroll
+                        for (int c = 0; c < CPT; ++c)
+                            if (c < lo || c >= hi) PSET(c, 0.f);
+                    }
+                }
                 const bool diag = a.causal && strm_tile * kTile + kTile - 1 > tile * kTile + a.shift;
-                if (diag || strm_tile * kTile + kTile > nk) {
+                if (RULED) {
+                } else if (diag || strm_tile * kTile + kTile > nk) {
                     // my row sees my first `seen` columns: keys below the count, at most row + shift
                     seen = nk - col_g0;
                     if (diag && row_g + a.shift + 1 - col_g0 < seen) seen = row_g + a.shift + 1 - col_g0;
@@ -1677,7 +1854,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             uint16_t* dst2 = (uint16_t*)a.out2 + m->b * a.o2_sb + row * a.o2_sn + m->head_x * a.o2_sh;
 #pragma unroll
             for (int col = wg * kCols; col < (wg + 1) * kCols; col += 8) {
-                if (PREC != 0 && col >= a.d) break;
+                if (ANY_D && col >= a.d) break;
                 *reinterpret_cast<uint4*>(dst1 + col) = make_uint4(0u, 0u, 0u, 0u);
                 if (KS) *reinterpret_cast<uint4*>(dst2 + col) = make_uint4(0u, 0u, 0u, 0u);
             }
@@ -1854,11 +2031,14 @@ bwd_dq_convert_kernel(const float* __restrict__ acc, T* __restrict__ dq, int Nq,
 // convert their tiles themselves.
 // the kernel instance and its shared memory for a dropout form (0 none, 1 drawn in the kernel, 2 loaded;
 // the converting-in-kernel instances, which serve the entry without a workspace, never load)
-template <int D, bool BF16, int MODE, bool INLINE, int PREC, bool DS = false>
+template <int D, bool BF16, int MODE, bool INLINE, int PREC, bool DS = false, int RULES = 0>
 auto pick_kernel(int drop) {
+    if constexpr (RULES != 0) return bwd_sm100_kernel<D, BF16, MODE, kNWG, 0, INLINE, PREC, DS, RULES>;
+    else {
     if (drop == 2 && !INLINE) return bwd_sm100_kernel<D, BF16, MODE, kNWG, INLINE ? 1 : 2, INLINE, PREC, DS>;
     if constexpr (PREC == 2) return bwd_sm100_kernel<D, BF16, MODE, kNWG, 0, INLINE, PREC, DS>;       // bias_is_staged(): never drop = 1
     else return drop ? bwd_sm100_kernel<D, BF16, MODE, kNWG, 1, INLINE, PREC, DS> : bwd_sm100_kernel<D, BF16, MODE, kNWG, 0, INLINE, PREC, DS>;
+    }
 }
 template <int D, int MODE, int PREC>
 int pick_smem(int drop) {
@@ -1867,8 +2047,9 @@ int pick_smem(int drop) {
                      : (drop ? BwdCfg<D, MODE, 1, PREC>::kSmemBytes : BwdCfg<D, MODE, 0, PREC>::kSmemBytes);
 }
 
-template <int D, bool BF16, bool INLINE, int PREC>
-int launch(const fa_b200_params& p, const BwdWorkspace& ws) {
+// `rules`: RULES != 0 instances only.
+template <int D, bool BF16, bool INLINE, int PREC, int RULES = 0>
+int launch(const fa_b200_params& p, const BwdWorkspace& ws, const Rules* rules = nullptr) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     const CUtensorMapDataType dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     constexpr bool COPIES = BF16 && !INLINE && PREC == 0;
@@ -1938,6 +2119,12 @@ int launch(const fa_b200_params& p, const BwdWorkspace& ws) {
     }
     CUtensorMap mb = mq, mds = mq;
     BwdArgs a;
+    a.rules = Rules{};
+    a.cap_in = a.cap_out = 0.f;
+    if constexpr (RULES != 0) {
+        a.rules = *rules;
+        if (RULES == 2) { a.cap_in = (float)((double)p.scale / rules->cap); a.cap_out = rules->cap * kLog2e; }
+    }
     a.bias_b = p.bias.stride_b != 0 && p.B > 1; a.bias_h = p.bias.stride_h != 0 && p.H > 1;
     if (PREC == 2 && (r = cached_tmap_bnhd(&mb, p.bias.ptr, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, a.bias_b ? p.B : 1, p.Nq, a.bias_h ? p.H : 1,
                                            p.Nk, p.bias.stride_b, p.bias.stride_n, p.bias.stride_h, 128, 32, 1))) {
@@ -1994,7 +2181,7 @@ int launch(const fa_b200_params& p, const BwdWorkspace& ws) {
     constexpr int kThreads = 128 * kNWG + kExtraThreads;
     const dim3 grid_kv((p.Nk + kTile - 1) / kTile, p.Hkv, p.B);
     const dim3 grid_q((p.Nq + kTile - 1) / kTile, p.H, p.B);
-    if constexpr (D == 64 && PREC == 0) if (fused) {
+    if constexpr (D == 64 && PREC == 0 && RULES == 0) if (fused) {
         // one key-stationary kernel for dK, dV and the fp32 dQ sums, then the conversion of dQ
         auto k2 = pick_kernel<D, BF16, 2, INLINE, PREC>(drop);
         const int smem2 = pick_smem<D, 2, PREC>(drop);
@@ -2013,8 +2200,8 @@ int launch(const fa_b200_params& p, const BwdWorkspace& ws) {
         return FA_OK;
     }
     if (COPIES && ws.k16_bytes == 0) { set_error("workspace layout lacks the fp16 copy of K"); return FA_EWORKSPACE; }
-    auto k0 = pick_kernel<D, BF16, 0, INLINE, PREC>(drop);
-    auto k1 = pick_kernel<D, BF16, 1, INLINE, PREC>(drop);
+    auto k0 = pick_kernel<D, BF16, 0, INLINE, PREC, false, RULES>(drop);
+    auto k1 = pick_kernel<D, BF16, 1, INLINE, PREC, false, RULES>(drop);
     if constexpr (PREC != 0) if (p.d_scores) k1 = pick_kernel<D, BF16, 1, INLINE, PREC, true>(drop);
     const int smem0 = pick_smem<D, 0, PREC>(drop), smem1 = pick_smem<D, 1, PREC>(drop);
     FA_CUDA_CHECK(set_smem_limit_once(k0, smem0, p.device, &smem_done[drop], &smem_mu));
@@ -2054,7 +2241,16 @@ int launch(const fa_b200_params& p, const BwdWorkspace& ws) {
 
 }  // namespace
 
-#ifndef FA_PAIR_INSTANCES
+#if defined(FA_RULES_INSTANCES)
+template <int RULES>
+int bwd_by_type(const fa_b200_params& p, const BwdWorkspace& ws, const Rules& rules) {
+    if (p.dtype == FA_B200_BF16) return p.D > 64 ? launch<128, true, false, 0, RULES>(p, ws, &rules) : launch<64, true, false, 0, RULES>(p, ws, &rules);
+    return p.D > 64 ? launch<128, false, false, 0, RULES>(p, ws, &rules) : launch<64, false, false, 0, RULES>(p, ws, &rules);
+}
+int sm100_rules_bwd(const fa_b200_params& p, const BwdWorkspace& ws, const Rules& rules) {
+    return rules.cap > 0.f ? bwd_by_type<2>(p, ws, rules) : bwd_by_type<1>(p, ws, rules);
+}
+#elif !defined(FA_PAIR_INSTANCES)
 bool sm100_bwd_fused_supported(const fa_b200_params& p) {
     // D = 64 only.  At D = 128 tensor memory is full (S^T, dP^T, dK, dV), the per-step dQ tile has
     // to share dP^T's columns, which serialises the step, and the fp32 additions (64 KB per step)

@@ -378,10 +378,16 @@ int validate_rules(const fa_b200_params* p, const fa_b200_rules* r) {
     }
     return FA_OK;
 }
+// The tensor-core backward's workspace; its copies are rows of whole 64- or 128-column tiles.
+BwdWorkspace rules_workspace(const fa_b200_params& p) {
+    fa_b200_params q = p;
+    q.D = p.D > 64 ? 128 : 64;
+    return bwd_workspace_layout(q, FA_B200_VARIANT_TCGEN05_2PASS);
+}
 // Kernel family of a call with rules.
 int choose_rules_variant(const fa_b200_params& p, bool backward, int* variant) {
     const char* why = "";
-    const bool tc = !backward && sm100_pair_supports(p, backward, &why);
+    const bool tc = sm100_pair_supports(p, backward, &why);
     if (p.variant == FA_B200_VARIANT_TCGEN05 || p.variant == FA_B200_VARIANT_TCGEN05_2PASS) {
         if (!tc) { set_error("tcgen05 kernels do not cover this call: %s", why); return FA_EUNSUPPORTED; }
     }
@@ -419,7 +425,12 @@ int fa_b200_fwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r, void
 size_t fa_b200_bwd_rules_workspace_bytes(const fa_b200_params* p) {
     if (!p || p->struct_bytes != sizeof(fa_b200_params)) return 0;
     if (p->B <= 0 || p->Nq <= 0 || p->H <= 0 || p->Hkv <= 0 || p->D <= 0) return 256;
-    return bwd_workspace_layout(*p, FA_B200_VARIANT_SIMT).total;
+    // the largest family the call could be routed to, so that the answer does not depend on alignment
+    fa_b200_params q = *p;
+    q.q = q.k = q.v = q.o = q.d_o = q.dq = q.dk = q.dv = q.o_lo = fa_b200_tensor{};
+    const char* why = "";
+    return p->variant != FA_B200_VARIANT_SIMT && sm100_pair_supports(q, true, &why) ? rules_workspace(*p).total
+                                                                                    : bwd_workspace_layout(*p, FA_B200_VARIANT_SIMT).total;
 }
 
 int fa_b200_bwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r) {
@@ -433,14 +444,14 @@ int fa_b200_bwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r) {
     if (p->Nq == 0) return zero_dk_dv(p);
     int variant;
     if ((rc = choose_rules_variant(*p, true, &variant))) return rc;
-    const BwdWorkspace ws = bwd_workspace_layout(*p, variant);
+    const BwdWorkspace ws = variant == FA_B200_VARIANT_SIMT ? bwd_workspace_layout(*p, variant) : rules_workspace(*p);
     if (!p->workspace || p->workspace_bytes < ws.total) {
         set_error("backward needs %zu bytes of workspace, got %zu", ws.total, p->workspace ? p->workspace_bytes : (size_t)0);
         return FA_EWORKSPACE;
     }
     if (((uintptr_t)p->workspace & 255u) != 0) { set_error("workspace must be 256-byte aligned"); return FA_EALIGN; }
     const Rules u = make_rules(*r, p->Nq, p->Nk);
-    return simt_bwd(*p, ws, &u);
+    return variant != FA_B200_VARIANT_SIMT ? sm100_rules_bwd(*p, ws, u) : simt_bwd(*p, ws, &u);
 }
 
 // ---------------------------------------------------------------------------
