@@ -1014,7 +1014,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             ? a.d_scores + (((int64_t)b * a.H + head_x) * a.Nq + row_g) * (int64_t)a.Nk : nullptr;
         [[maybe_unused]] const float ds_mul = sc.ds_mul;
         // rules: position of row 0; query-stationary: my row's keys, what a key's distance takes off in log2 units
-        [[maybe_unused]] int origin = 0;
+        [[maybe_unused]] int origin = 0, bend = 0;
         [[maybe_unused]] int2 keys = make_int2(0, 0);
         [[maybe_unused]] float row_slope = 0.f;
         if constexpr (RULED) {
@@ -1187,25 +1187,33 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                             }
             }
             if constexpr (RULES == 2) {
-                // tanh(u) in the place of u = S scale / cap
-                const uint64_t in2 = f2_pack(a.cap_in, a.cap_in);
-                float top = 0.f;
+                // tanh(u) in the place of u = S scale / cap (the forms of score_rules.cuh: `bend`)
+                auto bent = [&](auto form) {
+                    const uint64_t in2 = f2_pack(a.cap_in, a.cap_in);
+                    float top = 0.f;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int c = 0; c < 16; c += 2) {
-                        const uint64_t u = f2_mul(f2_pack(__uint_as_float(pf[h][c]), __uint_as_float(pf[h][c + 1])), in2), z = f2_mul(u, u);
-                        float x0, x1;
-                        f2_unpack(z, x0, x1);
-                        top = max3(top, x0, x1);
-                        f2_unpack(f2_tanh_poly(u, z), x0, x1);
-                        pf[h][c] = __float_as_uint(x0);
-                        pf[h][c + 1] = __float_as_uint(x1);
-                    }
-                if (__any_sync(0xffffffffu, top > kTanhPolyMax * kTanhPolyMax)) {
+                        for (int c = 0; c < 16; c += 2) {
+                            const uint64_t u = f2_mul(f2_pack(__uint_as_float(pf[h][c]), __uint_as_float(pf[h][c + 1])), in2), z = f2_mul(u, u);
+                            float x0, x1;
+                            f2_unpack(z, x0, x1);
+                            top = max3(top, x0, x1);
+                            f2_unpack(f2_tanh_poly<decltype(form)::value>(u, z), x0, x1);
+                            pf[h][c] = __float_as_uint(x0);
+                            pf[h][c + 1] = __float_as_uint(x1);
+                        }
+                    const float most = decltype(form)::value ? kTanhLongMax : kTanhShortMax;
+                    return !__any_sync(0xffffffffu, top > most * most);
+                };
+                auto again = [&] {
                     tmem_ld_16x256b_x4(tT1 + t_lo, pf[0]);
                     tmem_ld_16x256b_x4(tT1 + t_hi, pf[1]);
                     tmem_wait_ld();
+                };
+                if (bend == 0 && !bent(std::false_type{})) { bend = 1; again(); }
+                if (bend == 1 && !bent(std::true_type{})) { bend = 2; again(); }
+                if (bend == 2) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -1507,18 +1515,21 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                         PSET(c, u0);
                         PSET(c + 1, u1);
                     }
-                    if (__any_sync(0xffffffffu, top > kTanhPolyMax * kTanhPolyMax)) {
-#pragma unroll
-                        for (int c = 0; c < CPT; ++c) PSET(c, tanh_any(PF(c)));
-                    } else {
+                    auto bent = [&](auto form) {
 #pragma unroll
                         for (int c = 0; c < CPT; c += 2) {
                             const uint64_t u = f2_pack(PF(c), PF(c + 1));
                             float x0, x1;
-                            f2_unpack(f2_tanh_poly(u, f2_mul(u, u)), x0, x1);
+                            f2_unpack(f2_tanh_poly<decltype(form)::value>(u, f2_mul(u, u)), x0, x1);
                             PSET(c, x0);
                             PSET(c + 1, x1);
                         }
+                    };
+                    if (!__any_sync(0xffffffffu, top > kTanhShortMax * kTanhShortMax)) bent(std::false_type{});
+                    else if (!__any_sync(0xffffffffu, top > kTanhLongMax * kTanhLongMax)) bent(std::true_type{});
+                    else {
+#pragma unroll
+                        for (int c = 0; c < CPT; ++c) PSET(c, tanh_any(PF(c)));
                     }
                 }
                 [[maybe_unused]] uint64_t d2 = 0ull;

@@ -86,7 +86,7 @@ static_assert(tile::kFwdQTilesPerCta == 2, "the kernel is written for two query 
 //   2  the same for a call whose rows fit one tile (decoding): the tile's even key blocks go through S_0, P_0 and O_0,
 //      the odd ones through S_1, P_1 and O_1, and the two sums are put together in the epilogue; the room of the
 //      second query tile goes to the K and V rings.
-template <int D, int PREC, int SCHED>
+template <int D, int PREC, int SCHED, int RULES = 0>
 struct FwdCfg {
     static constexpr int kNBox = D / 64;
     static constexpr int kTileBytes = kNBox * kBoxBytes;
@@ -112,7 +112,11 @@ struct FwdCfg {
     static constexpr int kORead = kMlFull + 1;             // SCHED = 2: O_1 has been read (both: one arrival per warp of a warpgroup)
     static constexpr int kBiasFull = kORead + 1;           // PREC = 2: [2 tiles][kBiasSlots]
     static constexpr int kBiasEmpty = kBiasFull + 2 * kBiasSlots;      // ... one arrival per warp of the warpgroup
-    static constexpr int kNumBars = kBiasEmpty + 2 * kBiasSlots;
+    static constexpr bool kDealt = RULES != 0 && SCHED == 0;    // the pairs are dealt out as CTAs get done (Dealer)
+    static constexpr int kSchedFull = kBiasEmpty + 2 * kBiasSlots;     // [2] the next pair's number is in its slot
+    static constexpr int kSchedEmpty = kSchedFull + (kDealt ? 2 : 0);  // [2] ... and has been read (one arrival per reading warp)
+    static constexpr int kClc = kSchedEmpty + (kDealt ? 2 : 0);        // the answer to the request for another pair has landed
+    static constexpr int kNumBars = kDealt ? (kClc + 2) & ~1 : kClc;      // (even: what lies behind them is 16-byte aligned)
     static constexpr int kMlBytes = SCHED == 2 ? kBlockM * 8 : 0;
     static constexpr int kWalkBytes = SCHED ? 8 * 40 : 0;  // a WalkRecord per softmax warp
     static constexpr int kSmemBytes = (kQTiles + 2 * kStages) * kTileBytes + kBiasBytes + kNumBars * 8 + 64 + kMlBytes + kWalkBytes + 1024;
@@ -164,10 +168,11 @@ struct FwdArgs {
 };
 
 // A stretch of work: key blocks [j0, j1) of a pair.  n[t]: behind the last block of the pair's tile t
-// (0: no rows); count(t): how many of them lie in this stretch.  With rules a pair's blocks begin at jb, not at 0.
+// (0: no rows); count(t): how many of them lie in this stretch.  With rules a tile's blocks begin at s[t], a pair's at jb.
 struct Stretch {
-    int pair, h, b, nk, j0, j1, n[2], jb;
-    __device__ __forceinline__ int count(int t) const { const int e = n[t] < j1 ? n[t] : j1; return e > j0 ? e - j0 : 0; }
+    int pair, h, b, nk, j0, j1, n[2], jb, s[2];
+    __device__ __forceinline__ int first(int t) const { return j0 > s[t] ? j0 : s[t]; }
+    __device__ __forceinline__ int count(int t) const { const int f = first(t), e = n[t] < j1 ? n[t] : j1; return e > f ? e - f : 0; }
     __device__ __forceinline__ bool whole() const { return j0 == jb && j1 >= n[0] && j1 >= n[1]; }
 };
 
@@ -195,8 +200,7 @@ __device__ __forceinline__ int2 tile_hull(const FwdArgs& a, int b, int q_per_til
     return r.y > 0 ? make_int2(max(r.x, 0), min(r.y, a.Nk)) : make_int2(0, 0);
 }
 // A tile whose rows see nothing walks one block, which gives them their zeros.
-__device__ __forceinline__ void ruled_blocks(const FwdArgs& a, int b, int q_per_tile, int pair, int (&n)[2], int& jb) {
-    int lo[2];
+__device__ __forceinline__ void ruled_blocks(const FwdArgs& a, int b, int q_per_tile, int pair, int (&lo)[2], int (&n)[2], int& jb) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int2 h = tile_hull(a, b, q_per_tile, pair, t);
@@ -208,14 +212,14 @@ __device__ __forceinline__ void ruled_blocks(const FwdArgs& a, int b, int q_per_
     if (jb == 0x7fffffff) jb = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
-        if (n[t] == 0 && (pair * 2 + t) * q_per_tile < a.Nq) n[t] = jb + 1;
+        if (n[t] == 0) { lo[t] = jb; n[t] = (pair * 2 + t) * q_per_tile < a.Nq ? jb + 1 : 0; }
 }
 template <int RULES>
 __device__ __forceinline__ void stretch_blocks(const FwdArgs& a, int q_per_tile, Stretch& s) {
-    s.jb = 0;
+    s.jb = s.s[0] = s.s[1] = 0;
     if constexpr (RULES != 0) {
         s.nk = a.Nk;
-        ruled_blocks(a, s.b, q_per_tile, s.pair, s.n, s.jb);
+        ruled_blocks(a, s.b, q_per_tile, s.pair, s.s, s.n, s.jb);
     } else {
         s.nk = kv_len_of(a.kv_len, s.b, a.Nk);
         s.n[0] = num_blocks(a, q_per_tile, s.pair, 0, s.nk); s.n[1] = num_blocks(a, q_per_tile, s.pair, 1, s.nk);
@@ -224,8 +228,8 @@ __device__ __forceinline__ void stretch_blocks(const FwdArgs& a, int q_per_tile,
 template <int RULES>
 __device__ __forceinline__ int pair_blocks(const FwdArgs& a, int b, int pair, int nk) {
     if constexpr (RULES != 0) {
-        int n[2], jb;
-        ruled_blocks(a, b, a.q_per_tile, pair, n, jb);
+        int lo[2], n[2], jb;
+        ruled_blocks(a, b, a.q_per_tile, pair, lo, n, jb);
         return (n[0] > n[1] ? n[0] : n[1]) - jb;
     }
     const int n0 = num_blocks(a, a.q_per_tile, pair, 0, nk), n1 = num_blocks(a, a.q_per_tile, pair, 1, nk);
@@ -341,26 +345,76 @@ template <> struct WorkLoop<0, 0> {       // whole pairs, round robin
         return true;
     }
 };
-// Whole pairs with rules: what a pair costs is on the device.  In groups of columns whose K and V stay in L2, the last pair of
-// all columns first, which under a causal mask is the longest, then the one before it.
+// Whole pairs with rules: what a pair costs is on the device, so pairs are not dealt out beforehand.  The grid has a block a
+// pair; a CTA starts with its own and goes on with blocks not yet launched (clusterlaunchcontrol, as in the backward).
+// The order: groups of columns whose K and V stay in L2, in a group the last pair of all columns first, which under a
+// causal mask is the longest, then the one before it.  The producer asks (Dealer) and leaves the pair's number in one of two
+// slots for the other roles (WorkLoop).  Round robin: B4 N4096 H32 D128 bf16 with 8 documents a row 317 us.
+struct Deal {                              // in shared memory, at RangeStart's place; 16-byte aligned answer
+    int w[2], pad[2];
+    uint32_t answer[4];
+};
+template <int RULES>
+__device__ __forceinline__ void dealt_stretch(const FwdArgs& a, int w, Stretch& s) {
+    const int cols = a.B * a.H, per_group = a.cols_per_group * a.n_pairs;
+    const int group = w / per_group, at = w - group * per_group;
+    const int here = min(a.cols_per_group, cols - group * a.cols_per_group);
+    const int col = group * a.cols_per_group + at % here;
+    s.pair = a.n_pairs - 1 - at / here;
+    s.h = col % a.H;
+    s.b = col / a.H;
+    stretch_blocks<RULES>(a, kBlockM, s);
+    s.j0 = s.jb;
+    s.j1 = s.n[0] > s.n[1] ? s.n[0] : s.n[1];
+}
 template <int RULES> struct WorkLoop<0, RULES> {
     static constexpr int kSub = 1;
-    int w;
-    __device__ __forceinline__ WorkLoop(const FwdArgs&, const volatile RangeStart*) : w(blockIdx.x) {}
-    __device__ __forceinline__ bool more(const FwdArgs& a) const { return w < a.n_items; }
-    __device__ __forceinline__ void advance() { w += gridDim.x; }
-    __device__ __forceinline__ bool get(const FwdArgs& a, int, Stretch& s) const {
-        const int cols = a.B * a.H, per_group = a.cols_per_group * a.n_pairs;
-        const int group = w / per_group, at = w - group * per_group;
-        const int here = min(a.cols_per_group, cols - group * a.cols_per_group);
-        const int col = group * a.cols_per_group + at % here;
-        s.pair = a.n_pairs - 1 - at / here;
-        s.h = col % a.H;
-        s.b = col / a.H;
-        stretch_blocks<RULES>(a, kBlockM, s);
-        s.j0 = s.jb;
-        s.j1 = s.n[0] > s.n[1] ? s.n[0] : s.n[1];
-        return true;
+    volatile Deal* deal;
+    uint64_t* bars;                        // kSchedFull[2], kSchedEmpty[2], kClc
+    volatile uint32_t* abort_flag;
+    bool warp;                             // a warp reads, not a thread
+    int k, w;
+    __device__ __forceinline__ WorkLoop(volatile Deal* d, uint64_t* b, volatile uint32_t* f, bool wp) : deal(d), bars(b), abort_flag(f), warp(wp), k(0), w(-1) {}
+    __device__ __forceinline__ bool more(const FwdArgs&) {
+        bool there = mbar_wait(&bars[k & 1], (uint32_t)(k >> 1) & 1u, abort_flag);
+        if (warp) there = __all_sync(0xffffffffu, there);
+        w = there ? deal->w[k & 1] : -1;
+        if (there) { if (warp) mbar_arrive_warp(&bars[2 + (k & 1)]); else mbar_arrive(&bars[2 + (k & 1)]); }
+        ++k;
+        return w >= 0;
+    }
+    __device__ __forceinline__ void advance() {}
+    __device__ __forceinline__ bool get(const FwdArgs& a, int, Stretch& s) const { dealt_stretch<RULES>(a, w, s); return true; }
+};
+// The producer's side of it (one thread).
+template <int RULES> struct Dealer {
+    static constexpr int kSub = 1;
+    volatile Deal* deal;
+    uint64_t* bars;
+    volatile uint32_t* abort_flag;
+    int k, w, asked;
+    __device__ __forceinline__ Dealer(volatile Deal* d, uint64_t* b, volatile uint32_t* f) : deal(d), bars(b), abort_flag(f), k(0), w(blockIdx.x), asked(0) { leave(); }
+    __device__ __forceinline__ void leave() {
+        if (!mbar_wait(&bars[2 + (k & 1)], ((uint32_t)(k >> 1) & 1u) ^ 1u, abort_flag)) { w = -1; return; }
+        deal->w[k & 1] = w;
+        mbar_arrive(&bars[k & 1]);
+    }
+    __device__ __forceinline__ void ask() {
+        if (asked == k) { clc_request((uint32_t*)deal->answer, &bars[4]); ++asked; }
+    }
+    __device__ __forceinline__ bool more(const FwdArgs&) const { return w >= 0; }
+    __device__ __forceinline__ void advance() {
+        ask();
+        if (!mbar_wait(&bars[4], (uint32_t)k & 1u, abort_flag)) { w = -1; return; }
+        uint3 block;
+        w = clc_answer_block((const uint32_t*)deal->answer, block) ? (int)block.x : -1;
+        fence_proxy_async_smem();          // read before the next answer is written
+        ++k;
+        leave();
+    }
+    __device__ __forceinline__ bool get(const FwdArgs& a, int, Stretch& s) const { dealt_stretch<RULES>(a, w, s); return true; }
+    __device__ __forceinline__ void unwind() const {
+        for (int spin = 0; spin < 4096 && asked > 0 && !mbar_try_wait(&bars[4], (uint32_t)(asked - 1) & 1u); ++spin) {}
     }
 };
 template <int SCHED, int RULES> struct WorkLoop {       // split schedule: the CTA's range of units
@@ -385,8 +439,12 @@ template <int SCHED, int RULES> struct WorkLoop {       // split schedule: the C
 // Held in registers, the D = 128 kernel spilled 424 bytes instead of 60 and the chunk below took 152 us instead of 112.
 struct WalkRecord { int b, h, pair, at, units, cur_pair, cur_h, cur_b, cur_j0, cur_j1; };
 template <int SCHED, int RULES> struct SoftmaxLoop;
+template <> struct SoftmaxLoop<0, 0> : WorkLoop<0, 0> {
+    __device__ __forceinline__ SoftmaxLoop(const FwdArgs& a, const volatile RangeStart* r, volatile WalkRecord*) : WorkLoop<0, 0>(a, r) {}
+    __device__ __forceinline__ void again(const FwdArgs&, Stretch&) const {}
+};
 template <int RULES> struct SoftmaxLoop<0, RULES> : WorkLoop<0, RULES> {
-    __device__ __forceinline__ SoftmaxLoop(const FwdArgs& a, const volatile RangeStart* r, volatile WalkRecord*) : WorkLoop<0, RULES>(a, r) {}
+    using WorkLoop<0, RULES>::WorkLoop;
     __device__ __forceinline__ void again(const FwdArgs&, Stretch&) const {}
 };
 template <int SCHED, int RULES> struct SoftmaxLoop {
@@ -436,7 +494,7 @@ template <int D, bool BF16, int DROP, int PREC, int SCHED, int RULES = 0>
 __global__ void __launch_bounds__(kThreads, 1)
 fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_bias, const FwdArgs a) {
-    using Cfg = FwdCfg<D, PREC, SCHED>;
+    using Cfg = FwdCfg<D, PREC, SCHED, RULES>;
     constexpr bool FREE = SCHED != 0, TWIN = SCHED == 2;
     constexpr bool RULED = RULES != 0, ANY_D = PREC != 0 || RULED;
     constexpr bool NOTHING = FREE || RULED;     // a row may have seen nothing yet
@@ -461,6 +519,13 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     volatile uint32_t* abort_flag = (volatile uint32_t*)(tmem_slot + 1);
     [[maybe_unused]] float2* sMl = (float2*)((uint8_t*)(bars + Cfg::kNumBars) + 64);      // SCHED = 2: [128]
     volatile RangeStart* range = (volatile RangeStart*)(tmem_slot + 4);      // seven words of the 64 bytes behind the barriers
+    constexpr bool DEALT = Cfg::kDealt;
+    static_assert(!DEALT || (Cfg::kNumBars % 2 == 0 && sizeof(Deal) <= 48), "the answer to a request is 16-byte aligned");
+    // a role's walk (WorkLoop); `by_warp`: the role is a warp, not one thread
+    auto walk_of = [&](bool by_warp) {
+        if constexpr (DEALT) return WorkLoop<SCHED, RULES>((volatile Deal*)(tmem_slot + 4), bars + Cfg::kSchedFull, abort_flag, by_warp);
+        else return WorkLoop<SCHED, RULES>(a, range);
+    };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -469,7 +534,8 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             const bool wg_bar = (i >= Cfg::kPFull && i < Cfg::kPFull + 2) || (i >= Cfg::kPHalf && i < Cfg::kPHalf + 2) ||
                                 i == Cfg::kMlFull || i == Cfg::kORead || i >= Cfg::kBiasEmpty;
             const bool conv_bar = (i >= Cfg::kVConv && i < Cfg::kVConv + ST);
-            mbar_init(&bars[i], wg_bar ? 4u : (conv_bar ? 2u : 1u));
+            const bool read_bar = DEALT && i >= Cfg::kSchedEmpty && i < Cfg::kSchedEmpty + 2;         // MMA, converting and softmax warps
+            mbar_init(&bars[i], read_bar ? 11u : (DEALT && i >= Cfg::kSchedFull) ? 1u : (wg_bar ? 4u : (conv_bar ? 2u : 1u)));
         }
         if (lane == 0) wait_control_init(abort_flag, a.wait_limit_ms);
         fence_mbar_init();
@@ -501,7 +567,12 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             int q_loads[2] = {0, 0};
             bool ok = true;
             const uint32_t q_bytes = FREE ? (uint32_t)(Cfg::kNBox * 128 * pack * q_per_tile) : TILE;
-            for (WorkLoop<SCHED, RULES> wl(a, range); wl.more(a) && ok; wl.advance()) {
+            auto dealer = [&] {
+                if constexpr (DEALT) return Dealer<RULES>((volatile Deal*)(tmem_slot + 4), bars + Cfg::kSchedFull, abort_flag);
+                else return WorkLoop<SCHED, RULES>(a, range);
+            };
+            auto wl = dealer();
+            for (; wl.more(a) && ok; wl.advance()) {
                 for (int u = 0; u < wl.kSub && ok; ++u) {
                     Stretch st;
                     if (!wl.get(a, u, st)) continue;
@@ -523,6 +594,8 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     for (int j = st.j0; j < st.j1 && ok; ++j, ++kvc) {
                         const int s = kvc % ST;
                         const uint32_t ph = (uint32_t)(kvc / ST) & 1u;
+                        // (the answer is there when the pair ends, and no CTA that would get to that pair sooner goes without)
+                        if constexpr (DEALT) if (j + 3 >= st.j1) wl.ask();
                         ok = mbar_wait(&bars[Cfg::kKEmpty + s], ph ^ 1u, abort_flag);
                         if (!ok) break;
                         mbar_expect_tx(&bars[Cfg::kKFull + s], TILE);
@@ -544,6 +617,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     }
                 }
             }
+            if constexpr (DEALT) if (!ok) wl.unwind();
             if (!ok) {
                 // unwinding: let copies already issued land before the CTA gives up its
                 // shared memory (bounded: a copy that has not landed by now never will)
@@ -607,7 +681,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             int q_uses[2] = {0, 0};         // pairs that used tile t (Q_full phase)
             int p_waits[2] = {0, 0};        // P_t hand-offs so far (P_full phase)
             bool ok = true;
-            for (WorkLoop<SCHED, RULES> wl(a, range); TWIN && wl.more(a) && ok; wl.advance()) {
+            for (auto wl = walk_of(false); TWIN && wl.more(a) && ok; wl.advance()) {
                 Stretch st;
                 wl.get(a, 0, st);
                 // one tile: block j of the stretch belongs to accumulator set j & 1
@@ -650,11 +724,16 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
                 kvc += nb;
             }
-            for (WorkLoop<SCHED, RULES> wl(a, range); !TWIN && wl.more(a) && ok; wl.advance()) {
+            for (auto wl = walk_of(false); !TWIN && wl.more(a) && ok; wl.advance()) {
                 for (int u = 0; u < wl.kSub && ok; ++u) {
                     Stretch st;
                     if (!wl.get(a, u, st)) continue;
-                    const int nblk[2] = {st.count(0), st.count(1)};
+                    // tile t: blocks [b0[t], nblk[t]) of the stretch; a block between the tiles' may be neither's
+                    const int b0[2] = {RULED ? st.first(0) - st.j0 : 0, RULED ? st.first(1) - st.j0 : 0};
+                    int nblk[2] = {st.count(0), st.count(1)};
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        if (RULED && nblk[t]) nblk[t] += b0[t];
                     const int nmax = st.j1 - st.j0;
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
@@ -667,7 +746,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     tc_fence_after_sync();
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        if (nblk[t] == 0) continue;
+                        if (nblk[t] == 0 || b0[t] > 0) continue;
                         issue_s(t, kvc % ST);
                         mma_commit(&bars[Cfg::kSFull + t]);
                         if (nblk[t] == 1) mma_commit(&bars[Cfg::kQEmpty + t]);
@@ -684,21 +763,21 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         if (!ok) break;
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
-                            if (j < nblk[t]) {
+                            if (j < nblk[t] && j >= b0[t]) {
                                 // the first 64 keys of P_t arrive while the second 64 are still computed
                                 ok = mbar_wait(&bars[Cfg::kPHalf + t], (uint32_t)p_waits[t] & 1u, abort_flag);
                                 if (!ok) break;
                                 tc_fence_after_sync();
-                                issue_pv(t, vs, j > 0, 0);
+                                issue_pv(t, vs, j > b0[t], 0);
                                 ok = mbar_wait(&bars[Cfg::kPFull + t], (uint32_t)p_waits[t] & 1u, abort_flag);
                                 if (!ok) break;
                                 ++p_waits[t];
                                 tc_fence_after_sync();
-                                issue_pv(t, vs, j > 0, 1);
+                                issue_pv(t, vs, j > b0[t], 1);
                                 if (j == nblk[t] - 1) mma_commit(&bars[Cfg::kODone + t]);
                             }
                             if (t == 1) mma_commit(&bars[Cfg::kVEmpty + vs]);
-                            if (j + 1 < nblk[t]) {
+                            if (j + 1 < nblk[t] && j + 1 >= b0[t]) {
                                 if (!k_ready) {
                                     ok = mbar_wait(&bars[Cfg::kKFull + ks], kph, abort_flag);
                                     if (!ok) break;
@@ -710,6 +789,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                                 if (j + 2 == nblk[t]) mma_commit(&bars[Cfg::kQEmpty + t]);   // last S of tile t
                             }
                         }
+                        if (RULED && ok && j + 1 < nmax && !k_ready) ok = mbar_wait(&bars[Cfg::kKFull + ks], kph, abort_flag);
                         if (ok && j + 1 < nmax) mma_commit(&bars[Cfg::kKEmpty + ks]);
                     }
                     kvc += nmax;
@@ -724,7 +804,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const int ct = (warp - 10) * 32 + lane;
         int kvc = 0;
         bool ok = true;
-        for (WorkLoop<SCHED, RULES> wl(a, range); wl.more(a) && ok; wl.advance()) {
+        for (auto wl = walk_of(true); wl.more(a) && ok; wl.advance()) {
             for (int u = 0; u < wl.kSub && ok; ++u) {
                 Stretch st;
                 if (!wl.get(a, u, st)) continue;
@@ -802,14 +882,18 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         bool ok = true;
 
         if (FREE && threadIdx.x == 0) a.part_meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-        for (SoftmaxLoop<SCHED, RULES> wl(a, range, walk); wl.more(a) && ok; wl.advance()) {
+        auto my_walk = [&] {
+            if constexpr (DEALT) return SoftmaxLoop<SCHED, RULES>((volatile Deal*)(tmem_slot + 4), bars + Cfg::kSchedFull, abort_flag, true);
+            else return SoftmaxLoop<SCHED, RULES>(a, range, walk);
+        };
+        for (auto wl = my_walk(); wl.more(a) && ok; wl.advance()) {
             for (int u = 0; u < wl.kSub && ok; ++u) {
                 Stretch st;
                 if (!wl.get(a, u, st)) continue;
                 // blocks [j0, n) are mine, with one tile every other one of them
                 constexpr int kStep = TWIN ? 2 : 1;
                 const int tile = TWIN ? 0 : st.pair * 2 + t;
-                const int first = st.j0 + (TWIN ? t : 0), n = TWIN ? st.j1 : st.j0 + st.count(t), nk = st.nk;
+                const int first = TWIN ? st.j0 + t : (RULED ? st.first(t) : st.j0), n = TWIN ? st.j1 : first + st.count(t), nk = st.nk;
                 // my row: query i of head h; a packed tile may hold rows of no query (row_ok() is false)
                 int i = tile * q_per_tile + (FREE ? r / pack : r);
                 int h = FREE ? st.h * pack + r % pack : st.h;
@@ -817,7 +901,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 if (FREE && !st.whole()) {
                     // the slot my row's partial goes to: a range's first stretch takes slot 0 unless it starts a pair
                     const int64_t slot = 2 * (int64_t)blockIdx.x + (st.j0 == st.jb ? 1 : 0);
-                    if (!TWIN && n == st.j0 && row_ok()) a.part_ml[slot * a.part_rows + t * kBlockM + r] = make_float2(-INFINITY, -1.f);
+                    if (!TWIN && n == first && row_ok()) a.part_ml[slot * a.part_rows + t * kBlockM + r] = make_float2(-INFINITY, -1.f);
                     if (threadIdx.x == 0 && st.j0 == st.jb) {
                         // the pair starts here and goes on in the ranges of the CTAs behind this one
                         const int total = range->total, ctas = range->ctas;
@@ -828,7 +912,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         a.part_meta[blockIdx.x] = make_int4(st.b, st.h, st.pair, k);
                     }
                 }
-                if (!TWIN && n == st.j0) continue;
+                if (!TWIN && n == first) continue;
                 // a warp none of whose rows is a query of the call keeps the pipeline's hand-offs going and computes
                 // nothing: its rows of P are whatever tensor memory holds, and no other row of O depends on them
                 const bool idle = TWIN && __all_sync(0xffffffffu, !row_ok());
@@ -836,7 +920,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 float m = -INFINITY, l = 0.f;
                 // rules: my row's keys and position, and what a key's distance takes off in log2 units
                 [[maybe_unused]] int2 keys = make_int2(0, 0);
-                [[maybe_unused]] int at = 0;
+                [[maybe_unused]] int at = 0, bend = 0;
                 [[maybe_unused]] float slope = 0.f;
                 if constexpr (RULED) {
                     if (row_ok()) {
@@ -919,56 +1003,74 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     }
                     if (PREC == 2 && !ok) break;
                     if constexpr (RULES == 2) {
-                        // u = S scale / cap, tanh(u) in its place
-                        const uint64_t in2 = f2_pack(a.cap_in, a.cap_in);
-                        float z0 = 0.f, z1 = 0.f;
+                        // tanh(u) in the place of u = S scale / cap: by the short polynomial while the scores stay small beside
+                        // the cap, else by the long one, else by the exponential; `bend` is where the last block got to
+                        auto bent = [&](auto form) {
+                            const uint64_t in2 = f2_pack(a.cap_in, a.cap_in);
+                            float z0 = 0.f, z1 = 0.f;
 #pragma unroll
-                        for (int c = 0; c < 128; c += 4) {
-                            const uint64_t ua = f2_mul(f2_pack(SF(c), SF(c + 1)), in2), ub = f2_mul(f2_pack(SF(c + 2), SF(c + 3)), in2);
-                            const uint64_t za = f2_mul(ua, ua), zb = f2_mul(ub, ub);
-                            float x0, x1, x2, x3;
-                            f2_unpack(za, x0, x1);
-                            f2_unpack(zb, x2, x3);
-                            z0 = max3(z0, x0, x1);
-                            z1 = max3(z1, x2, x3);
-                            f2_unpack(f2_tanh_poly(ua, za), x0, x1);
-                            f2_unpack(f2_tanh_poly(ub, zb), x2, x3);
-                            SSET(c, x0); SSET(c + 1, x1); SSET(c + 2, x2); SSET(c + 3, x3);
-                        }
-                        if (__any_sync(0xffffffffu, fmaxf(z0, z1) > kTanhPolyMax * kTanhPolyMax)) {
-                            // some score beyond the polynomial: the block's scores again
+                            for (int c = 0; c < 128; c += 2 * kTanhAtOnce) {
+                                uint64_t u[kTanhAtOnce], z[kTanhAtOnce];
+#pragma unroll
+                                for (int e = 0; e < kTanhAtOnce; ++e) {
+                                    float x0, x1;
+                                    u[e] = f2_mul(f2_pack(SF(c + 2 * e), SF(c + 2 * e + 1)), in2);
+                                    z[e] = f2_mul(u[e], u[e]);
+                                    f2_unpack(z[e], x0, x1);
+                                    if (e & 1) z1 = max3(z1, x0, x1); else z0 = max3(z0, x0, x1);
+                                }
+                                f2_tanh_poly<decltype(form)::value>(u, z);
+#pragma unroll
+                                for (int e = 0; e < kTanhAtOnce; ++e) {
+                                    float x0, x1;
+                                    f2_unpack(u[e], x0, x1);
+                                    SSET(c + 2 * e, x0); SSET(c + 2 * e + 1, x1);
+                                }
+                            }
+                            const float top = decltype(form)::value ? kTanhLongMax : kTanhShortMax;
+                            return !__any_sync(0xffffffffu, fmaxf(z0, z1) > top * top);
+                        };
+                        auto again = [&] {
 #pragma unroll
                             for (int c = 0; c < 4; ++c) tmem_ld_32x32(tS + c * 32, sr[c]);
                             tmem_wait_ld();
+                        };
+                        if (bend == 0 && !bent(std::false_type{})) { bend = 1; again(); }
+                        if (bend == 1 && !bent(std::true_type{})) { bend = 2; again(); }
+                        if (bend == 2) {
 #pragma unroll
                             for (int c = 0; c < 128; ++c) SSET(c, tanh_any(SF(c) * a.cap_in));
                         }
                     }
                     if constexpr (RULED) {
                         if (a.rules.slopes) {
-                            // x = S scale - slope |position - key|, whole numbers that fp32 holds exactly up to 2^24
+                            // x = S scale - slope |position - key|
                             const float from = (float)(at - col0), mul = RULES == 2 ? a.cap_out : a.scale_log2;
-                            const uint64_t mul2 = f2_pack(mul, mul), step2 = f2_pack(-2.f, -2.f);
-                            uint64_t d2 = f2_pack(from, from - 1.f);
+                            const uint64_t mul2 = f2_pack(mul, mul);
                             if (__any_sync(0xffffffffu, at < min(col0 + kBlockN, keys.y) - 1)) {        // keys ahead of a row
-#pragma unroll
-                                for (int c = 0; c < 128; c += 2) {
-                                    float d0, d1, x0, x1;
-                                    f2_unpack(d2, d0, d1);
-                                    f2_unpack(f2_mul(f2_pack(SF(c), SF(c + 1)), mul2), x0, x1);
-                                    SSET(c, fmaf(-slope, fabsf(d0), x0));
-                                    SSET(c + 1, fmaf(-slope, fabsf(d1), x1));
-                                    d2 = f2_add(d2, step2);
-                                }
-                            } else {
-                                const uint64_t slope2 = f2_pack(-slope, -slope);
+                                // (distances are whole numbers, exact up to 2^24)
 #pragma unroll
                                 for (int c = 0; c < 128; c += 2) {
                                     float x0, x1;
-                                    f2_unpack(f2_fma(d2, slope2, f2_mul(f2_pack(SF(c), SF(c + 1)), mul2)), x0, x1);
+                                    f2_unpack(f2_mul(f2_pack(SF(c), SF(c + 1)), mul2), x0, x1);
+                                    SSET(c, fmaf(-slope, fabsf(from - (float)c), x0));
+                                    SSET(c + 1, fmaf(-slope, fabsf(from - (float)(c + 1)), x1));
+                                }
+                            } else {
+                                // what is taken off falls by the slope from column to column; four chains of sixteen additions,
+                                // each off by 2^-24 of what is taken off
+                                const uint64_t step2 = f2_pack(8.f * slope, 8.f * slope);
+                                uint64_t off2[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) off2[e] = f2_pack(-slope * (from - (float)(2 * e)), -slope * (from - (float)(2 * e + 1)));
+#pragma unroll
+                                for (int c = 0; c < 128; c += 2) {
+                                    float x0, x1;
+                                    uint64_t& o2 = off2[(c >> 1) & 3];
+                                    f2_unpack(f2_fma(f2_pack(SF(c), SF(c + 1)), mul2, o2), x0, x1);
+                                    o2 = f2_add(o2, step2);
                                     SSET(c, x0);
                                     SSET(c + 1, x1);
-                                    d2 = f2_add(d2, step2);
                                 }
                             }
                         }
@@ -1087,7 +1189,8 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         f2_unpack(f2_fma(f2_pack(SF(c), SF(c + 1)), c2, nm2), x0, x1);
                         f2_unpack(f2_fma(f2_pack(SF(c + 2), SF(c + 3)), c2, nm2), x2, x3);
                         p0 = ex2(x0); p1 = ex2(x1);
-                        if ((c >> 2) % Cfg::kPolyPeriod == 0) ex2_poly2(x2, x3, p2, p3);
+                        // (a cap's tanh keeps the FMA pipes busy enough)
+                        if (RULES != 2 && (c >> 2) % Cfg::kPolyPeriod == 0) ex2_poly2(x2, x3, p2, p3);
                         else { p2 = ex2(x2); p3 = ex2(x3); }
                         la = f2_add(la, f2_pack(p0, p1));
                         lb = f2_add(lb, f2_pack(p2, p3));
@@ -1527,17 +1630,18 @@ int launch(const fa_b200_params& p, void* ws, size_t ws_bytes, const Rules* rule
     auto kernel = fwd_sm100_kernel<D, BF16, 0, PREC, 0, RULES>;
     if constexpr (RULES == 0) if (drop == 2) kernel = fwd_sm100_kernel<D, BF16, 2, PREC, 0>;
     if constexpr (PREC != 2 && RULES == 0) if (drop == 1) kernel = fwd_sm100_kernel<D, BF16, 1, PREC, 0>;      // bias_is_staged()
-    int smem = FwdCfg<D, PREC, 0>::kSmemBytes;
+    int smem = FwdCfg<D, PREC, 0, RULES>::kSmemBytes;
     if constexpr (PREC == 0) {
         if (plan.sched == 1) kernel = fwd_sm100_kernel<D, BF16, 0, PREC, 1, RULES>;
-        if (plan.sched == 2) { kernel = fwd_sm100_kernel<D, BF16, 0, PREC, 2, RULES>; smem = FwdCfg<D, PREC, 2>::kSmemBytes; }
+        if (plan.sched == 2) { kernel = fwd_sm100_kernel<D, BF16, 0, PREC, 2, RULES>; smem = FwdCfg<D, PREC, 2, RULES>::kSmemBytes; }
     }
     {
         static std::mutex mu;
         static uint64_t done[5] = {0, 0, 0, 0, 0};
         FA_CUDA_CHECK(set_smem_limit_once(kernel, smem, p.device, &done[plan.sched ? 2 + plan.sched : drop], &mu));
     }
-    const int grid = plan.sched ? plan.ctas : (a.n_items < sms ? a.n_items : sms);     // one persistent CTA per SM
+    // one persistent CTA per SM; dealt pairs: a block a pair
+    const int grid = plan.sched ? plan.ctas : (FwdCfg<D, PREC, 0, RULES>::kDealt || a.n_items < sms ? a.n_items : sms);
     kernel<<<grid, kThreads, smem, (cudaStream_t)p.stream>>>(mq, mk, mv, mb, a);
     FA_CUDA_CHECK(cudaGetLastError());
     if constexpr (PREC == 0) if (plan.sched) {

@@ -4,21 +4,39 @@
 
 namespace fa {
 
-// tanh(u) for |u| <= 1 on the FMA pipes, z = u * u: an odd polynomial with the least largest relative error there, 5.9e-7
-// (fitted by reweighted least squares).  A score of size s is off by 5.9e-7 s: the rounding of a sum of products of size s.
-// The special-function unit, which the softmax keeps busiest, would be asked twice for each score.
-constexpr float kTanhPolyMax = 1.f;
+// tanh(u) on the FMA pipes, z = u * u: odd polynomials with the least largest relative error (fitted by reweighted least
+// squares), four terms for |u| <= 1/2, 5.5e-7, six for |u| <= 1, 5.9e-7.  A score of size s is off by 6e-7 s: the rounding of
+// a sum of products of size s.  The special-function unit, which the softmax keeps busiest, would be asked twice for each.
+constexpr float kTanhShortMax = 0.5f, kTanhLongMax = 1.f;
+template <bool LONG>
 __device__ __forceinline__ uint64_t f2_tanh_poly(uint64_t u, uint64_t z) {
     using namespace ptx;
-    const uint64_t c0 = f2_pack(0.999999414f, 0.999999414f), c1 = f2_pack(-0.333290423f, -0.333290423f);
-    const uint64_t c2 = f2_pack(0.132814332f, 0.132814332f), c3 = f2_pack(-0.0516056576f, -0.0516056576f);
-    const uint64_t c4 = f2_pack(0.0167430985f, 0.0167430985f), c5 = f2_pack(-0.00306705425f, -0.00306705425f);
-    uint64_t r = f2_fma(c5, z, c4);
-    r = f2_fma(r, z, c3);
-    r = f2_fma(r, z, c2);
-    r = f2_fma(r, z, c1);
-    r = f2_fma(r, z, c0);
+    constexpr float c[6] = {LONG ? 0.999999414f : 0.999999456f, LONG ? -0.333290423f : -0.333263176f, LONG ? 0.132814332f : 0.13190294f,
+                            LONG ? -0.0516056576f : -0.0444021663f, 0.0167430985f, -0.00306705425f};
+    uint64_t r = LONG ? f2_fma(f2_pack(c[5], c[5]), z, f2_pack(c[4], c[4])) : f2_pack(c[3], c[3]);
+    if (LONG) r = f2_fma(r, z, f2_pack(c[3], c[3]));
+    r = f2_fma(r, z, f2_pack(c[2], c[2]));
+    r = f2_fma(r, z, f2_pack(c[1], c[1]));
+    r = f2_fma(r, z, f2_pack(c[0], c[0]));
     return f2_mul(r, u);
+}
+// The same for several pairs step by step, so that no step waits for the one before it; u is replaced.
+constexpr int kTanhAtOnce = 8;
+template <bool LONG>
+__device__ __forceinline__ void f2_tanh_poly(uint64_t (&u)[kTanhAtOnce], const uint64_t (&z)[kTanhAtOnce]) {
+    using namespace ptx;
+    constexpr float c[6] = {LONG ? 0.999999414f : 0.999999456f, LONG ? -0.333290423f : -0.333263176f, LONG ? 0.132814332f : 0.13190294f,
+                            LONG ? -0.0516056576f : -0.0444021663f, 0.0167430985f, -0.00306705425f};
+    constexpr int n = LONG ? 6 : 4;
+    uint64_t r[kTanhAtOnce];
+#pragma unroll
+    for (int e = 0; e < kTanhAtOnce; ++e) r[e] = f2_fma(f2_pack(c[n - 1], c[n - 1]), z[e], f2_pack(c[n - 2], c[n - 2]));
+#pragma unroll
+    for (int k = n - 3; k >= 0; --k)
+#pragma unroll
+        for (int e = 0; e < kTanhAtOnce; ++e) r[e] = f2_fma(r[e], z[e], f2_pack(c[k], c[k]));
+#pragma unroll
+    for (int e = 0; e < kTanhAtOnce; ++e) u[e] = f2_mul(r[e], u[e]);
 }
 // tanh of any u: 1 - 2 / (1 + e^2u), off by at most 2^-22; 1 and -1 far out, a NaN stays one.
 __device__ __forceinline__ float tanh_any(float u) {
