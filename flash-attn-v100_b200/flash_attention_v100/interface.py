@@ -21,7 +21,7 @@ import torch.distributed as dist
 from .config import get_enhanced_config
 from .ops.attention import FlashAttentionV100Function, native_call
 from .ops.key_ranges import KeyRanges, build_key_ranges
-from .ops.rules import RuledAttentionFunction, check_rules
+from .ops.rules import RuledAttentionFunction, check_rules, native_call_rules
 from .utils import validate_inputs as _validate_inputs
 
 log = logging.getLogger("flash_attention_v100")
@@ -484,13 +484,17 @@ def flash_attention_v100_with_rules(
     Keys and values behind an entry's counts (or outside every range) may be unwritten memory in a call without gradients; in
     a training step they have to be numbers.  Gradients are bit-reproducible.  One GPU: that of the tensors.
     """
+    manager = get_flash_attention_manager()
+    profile = manager.enable_profiling or enable_profiling
+    if type(key_ranges) is KeyRanges and not causal and key_lengths is None and not profile and causal_alignment in ("top_left", "bottom_right"):
+        result = native_call_rules(q, k, v, scale, score_cap, distance_slopes, key_ranges)
+        if result is not None:
+            return result if return_softmax_lse else result[0]
     q, k, v, scale = _validate_inputs(q, k, v, scale)
     if key_ranges is not None and (causal or key_lengths is not None):
         raise ValueError("key_ranges say which keys are seen: causal and key_lengths cannot be combined with them")
     shift = _causal_shift(causal, causal_alignment, q.shape[1], k.shape[1], key_lengths)
     cap, slopes = check_rules(q, k, score_cap, distance_slopes, key_ranges)
-    manager = get_flash_attention_manager()
-    profile = manager.enable_profiling or enable_profiling
     if profile:
         start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         start.record(torch.cuda.current_stream(q.device))

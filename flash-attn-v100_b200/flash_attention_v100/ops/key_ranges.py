@@ -65,6 +65,19 @@ def _lengths(name: str, t: Optional[torch.Tensor], shapes, device: torch.device)
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _device_index(device, *tensors) -> Optional[int]:
+    """The CUDA device the ranges are built on, None where there is no GPU or it is another kind of device."""
+    if device is None:
+        device = next((t.device for t in tensors if isinstance(t, torch.Tensor)), None)
+        if device is None:
+            return torch.cuda.current_device() if torch.cuda.is_available() else None
+    elif not isinstance(device, torch.device):
+        device = torch.device(device)
+    if device.type != "cuda" or not torch.cuda.is_available():
+        return None
+    return torch.cuda.current_device() if device.index is None else device.index
+
+
 def build_key_ranges(seq_q: int, seq_k: int, *, batch: int = 1, causal: bool = False, window: Optional[int] = None,
                      document_offsets: Optional[torch.Tensor] = None, prefix_lengths: Optional[torch.Tensor] = None,
                      key_lengths: Optional[torch.Tensor] = None, query_offsets: Union[torch.Tensor, int, None] = None,
@@ -89,6 +102,14 @@ def build_key_ranges(seq_q: int, seq_k: int, *, batch: int = 1, causal: bool = F
         out: an earlier KeyRanges of the same sizes, written anew in place (a captured graph reads it again).  A backward
             whose forward read its earlier contents raises
     """
+    if out is None and rows is None and (window is None or window >= 1) and not torch.compiler.is_compiling():
+        # (None: a form the native operator does not serve, or one that is refused below)
+        starts, start = (query_offsets, 0) if isinstance(query_offsets, torch.Tensor) else (None, query_offsets or 0)
+        index = _device_index(device, document_offsets, prefix_lengths, key_lengths, starts)
+        if index is not None:
+            result = _cabi.load_op().key_ranges(seq_q, seq_k, batch, bool(causal), window or 0, document_offsets, prefix_lengths, key_lengths, starts, start, index)
+            if result is not None:
+                return KeyRanges(result[0], result[1], batch, seq_q, seq_k)
     if seq_q < 0 or seq_k < 0 or batch < 0:
         raise ValueError(f"sizes must not be negative (seq_q {seq_q}, seq_k {seq_k}, batch {batch})")
     if window is not None and not 1 <= window <= _INT32_MAX:

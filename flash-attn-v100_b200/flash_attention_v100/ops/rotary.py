@@ -131,6 +131,10 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, inv_f
         interleaved: pairs are neighbouring columns 2i, 2i + 1 instead of i, i + pairs
         inplace: write over q and k (no gradients), e.g. rows of a key cache
     """
+    if not inplace and type(attention_factor) is float and not torch.compiler.is_compiling():
+        result = _cabi.load_op().rotary(q, k, positions, inv_freq, bool(interleaved), attention_factor)
+        if result is not None:
+            return result
     xs = (q,) if k is None else (q, k)
     for name, x in zip("qk", xs):
         if not isinstance(x, torch.Tensor):

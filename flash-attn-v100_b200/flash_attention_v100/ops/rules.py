@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from ..kernels import _cabi
-from .attention import _base_params, _status_word, _tensor4, saves_output_residual
+from .attention import _base_params, _tensor4, _variant_override, saves_output_residual
 from ..utils import _last_dim_contiguous
 from .key_ranges import KeyRanges
 
@@ -51,6 +51,13 @@ def check_rules(q: torch.Tensor, k: torch.Tensor, score_cap: Optional[float], sl
         if ranges.device != q.device:
             raise ValueError("key_ranges must be on the same device as input tensors")
     return cap, slopes
+
+
+def native_call_rules(q, k, v, scale, score_cap, slopes, ranges: KeyRanges):
+    """(o, lse) by the native operator, or None where it does not serve the call (as attention.native_call)."""
+    if torch.compiler.is_compiling() or getattr(_variant_override, "value", _cabi.VARIANT_AUTO) != _cabi.VARIANT_AUTO:
+        return None
+    return _cabi.load_op().attention_rules(q, k, v, scale, score_cap, slopes, ranges.plan, ranges.batch, ranges.seq_q, ranges.seq_k)
 
 
 def launch_forward_rules(q, k, v, scale, cap, slopes, plan, plan_batch, o_residual=None, split_keys=False):

@@ -297,3 +297,61 @@ def test_a_decoding_step_in_a_graph(device):
             qr = rotary64(q, at.to(device), f, False).to(torch.bfloat16)
             want = attention64(qr, k, v, see, at, D ** -0.5, 25.0, slopes)[0]
             assert rel(o, want) <= 2 * TOLERANCE[torch.bfloat16]      # (q's rounding may fall on the other side)
+
+
+@pytest.mark.parametrize("wants", ["qkv", "k", "none"])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_native_and_general_forms_agree(device, dtype, wants):
+    """The native operator and the Python one: same bits, also under a mode that watches operators."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    t = TYPES[dtype]
+    base = _inputs(2, 90, 90, 4, 2, 64, t, device)
+    offsets = torch.tensor([[0, 40, 90], [0, 0, 77]], dtype=torch.int32, device=device)
+    f = fa.rotary_frequencies(64, device=device)[0]
+    slopes = _slopes(4, device).float()
+    got = []
+    for native in (True, False):
+        q, k, v, g = (x.clone().requires_grad_(n in wants) for x, n in zip(base, "qkvg"))
+
+        def step():
+            r = fa.build_key_ranges(90, 90, batch=2, causal=True, document_offsets=offsets)
+            turned = fa.rotary_embedding(q, k, inv_freq=f, positions=r.positions, attention_factor=1.5)
+            o, lse = fa.flash_attention_v100_with_rules(*turned, v, score_cap=9.0, distance_slopes=slopes, key_ranges=r, return_softmax_lse=True)
+            return r, turned, o, lse
+
+        if native:
+            r, turned, o, lse = step()
+        else:
+            with Watch():
+                r, turned, o, lse = step()
+        if wants != "none":
+            o.backward(g)
+        assert o.requires_grad == (wants != "none") and not lse.requires_grad
+        got.append([r.first, r.end, r.positions, turned[0], turned[1], o, lse, q.grad, k.grad, v.grad])
+    for a, b in zip(*got):
+        assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+
+
+def test_a_changed_operand_is_noticed(device):
+    q, k, v, g = _inputs(1, 64, 64, 1, 1, 64, torch.float16, device)
+    r = fa.build_key_ranges(64, 64, causal=True, device=device)
+    q.requires_grad_(True)
+    o = fa.flash_attention_v100_with_rules(q, k, v, key_ranges=r)
+    k.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.backward(g)
+
+
+def test_gradient_of_a_gradient_is_refused(device):
+    q, k, v, g = _inputs(1, 64, 64, 1, 1, 64, torch.float16, device)
+    r = fa.build_key_ranges(64, 64, causal=True, device=device)
+    q.requires_grad_(True)
+    o = fa.flash_attention_v100_with_rules(q, k, v, key_ranges=r)
+    d, = torch.autograd.grad(o.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(d.sum(), q)
