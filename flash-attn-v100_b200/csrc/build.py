@@ -17,7 +17,7 @@ OP_SOURCE = "torch_op.cpp"
 SOURCES = ["host_api.cu", "simt_kernels.cu", "fwd_sm100.cu", "fwd_tf32_sm100.cu", "bwd_sm100.cu", "bwd_f32_sm100.cu", "combine.cu", "compact.cu",
            "fwd_pair_sm100.cu", "bwd_pair_sm100.cu", "key_ranges.cu", "rotary.cu",
            "fwd_rules_sm100.cu", "bwd_rules_sm100.cu"]
-HEADERS = ["fa_common.cuh", "philox.cuh", "sm100_ptx.cuh", "tma_host.cuh", "tile_config.cuh", "score_rules.cuh",
+HEADERS = ["fa_common.cuh", "philox.cuh", "sm100_ptx.cuh", "tma_host.cuh", "tile_config.cuh", "score_rules.cuh", "fwd_decode.cuh",
            os.path.join("..", "..", "include", "fa_b200.h")]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -165,6 +165,7 @@ struct FwdArgs {
     Rules rules;
     float cap_in, cap_out;         // u = S * cap_in, x = tanh(u) * cap_out (log2 units)
     int cols_per_group;            // whole pairs: (batch, head) columns per group of work items
+    const void* q; int64_t q_sb, q_sn, q_sh;               // fwd_decode_kernel
 };
 
 // A stretch of work: key blocks [j0, j1) of a pair.  n[t]: behind the last block of the pair's tile t
@@ -1457,10 +1458,14 @@ __global__ void __launch_bounds__(256) fwd_merge_kernel(const FwdArgs a) {
     if (warp == 0) a.lse[((int64_t)b * a.H + h) * a.Nq + i] = kLn2 * ((m - kPShift) + log2f(l));
 }
 
+#ifdef FA_RULES_INSTANCES
+#include "fwd_decode.cuh"
+#endif
+
 // How a call's query rows are tiled and its work divided.
 struct FwdPlan {
     int pack, q_per_tile, heads, n_pairs;
-    int sched;                     // FwdCfg's SCHED
+    int sched;                     // FwdCfg's SCHED; 3: fwd_decode_kernel
     int ctas, part_rows;           // split schedule: ranges, rows per slot
     int start_cost;                // FwdArgs
     size_t ml_off, meta_off, bytes;        // workspace: partial sums | maxima and row sums | ranges' pairs
@@ -1507,6 +1512,7 @@ constexpr int kMergeUnits = 4;
 // of 2048-4096 keys, H32 Hkv8 D128 84 -> 82.  Without counts pairs are alike, and in the kernel of several tiles the
 // walk with starts took registers from the softmax (700 queries on 8892 keys 93 -> 100 us).
 constexpr int kLongRange = 8;
+constexpr int kDecodeRows = 16;        // rows of a K/V head that fwd_decode_kernel serves
 FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, bool ruled = false) {
     FwdPlan pl;
     memset(&pl, 0, sizeof(pl));
@@ -1514,6 +1520,25 @@ FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, bool r
     pl.pack = 1; pl.q_per_tile = kBlockM; pl.heads = p.H; pl.n_pairs = pairs_of(kBlockM);
     if (!free || sms <= 0 || p.Nq > (1 << 20) || dropout_threshold(p.dropout_p) != 0u) return pl;
     const int group = p.H / p.Hkv;
+    auto scratch = [&](int rows) {
+        pl.part_rows = (int)align_up((size_t)rows, 32);
+        const size_t slots = 2 * (size_t)pl.ctas * pl.part_rows;
+        pl.ml_off = align_up(slots * D * sizeof(float), 256);
+        pl.meta_off = pl.ml_off + align_up(slots * sizeof(float2), 256);
+        pl.bytes = pl.meta_off + align_up((size_t)pl.ctas * sizeof(int4), 256);
+    };
+    if (ruled && (int64_t)p.Nq * group <= kDecodeRows) {
+        // the rows of a K/V head together, a range of its key blocks a CTA; a pair's end (the warps' sums) takes about a block's time
+        const int64_t units = (int64_t)p.B * p.Hkv * ((p.Nk + kBlockN - 1) / kBlockN);
+        if (units < (1 << 28)) {
+            pl.pack = group; pl.q_per_tile = kBlockM / group; pl.heads = p.Hkv; pl.n_pairs = 1;
+            pl.ctas = (int)(units < sms ? units : sms);
+            pl.sched = 3;
+            pl.start_cost = units / pl.ctas >= kLongRange ? 1 : 0;
+            scratch(p.Nq * group);
+            return pl;
+        }
+    }
     int64_t col = column_units(p, kBlockM, pl.n_pairs);
     const int items = p.causal ? (pl.n_pairs + 1) / 2 : pl.n_pairs;              // per column: a pair, or a pair and its mirror
     const int64_t n_items = (int64_t)items * p.B * p.H;
@@ -1532,12 +1557,7 @@ FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, bool r
         pl.sched = one_tile ? 2 : 1;
         pl.start_cost = counts && one_tile && ranges >= kLongRange ? 3 : 0;
         const int tiles = (int)(((int64_t)p.Nq + pl.q_per_tile - 1) / pl.q_per_tile);
-        const int rows = tiles > 1 ? 2 * kBlockM : p.Nq * pl.pack;
-        pl.part_rows = (int)align_up((size_t)rows, 32);
-        const size_t slots = 2 * (size_t)pl.ctas * pl.part_rows;
-        pl.ml_off = align_up(slots * D * sizeof(float), 256);
-        pl.meta_off = pl.ml_off + align_up(slots * sizeof(float2), 256);
-        pl.bytes = pl.meta_off + align_up((size_t)pl.ctas * sizeof(int4), 256);
+        scratch(tiles > 1 ? 2 * kBlockM : p.Nq * pl.pack);
         return pl;
     }
     return plan_schedule(p, D, sms, false);
@@ -1577,6 +1597,7 @@ int launch(const fa_b200_params& p, void* ws, size_t ws_bytes, const Rules* rule
         const int64_t col_bytes = 2 * (int64_t)p.Nk * D * 2 / (p.H / p.Hkv);
         const int64_t g = (int64_t)tile::kFwdGroupBytes / (col_bytes > 0 ? col_bytes : 1), cols = (int64_t)p.B * p.H;
         a.cols_per_group = (int)(g < 1 ? 1 : (g > cols ? cols : g));
+        a.q = p.q.ptr; a.q_sb = p.q.stride_b; a.q_sn = p.q.stride_n; a.q_sh = p.q.stride_h;
     }
     a.bias_b = bias_b; a.bias_h = bias_h;
     a.o = p.o.ptr;
@@ -1635,15 +1656,26 @@ int launch(const fa_b200_params& p, void* ws, size_t ws_bytes, const Rules* rule
         if (plan.sched == 1) kernel = fwd_sm100_kernel<D, BF16, 0, PREC, 1, RULES>;
         if (plan.sched == 2) { kernel = fwd_sm100_kernel<D, BF16, 0, PREC, 2, RULES>; smem = FwdCfg<D, PREC, 2, RULES>::kSmemBytes; }
     }
+#ifdef FA_RULES_INSTANCES
+    if (plan.sched == 3) {
+        static std::mutex mu;
+        static uint64_t done = 0;
+        auto decode = fwd_decode_kernel<D, BF16, RULES>;
+        FA_CUDA_CHECK(set_smem_limit_once(decode, DecodeCfg<D>::kSmemBytes, p.device, &done, &mu));
+        decode<<<plan.ctas, 288, DecodeCfg<D>::kSmemBytes, (cudaStream_t)p.stream>>>(mk, mv, a);
+        FA_CUDA_CHECK(cudaGetLastError());
+        if (p.Nk <= kBlockN) return FA_OK;         // a block a pair: none is cut
+    } else
+#endif
     {
         static std::mutex mu;
         static uint64_t done[5] = {0, 0, 0, 0, 0};
         FA_CUDA_CHECK(set_smem_limit_once(kernel, smem, p.device, &done[plan.sched ? 2 + plan.sched : drop], &mu));
-    }
     // one persistent CTA per SM; dealt pairs: a block a pair
     const int grid = plan.sched ? plan.ctas : (FwdCfg<D, PREC, 0, RULES>::kDealt || a.n_items < sms ? a.n_items : sms);
     kernel<<<grid, kThreads, smem, (cudaStream_t)p.stream>>>(mq, mk, mv, mb, a);
     FA_CUDA_CHECK(cudaGetLastError());
+    }
     if constexpr (PREC == 0) if (plan.sched) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)plan.ctas, (unsigned)(plan.part_rows / 32));
