@@ -194,9 +194,14 @@ __device__ __forceinline__ int2 tile_hull(const FwdArgs& a, int b, int q_per_til
     }
     const int last = (row0 + q_per_tile < a.Nq ? row0 + q_per_tile : a.Nq) - 1;
     int2 r = make_int2(0x7fffffff, 0);
-    for (int i = row0 / 16; i <= last / 16; ++i) {
-        const int2 h = a.rules.q_parts[b * a.rules.q_parts_b + i];
-        if (h.y > 0) { r.x = min(r.x, h.x); r.y = max(r.y, h.y); }
+    const int2* parts = a.rules.q_parts + b * a.rules.q_parts_b;
+    for (int i = row0 / 16; i <= last / 16; i += 4) {              // (four loads on their way at once)
+        int2 h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = parts[min(i + e, last / 16)];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (h[e].y > 0) { r.x = min(r.x, h[e].x); r.y = max(r.y, h[e].y); }
     }
     return r.y > 0 ? make_int2(max(r.x, 0), min(r.y, a.Nk)) : make_int2(0, 0);
 }
@@ -286,7 +291,20 @@ __device__ __forceinline__ void find_range(const FwdArgs& a, int lane, volatile 
         return sum;
     };
     int total = 0, col = 0;
-    if (RULES || a.kv_len) {
+    // rules: a pair's blocks are two loads and more away.  Columns of many pairs a lane a pair (one by one it took 14 us of a
+    // chunk's 134: 700 queries on 8892 keys), one plan for all batch entries once
+    const bool same = RULES && a.rules.q_tiles_b == 0, wide = RULES && a.n_pairs > 4;
+    auto column_by_warp = [&](int b) {
+        int sum = 0;
+        for (int pr = lane; pr < a.n_pairs; pr += 32) sum += pair_blocks<RULES>(a, b, pr, a.Nk) + c0;
+        return __shfl_sync(0xffffffffu, warp_scan(sum, lane), 31);
+    };
+    if (same) {
+        col = column_by_warp(0);
+        total = a.B * a.heads * col;
+    } else if (wide) {
+        for (int b = 0; b < a.B; ++b) total += a.heads * column_by_warp(b);
+    } else if (RULES || a.kv_len) {
         for (int b = lane; b < a.B; b += 32) total += a.heads * column(b);
         total = __shfl_sync(0xffffffffu, warp_scan(total, lane), 31);
     } else {
@@ -299,7 +317,14 @@ __device__ __forceinline__ void find_range(const FwdArgs& a, int lane, volatile 
     const int first = range_begin((int)blockIdx.x, ctas, total);
     const int units = range_begin((int)blockIdx.x + 1, ctas, total) - first;
     int at = first, b;
-    if (RULES || a.kv_len) {
+    if (wide && !same) {
+        for (b = 0; b < a.B - 1; ++b) {
+            col = column_by_warp(b);
+            if (at < a.heads * col) break;
+            at -= a.heads * col;
+        }
+        if (b == a.B - 1) col = column_by_warp(b);
+    } else if (!same && (RULES || a.kv_len)) {
         b = warp_find(a.B, lane, at, [&](int i) { return a.heads * column(i); });
         col = column(b);
     } else {
@@ -920,15 +945,23 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 const uint32_t bh = dropout_column(a.rng, st.b, h);
                 float m = -INFINITY, l = 0.f;
                 // rules: my row's keys and position, and what a key's distance takes off in log2 units
-                [[maybe_unused]] int2 keys = make_int2(0, 0);
-                [[maybe_unused]] int at = 0, bend = 0;
+                // A row that sees nothing, or is none, takes everything: it would have every block of its warp masked.  The
+                // former's results are put aside at the end.
+                [[maybe_unused]] int2 keys = make_int2(0, 0x7fffffff);
+                [[maybe_unused]] int at = 0, bend = 0, all_from = 0, all_to = 0;      // keys that all of my warp's rows see
                 [[maybe_unused]] float slope = 0.f;
+                [[maybe_unused]] bool dead = false, ahead = false;                    // ahead: some row of my warp sees keys behind its position
                 if constexpr (RULED) {
                     if (row_ok()) {
-                        keys = a.rules.rows[st.b * a.rules.rows_b + i];
+                        const int2 x = a.rules.rows[st.b * a.rules.rows_b + i];
+                        dead = x.x >= x.y;
+                        if (!dead) keys = x;
                         if (a.rules.slopes) slope = a.rules.slopes[h] * kLog2e;
                     }
                     at = i + a.rules.origin[st.b * a.rules.origin_b];
+                    all_from = __reduce_max_sync(0xffffffffu, keys.x);
+                    all_to = __reduce_min_sync(0xffffffffu, keys.y);
+                    ahead = __any_sync(0xffffffffu, row_ok() && !dead && at < keys.y - 1);
                 }
                 // my row of the bias (a row beyond Nq, whose results nobody keeps, reads the last one)
                 const float* brow = nullptr;
@@ -1048,7 +1081,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                             // x = S scale - slope |position - key|
                             const float from = (float)(at - col0), mul = RULES == 2 ? a.cap_out : a.scale_log2;
                             const uint64_t mul2 = f2_pack(mul, mul);
-                            if (__any_sync(0xffffffffu, at < min(col0 + kBlockN, keys.y) - 1)) {        // keys ahead of a row
+                            if (ahead && __any_sync(0xffffffffu, at < min(col0 + kBlockN, keys.y) - 1)) {
                                 // (distances are whole numbers, exact up to 2^24)
 #pragma unroll
                                 for (int c = 0; c < 128; c += 2) {
@@ -1075,8 +1108,8 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                                 }
                             }
                         }
-                        const int lo = keys.x - col0, hi = keys.y - col0;             // the columns my row sees
-                        if (__any_sync(0xffffffffu, lo > 0 || hi < kBlockN)) {
+                        if (col0 < all_from || col0 + kBlockN > all_to) {
+                            const int lo = keys.x - col0, hi = keys.y - col0;         // the columns my row sees
 #pragma unroll
                             for (int c = 0; c < 128; ++c)
                                 if (c < lo || c >= hi) SSET(c, -INFINITY);
@@ -1242,6 +1275,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
                 if (!ok) break;
 
+                if (RULED && dead) { m = -INFINITY; l = 0.f; }
                 // ---- epilogue: O_t / l -> 16 bit -> global, straight from registers
                 if constexpr (FREE) {
                     wl.again(a, st);
@@ -1301,6 +1335,10 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         }
                     } else {
                         tmem_wait_ld();
+                    }
+                    if (RULED && dead) {               // (0 times what it has summed may be no zero)
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) orr[c] = 0u;
                     }
                 };
                 if (FREE && !st.whole()) {
