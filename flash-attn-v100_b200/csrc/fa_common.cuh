@@ -123,6 +123,7 @@ struct Rules {
     int64_t rows_b, q_tiles_b, q_parts_b, k_tiles_b, origin_b;
     const float* slopes;           // optional, one per head
     float cap;                     // 0: none
+    int max_keys;                  // most keys a row sees (0: not known); a hint
 };
 static inline Rules make_rules(const fa_b200_rules& r, int Nq, int Nk) {
     const RangesLayout l = ranges_layout(r.plan_batch, Nq, Nk);
@@ -133,7 +134,7 @@ static inline Rules make_rules(const fa_b200_rules& r, int Nq, int Nk) {
     u.k_tiles = (const int2*)(base + l.k_tiles); u.origin = base + l.origin;
     u.rows_b = shared ? 0 : l.nq_pad; u.q_tiles_b = shared ? 0 : l.nq_pad / 128; u.q_parts_b = shared ? 0 : l.nq_pad / 16;
     u.k_tiles_b = shared ? 0 : l.nk_pad / 128; u.origin_b = shared ? 0 : 1;
-    u.slopes = r.slopes; u.cap = r.score_cap;
+    u.slopes = r.slopes; u.cap = r.score_cap; u.max_keys = r.max_keys;
     return u;
 }
 
@@ -167,7 +168,7 @@ static inline float pair_score_scale(const fa_b200_params& p) {
 bool sm100_pair_supports(const fa_b200_params& p, bool backward, const char** why);
 // The same kernels for calls with rules (fwd_rules_sm100.cu, bwd_rules_sm100.cu): what sm100_pair_supports covers.
 int sm100_rules_fwd(const fa_b200_params& p, const Rules& rules, void* ws, size_t ws_bytes);
-size_t sm100_rules_fwd_workspace_bytes(const fa_b200_params& p);
+size_t sm100_rules_fwd_workspace_bytes(const fa_b200_params& p, int max_keys);
 int sm100_rules_bwd(const fa_b200_params& p, const BwdWorkspace& ws, const Rules& rules);
 // fp32 forward on the tensor cores (fwd_tf32_sm100.cu): TF32 products taken three times
 int sm100_tf32_fwd(const fa_b200_params& p);

@@ -1551,7 +1551,12 @@ constexpr int kMergeUnits = 4;
 // walk with starts took registers from the softmax (700 queries on 8892 keys 93 -> 100 us).
 constexpr int kLongRange = 8;
 constexpr int kDecodeRows = 16;        // rows of a K/V head that fwd_decode_kernel serves
-FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, bool ruled = false) {
+// With rules whole pairs are dealt out as CTAs get done (Dealer), so a round-robin share is what the SMs have on average, one
+// pair at least, and a pair's keys are at most `max_keys` and its own 256 (0: not known).  Ranges cost more there, because a
+// packed tile's hull is read from memory wherever a walk comes to it: 700 queries on 8892 keys, H32 Hkv8 D128 bf16, whole ->
+// ranges, us: all keys 139 -> 133, with a cap 215 -> 172; window 4096 78 -> 90, 113 -> 115; window 1024 35 -> 57, 45 -> 68.
+constexpr int kMergeUnitsRules = 16;
+FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, bool ruled = false, int max_keys = 0) {
     FwdPlan pl;
     memset(&pl, 0, sizeof(pl));
     auto pairs_of = [&](int qpt) { return (int)(((int64_t)p.Nq + 2 * qpt - 1) / (2 * qpt)); };
@@ -1580,18 +1585,24 @@ FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, bool r
     int64_t col = column_units(p, kBlockM, pl.n_pairs);
     const int items = p.causal ? (pl.n_pairs + 1) / 2 : pl.n_pairs;              // per column: a pair, or a pair and its mirror
     const int64_t n_items = (int64_t)items * p.B * p.H;
-    const int64_t whole = (n_items + sms - 1) / sms * ((col + items - 1) / items);
+    int64_t whole = (n_items + sms - 1) / sms * ((col + items - 1) / items);
+    int64_t pair_most = (p.Nk + kBlockN - 1) / kBlockN;
+    if (ruled) {
+        if (max_keys > 0 && (max_keys + 2 * kBlockM) / kBlockN + 1 < pair_most) pair_most = (max_keys + 2 * kBlockM) / kBlockN + 1;
+        whole = (n_items * pair_most + sms - 1) / sms;
+        if (whole < pair_most) whole = pair_most;
+    }
     if (group > 1 && group <= kBlockM) {
         const int qpt = kBlockM / group, pairs = pairs_of(qpt);
         const int64_t packed = column_units(p, qpt, pairs);
         if (packed * p.Hkv * 20 <= col * p.H * 19) { pl.pack = group; pl.q_per_tile = qpt; pl.heads = p.Hkv; pl.n_pairs = pairs; col = packed; }
     }
-    const int64_t total = (int64_t)p.B * pl.heads * col;
+    const int64_t total = (int64_t)p.B * pl.heads * (ruled ? pl.n_pairs * pair_most : col);
     pl.ctas = (int)(total < sms ? total : sms);
     int64_t ranges = (total + pl.ctas - 1) / pl.ctas;
     const bool one_tile = p.Nq <= pl.q_per_tile, counts = p.kv_lengths || ruled;
     if (counts && one_tile) ranges = (3 * ranges + 3) / 4;
-    if (total < (1 << 28) && whole * 9 > (ranges + kMergeUnits) * 10) {
+    if (total < (1 << 28) && whole * 9 > (ranges + (ruled ? kMergeUnitsRules : kMergeUnits)) * 10) {
         pl.sched = one_tile ? 2 : 1;
         pl.start_cost = counts && one_tile && ranges >= kLongRange ? 3 : 0;
         const int tiles = (int)(((int64_t)p.Nq + pl.q_per_tile - 1) / pl.q_per_tile);
@@ -1607,8 +1618,9 @@ int launch(const fa_b200_params& p, void* ws, size_t ws_bytes, const Rules* rule
     const int d = p.D;
     const int sms = sm_count(p.device);
     if (sms <= 0) { set_error("cannot read the SM count of device %d", p.device); return FA_ECUDA; }
-    FwdPlan plan = plan_schedule(p, D, sms, ws != nullptr, RULES != 0);
-    if (ws_bytes < plan.bytes || ((uintptr_t)ws & 255u) != 0) plan = plan_schedule(p, D, sms, false, RULES != 0);
+    const int max_keys = rules ? rules->max_keys : 0;
+    FwdPlan plan = plan_schedule(p, D, sms, ws != nullptr, RULES != 0, max_keys);
+    if (ws_bytes < plan.bytes || ((uintptr_t)ws & 255u) != 0) plan = plan_schedule(p, D, sms, false, RULES != 0, max_keys);
     const CUtensorMapDataType dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap mq, mk, mv;
     int r;
@@ -1741,8 +1753,8 @@ int fwd_by_type(const fa_b200_params& p, const Rules& rules, void* ws, size_t ws
 int sm100_rules_fwd(const fa_b200_params& p, const Rules& rules, void* ws, size_t ws_bytes) {
     return rules.cap > 0.f ? fwd_by_type<2>(p, rules, ws, ws_bytes) : fwd_by_type<1>(p, rules, ws, ws_bytes);
 }
-size_t sm100_rules_fwd_workspace_bytes(const fa_b200_params& p) {
-    return plan_schedule(p, p.D > 64 ? 128 : 64, sm_count(p.device), true, true).bytes;
+size_t sm100_rules_fwd_workspace_bytes(const fa_b200_params& p, int max_keys) {
+    return plan_schedule(p, p.D > 64 ? 128 : 64, sm_count(p.device), true, true, max_keys).bytes;
 }
 #elif !defined(FA_PAIR_INSTANCES)
 bool tensor_ok(const fa_b200_tensor& t, int64_t B, int64_t N, int64_t H) {

@@ -400,12 +400,12 @@ int choose_rules_variant(const fa_b200_params& p, bool backward, int* variant) {
 
 extern "C" {
 
-size_t fa_b200_fwd_rules_workspace_bytes(const fa_b200_params* p) {
-    if (!p || p->struct_bytes != sizeof(fa_b200_params)) return 0;
+size_t fa_b200_fwd_rules_workspace_bytes(const fa_b200_params* p, const fa_b200_rules* r) {
+    if (!p || p->struct_bytes != sizeof(fa_b200_params) || !r || r->struct_bytes != sizeof(fa_b200_rules)) return 0;
     if (p->B <= 0 || p->Nq <= 0 || p->Nk <= 0 || p->H <= 0 || p->Hkv <= 0 || p->D <= 0 || p->H % p->Hkv != 0) return 0;
     int variant;
     if (choose_rules_variant(*p, false, &variant) != FA_OK || variant == FA_B200_VARIANT_SIMT) return 0;
-    return sm100_rules_fwd_workspace_bytes(*p);
+    return sm100_rules_fwd_workspace_bytes(*p, r->max_keys);
 }
 
 int fa_b200_fwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r, void* workspace, size_t workspace_bytes) {

@@ -1,11 +1,12 @@
 // Rotary positions: pairs of columns of every head turned by position * frequency (the definition is in fa_b200.h).
 //
-// A block takes kTokens tokens.  Its threads first put the tokens' cosines and sines into shared memory, a pair's once for
-// all heads of q and k: the angle and its reduction by whole turns in 64 bits (at position 10^6 a float angle would be
-// off by 0.06), sine and cosine of what is left in 32.  Then a thread's unit is one 16-byte piece of a head (two of them,
-// u and w, where the halves of the head are paired), read, turned and written.  Everything is read once and written once:
-// memory bounds it, and for a token or two the launch.
+// A block takes a few tokens.  Its threads ask for their pieces of the heads first, and while those are on their way put the
+// tokens' cosines and sines into shared memory, a pair's once for all heads of q and k: the angle and its reduction by whole
+// turns in 64 bits (at position 10^6 a float angle would be off by 0.06), sine and cosine of the part of a turn that is left
+// in 32.  A unit is one 16-byte piece of a head, or two of them, u and w, where the halves of the head are paired.  Everything
+// is read once and written once: memory bounds it, and for a token or two the launch.
 #include "fa_common.cuh"
+#include "sm100_ptx.cuh"
 #include <type_traits>
 
 namespace fa {
@@ -24,8 +25,12 @@ struct RotaryArgs {
 
 constexpr int kThreads = 256;
 constexpr int kMaxHalf = 64;       // head sizes up to 128
+constexpr int kAtOnce = 4;         // units a thread has on their way
+constexpr int kPasses = 2;
+constexpr int kMaxTurns = 1024;    // tokens times pairs of a block
+constexpr int kMaxTokens = 64;     // ... and tokens
 
-template <typename T, int VEC> struct Piece { T v[VEC]; };
+template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Piece { T v[VEC]; };
 template <typename T, int VEC>
 __device__ __forceinline__ Piece<T, VEC> load_piece(const T* p) {
     Piece<T, VEC> r;
@@ -39,92 +44,149 @@ __device__ __forceinline__ void store_piece(T* p, const Piece<T, VEC>& r) {
     else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
 }
 
+// Elements at, at + 1 of a piece as floats, and back.
+template <typename T, int VEC>
+__device__ __forceinline__ void get2(const Piece<T, VEC>& p, int at, float& x, float& y) {
+    if constexpr (sizeof(T) == 4) { x = to_f32<T>(p.v[at]); y = to_f32<T>(p.v[at + 1]); }
+    else ptx::unpack2<std::is_same<T, __nv_bfloat16>::value>(reinterpret_cast<const uint32_t*>(&p)[at / 2], x, y);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void put2(Piece<T, VEC>& p, int at, float x, float y) {
+    if constexpr (sizeof(T) == 4) { p.v[at] = from_f32<T>(x); p.v[at + 1] = from_f32<T>(y); }
+    else reinterpret_cast<uint32_t*>(&p)[at / 2] = ptx::pack2<std::is_same<T, __nv_bfloat16>::value>(x, y);
+}
+
 // VEC elements a piece: 16 bytes, or one where addresses, head size or the number of pairs do not allow pieces.
-template <typename T, int VEC, bool INTERLEAVED, int TOKENS>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
-    __shared__ float2 turn[TOKENS][kMaxHalf];            // factor * cos, factor * sin
-    const int64_t token0 = (int64_t)blockIdx.x * TOKENS;
-    const int n_tokens = (int)(a.tokens - token0 < TOKENS ? a.tokens - token0 : TOKENS);
-    for (int e = threadIdx.x; e < n_tokens * a.half; e += kThreads) {
-        const int t = e / a.half, i = e - t * a.half;
-        const int64_t token = token0 + t, b = token / a.N, n = token - b * a.N;
-        int64_t pos = a.position0 + n;
-        if (a.positions) {
-            const int64_t at = b * a.pos_sb + n * a.pos_sn;
-            pos = a.pos64 ? ((const int64_t*)a.positions)[at] : ((const int32_t*)a.positions)[at];
-        }
-        const double angle = (double)pos * a.inv_freq[i];
-        // less whole turns: 2 pi as a double and the rest of it
-        const double turns = rint(angle * 0.15915494309189533577);
-        const double rest = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.2831853071795864769, angle));
-        float s, c;
-        sincosf((float)rest, &s, &c);
-        turn[t][i] = make_float2(a.factor * c, a.factor * a.sign * s);
-    }
-    __syncthreads();
+template <typename T, int VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a, int tokens_per_block) {
+    // factor * cos and factor * sin of a token's pairs.  A unit's pairs v, v + 1 side by side, the units of one v next to each
+    // other: a warp's 8-byte loads go to different banks (in the pairs' order every load took four turns).
+    __shared__ __align__(8) float cos_of[kMaxTurns], sin_of[kMaxTurns];
+    __shared__ int64_t base_of[kMaxTokens][4];           // a token's place in x[0], x[1], y[0], y[1]
+    __shared__ int2 place[kMaxTokens];                   // its batch entry and row
+    const int64_t token0 = (int64_t)blockIdx.x * tokens_per_block;
+    const int n_tokens = (int)(a.tokens - token0 < tokens_per_block ? a.tokens - token0 : tokens_per_block);
     // units of a head: the pairs' pieces, then the copied ones
-    const int n_turned = INTERLEAVED && VEC > 1 ? 2 * a.half / VEC : a.half / (VEC > 1 ? VEC : 1);
-    const int in_place = a.x[0].ptr == a.y[0].ptr && (a.x[1].ptr == a.y[1].ptr);
+    constexpr bool ONE = INTERLEAVED && VEC > 1;         // a unit is one piece
+    const int n_turned = ONE ? 2 * a.half / VEC : a.half / VEC;
+    const bool in_place = a.x[0].ptr == a.y[0].ptr && a.x[1].ptr == a.y[1].ptr;
     const int n_units = n_turned + (in_place ? 0 : (a.D - 2 * a.half) / VEC);
     const int heads = a.heads[0] + a.heads[1];
-    const int total = n_tokens * heads * n_units;
-#pragma unroll 4
-    for (int e = threadIdx.x; e < total; e += kThreads) {
-        const int row = e / n_units, unit = e - row * n_units;
-        const int t = row / heads, hh = row - t * heads;
-        const int which = hh >= a.heads[0];
-        const int h = which ? hh - a.heads[0] : hh;
-        const int64_t token = token0 + t, b = token / a.N, n = token - b * a.N;
-        const fa_b200_tensor& xt = a.x[which];
-        const fa_b200_tensor& yt = a.y[which];
-        const T* x = (const T*)xt.ptr + b * xt.stride_b + n * xt.stride_n + h * xt.stride_h;
-        T* y = (T*)yt.ptr + b * yt.stride_b + n * yt.stride_n + h * yt.stride_h;
-        if (unit >= n_turned) {
-            const int c = 2 * a.half + (unit - n_turned) * VEC;
-            store_piece<T, VEC>(y + c, load_piece<T, VEC>(x + c));
-        } else if (INTERLEAVED && VEC > 1) {
-            const int c = unit * VEC;
-            Piece<T, VEC> p = load_piece<T, VEC>(x + c);
+    const int n_units_or_1 = n_units > 0 ? n_units : 1;
+
+    // A thread keeps its unit and goes through the rows (token, head), `step` rows at a time: no division behind the first ones
+    // (with them, 64-bit ones among them, the kernel took 150 us where it takes 60).
+    const int step = kThreads / n_units_or_1, unit = (int)threadIdx.x % n_units_or_1;
+    const int rows = n_tokens * heads, first = (int)threadIdx.x / n_units_or_1;
+    const bool idle = n_units == 0 || first >= step;     // (threads beyond whole rows)
+    if (threadIdx.x < (unsigned)n_tokens) {
+        const uint32_t token = (uint32_t)token0 + threadIdx.x, b = token / (uint32_t)a.N, n = token - b * (uint32_t)a.N;
 #pragma unroll
-            for (int v = 0; v < VEC; v += 2) {
-                const float2 cs = turn[t][c / 2 + v / 2];
-                const float u = to_f32<T>(p.v[v]), w = to_f32<T>(p.v[v + 1]);
-                p.v[v] = from_f32<T>(u * cs.x - w * cs.y);
-                p.v[v + 1] = from_f32<T>(w * cs.x + u * cs.y);
-            }
-            store_piece<T, VEC>(y + c, p);
-        } else {
-            const int i = unit * VEC;
-            const int c0 = INTERLEAVED ? 2 * i : i, c1 = INTERLEAVED ? 2 * i + 1 : i + a.half;
-            Piece<T, VEC> pu = load_piece<T, VEC>(x + c0), pw = load_piece<T, VEC>(x + c1);
+        for (int w = 0; w < 2; ++w) {
+            base_of[threadIdx.x][w] = (int64_t)b * a.x[w].stride_b + (int64_t)n * a.x[w].stride_n;
+            base_of[threadIdx.x][2 + w] = (int64_t)b * a.y[w].stride_b + (int64_t)n * a.y[w].stride_n;
+        }
+        place[threadIdx.x] = make_int2((int)b, (int)n);
+    }
+    __syncthreads();
+    int t = 0, hh = first;
+    while (hh >= heads) { hh -= heads; ++t; }
+    // columns of a unit's first and second piece (the second: halves, or single columns of interleaved pairs)
+    auto col0 = [&](int unit) { return unit >= n_turned ? 2 * a.half + (unit - n_turned) * VEC : (INTERLEAVED && VEC == 1 ? 2 * unit : unit * VEC); };
+    auto col1 = [&](int unit) { return INTERLEAVED ? 2 * unit + 1 : unit * VEC + a.half; };
+
+    const bool turned = unit < n_turned;
+    const int c0 = col0(unit), c1 = col1(unit);
+    constexpr int P = VEC == 1 ? 1 : (ONE ? VEC / 2 : VEC);          // pairs of a unit
+    auto slot = [&](int i) { return P == 1 ? i : ((i % P / 2) * n_turned + i / P) * 2 + (i & 1); };
+    for (int row0 = first, pass = 0; pass == 0 || row0 - first < rows; row0 += step * kAtOnce, ++pass) {
+        Piece<T, VEC> pu[kAtOnce], pw[kAtOnce];
+        T* y[kAtOnce];
+        int tt[kAtOnce];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float2 cs = turn[t][i + v];
-                const float u = to_f32<T>(pu.v[v]), w = to_f32<T>(pw.v[v]);
-                pu.v[v] = from_f32<T>(u * cs.x - w * cs.y);
-                pw.v[v] = from_f32<T>(w * cs.x + u * cs.y);
+        for (int k = 0; k < kAtOnce; ++k) {
+            if (idle || row0 + k * step >= rows) continue;
+            const int which = hh >= a.heads[0], h = which ? hh - a.heads[0] : hh;
+            const T* x = (const T*)a.x[which].ptr + base_of[t][which] + h * a.x[which].stride_h;
+            y[k] = (T*)a.y[which].ptr + base_of[t][2 + which] + h * a.y[which].stride_h;
+            tt[k] = t;
+            pu[k] = load_piece<T, VEC>(x + c0);
+            if (!ONE && turned) pw[k] = load_piece<T, VEC>(x + c1);
+            hh += step;
+            while (hh >= heads) { hh -= heads; ++t; }
+        }
+        if (pass == 0) {
+            for (int e = threadIdx.x; e < n_tokens * a.half; e += kThreads) {
+                const int at = e / a.half, i = e - at * a.half;
+                const int2 bn = place[at];
+                int64_t pos = a.position0 + bn.y;
+                if (a.positions) {
+                    const int64_t from = bn.x * a.pos_sb + bn.y * a.pos_sn;
+                    pos = a.pos64 ? ((const int64_t*)a.positions)[from] : ((const int32_t*)a.positions)[from];
+                }
+                const double turns = (double)pos * a.inv_freq[i] * 0.15915494309189533577;       // 1 / 2 pi
+                float s, c;
+                sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+                cos_of[at * a.half + slot(i)] = a.factor * c;
+                sin_of[at * a.half + slot(i)] = a.factor * a.sign * s;
             }
-            store_piece<T, VEC>(y + c0, pu);
-            store_piece<T, VEC>(y + c1, pw);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            if (idle || row0 + k * step >= rows) continue;
+            if (turned) {
+                const float *cs = cos_of + tt[k] * a.half, *sn = sin_of + tt[k] * a.half;
+                if constexpr (VEC == 1) {
+                    const float x = to_f32<T>(pu[k].v[0]), w = to_f32<T>(pw[k].v[0]), c = cs[unit], n = sn[unit];
+                    pu[k].v[0] = from_f32<T>(x * c - w * n);
+                    pw[k].v[0] = from_f32<T>(w * c + x * n);
+                } else {
+#pragma unroll
+                    for (int v = 0; v < P; v += 2) {
+                        // two pairs at once: u and w of both
+                        const uint64_t c2 = *reinterpret_cast<const uint64_t*>(cs + ((v / 2) * n_turned + unit) * 2);
+                        const uint64_t s2 = *reinterpret_cast<const uint64_t*>(sn + ((v / 2) * n_turned + unit) * 2);
+                        float u0, u1, w0, w1;
+                        if constexpr (ONE) { get2(pu[k], 2 * v, u0, w0); get2(pu[k], 2 * v + 2, u1, w1); }
+                        else { get2(pu[k], v, u0, u1); get2(pw[k], v, w0, w1); }
+                        const uint64_t u = ptx::f2_pack(u0, u1), w = ptx::f2_pack(w0, w1);
+                        ptx::f2_unpack(ptx::f2_fma(w, s2 ^ 0x8000000080000000ull, ptx::f2_mul(u, c2)), u0, u1);
+                        ptx::f2_unpack(ptx::f2_fma(u, s2, ptx::f2_mul(w, c2)), w0, w1);
+                        if constexpr (ONE) { put2(pu[k], 2 * v, u0, w0); put2(pu[k], 2 * v + 2, u1, w1); }
+                        else { put2(pu[k], v, u0, u1); put2(pw[k], v, w0, w1); }
+                    }
+                }
+                if (!ONE) store_piece<T, VEC>(y[k] + c1, pw[k]);
+            }
+            store_piece<T, VEC>(y[k] + c0, pu[k]);
         }
     }
 }
 
 template <typename T, int VEC, bool INTERLEAVED>
-int launch(const RotaryArgs& a, cudaStream_t st) {
-    constexpr int kTokens = 4;
-    const int64_t blocks = (a.tokens + kTokens - 1) / kTokens;
-    if (blocks > 0x7fffffff) { set_error("rotary: too many tokens"); return FA_EUNSUPPORTED; }
-    rotary_kernel<T, VEC, INTERLEAVED, kTokens><<<(unsigned)blocks, kThreads, 0, st>>>(a);
+int launch(const RotaryArgs& a, int device, cudaStream_t st) {
+    // tokens for a few passes of what a block's threads have on their way, fewer where that would leave SMs idle
+    const int64_t heads = a.heads[0] + a.heads[1];
+    const int64_t units = heads * ((INTERLEAVED && VEC > 1 ? 2 * a.half / VEC : a.half / VEC) + (a.D - 2 * a.half) / VEC);
+    int64_t tokens = units > 0 ? (int64_t)kThreads * kAtOnce * kPasses / units : 1;
+    const int64_t spread = a.tokens / (4 * (int64_t)(sm_count(device) > 0 ? sm_count(device) : 1));
+    if (tokens > spread) tokens = spread;
+    if (a.half > 0 && tokens > kMaxTurns / a.half) tokens = kMaxTurns / a.half;
+    if (tokens > kMaxTokens) tokens = kMaxTokens;
+    if (tokens < 1) tokens = 1;
+    const int64_t blocks = (a.tokens + tokens - 1) / tokens;
+    if (a.tokens > 0x7fffffff || heads * a.D * tokens > 0x3fffffff) { set_error("rotary: too many tokens or heads"); return FA_EUNSUPPORTED; }
+    rotary_kernel<T, VEC, INTERLEAVED><<<(unsigned)blocks, kThreads, 0, st>>>(a, (int)tokens);
     FA_CUDA_CHECK(cudaGetLastError());
     return FA_OK;
 }
 
 template <typename T>
-int pick(const RotaryArgs& a, bool pieces, cudaStream_t st) {
+int pick(const RotaryArgs& a, bool pieces, int device, cudaStream_t st) {
     constexpr int V = 16 / (int)sizeof(T);
-    if (pieces) return a.interleaved ? launch<T, V, true>(a, st) : launch<T, V, false>(a, st);
-    return a.interleaved ? launch<T, 1, true>(a, st) : launch<T, 1, false>(a, st);
+    if (pieces) return a.interleaved ? launch<T, V, true>(a, device, st) : launch<T, V, false>(a, device, st);
+    return a.interleaved ? launch<T, 1, true>(a, device, st) : launch<T, 1, false>(a, device, st);
 }
 
 }  // namespace
@@ -166,6 +228,6 @@ extern "C" int fa_b200_rotary(const fa_b200_rotary_params* p) {
     GuardDevice g(p->device);
     if (!g.ok) { set_error("cudaSetDevice(%d) failed", p->device); return FA_ECUDA; }
     cudaStream_t st = (cudaStream_t)p->stream;
-    if (p->dtype == FA_B200_F32) return pick<float>(a, pieces, st);
-    return p->dtype == FA_B200_BF16 ? pick<__nv_bfloat16>(a, pieces, st) : pick<__half>(a, pieces, st);
+    if (p->dtype == FA_B200_F32) return pick<float>(a, pieces, p->device, st);
+    return p->dtype == FA_B200_BF16 ? pick<__nv_bfloat16>(a, pieces, p->device, st) : pick<__half>(a, pieces, p->device, st);
 }

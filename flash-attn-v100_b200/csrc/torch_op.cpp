@@ -162,13 +162,13 @@ struct Attention : torch::autograd::Function<Attention> {
 // their Python forms take what is refused here ----
 struct Ruled {
     double scale, cap;
-    int64_t plan_batch;
+    int64_t plan_batch, max_keys;
     at::Tensor slopes, plan;    // slopes may be undefined
 };
 
 fa_b200_rules rules_of(const Ruled& r) {
     return {sizeof(fa_b200_rules), r.plan.const_data_ptr(), (int32_t)r.plan_batch, (float)r.cap,
-            r.slopes.defined() ? r.slopes.const_data_ptr<float>() : nullptr};
+            r.slopes.defined() ? r.slopes.const_data_ptr<float>() : nullptr, (int32_t)r.max_keys, 0};
 }
 
 void ruled_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const Ruled& r, bool split, bool residual, at::Tensor& o, at::Tensor& lse,
@@ -178,7 +178,7 @@ void ruled_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
     fa_b200_params p = params_of(q, k, v, o, lse, Call{r.scale, false, false, 0, {}});
     if (residual) { o_lo = at::empty(q.sizes(), q.options()); p.o_lo = operand(o_lo); }
     const fa_b200_rules u = rules_of(r);
-    const size_t n = split ? fa_b200_fwd_rules_workspace_bytes(&p) : 0;
+    const size_t n = split ? fa_b200_fwd_rules_workspace_bytes(&p, &u) : 0;
     at::Tensor ws;
     if (n) ws = bytes_like(q, n);
     raise_for_status(fa_b200_fwd_with_rules(&p, &u, n ? ws.mutable_data_ptr() : nullptr, n), "fa_b200_fwd_with_rules");
@@ -215,7 +215,7 @@ struct RuledAttention : torch::autograd::Function<RuledAttention> {
         variable_list out(4);
         if (!grads[0].defined()) return out;
         const variable_list kept = ctx->get_saved_variables();
-        const Ruled r{ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble(), ctx->saved_data["batch"].toInt(), kept[7], kept[5]};
+        const Ruled r{ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble(), ctx->saved_data["batch"].toInt(), 0, kept[7], kept[5]};
         at::Tensor d[3];
         at::AutoDispatchBelowADInplaceOrView below;
         ruled_backward(grads[0], kept[0], kept[1], kept[2], kept[3], kept[4], kept[6], r, d[0], d[1], d[2]);
@@ -383,14 +383,14 @@ template <typename F> void unlocked(F f) {
 
 // (o, lse) of flash_attention_v100_with_rules, or None.  seq_q, seq_k: the plan's.
 py::object attention_rules(py::handle q_, py::handle k_, py::handle v_, py::handle scale_, py::handle cap_, py::handle slopes_, py::handle plan_, int64_t batch,
-                           int64_t seq_q, int64_t seq_k) {
+                           int64_t seq_q, int64_t seq_k, int64_t max_keys) {
     const at::Tensor *qp, *kp, *vp, *sp, *pp;
     if (watched() || !plain(q_.ptr(), qp) || !plain(k_.ptr(), kp) || !plain(v_.ptr(), vp) || !plain(plan_.ptr(), pp)) return py::none();
     const at::Tensor q = *qp, k = *kp, v = *vp;
     if (!served(q, k, v)) return py::none();
     const int device = q.device().index();
     if (device >= kMaxDevices || !g_status_word[device].load(std::memory_order_acquire)) return py::none();
-    Ruled r{std::pow((double)q.size(3), -0.5), 0.0, batch, {}, *pp};
+    Ruled r{std::pow((double)q.size(3), -0.5), 0.0, batch, max_keys, {}, *pp};
     if (q.size(1) != seq_q || k.size(1) != seq_k || (batch != 1 && batch != q.size(0)) || r.plan.device() != q.device()) return py::none();
     if (!scale_.is_none()) {
         if (!PyFloat_CheckExact(scale_.ptr())) return py::none();
@@ -469,7 +469,7 @@ py::object rotary(py::handle q_, py::handle k_, py::handle positions_, py::handl
     return py::make_tuple(wrap(std::move(y[0])), wrap(std::move(y[1])));
 }
 
-// (plan, positions) of build_key_ranges, or None.
+// (plan, positions, first, end) of build_key_ranges, or None.
 py::object key_ranges(int64_t seq_q, int64_t seq_k, int64_t batch, bool causal, int64_t window, py::handle offsets_, py::handle prefixes_, py::handle lengths_,
                       py::handle starts_, int64_t start, int device) {
     if (watched() || seq_q < 0 || seq_k < 0 || batch < 0 || seq_q > INT32_MAX || seq_k > INT32_MAX || batch > INT32_MAX || window < 0 || window > INT32_MAX ||
@@ -519,7 +519,14 @@ py::object key_ranges(int64_t seq_q, int64_t seq_k, int64_t batch, bool causal, 
         p.stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
         raise_for_status(fa_b200_key_ranges(&p), "fa_b200_key_ranges");
     });
-    return py::make_tuple(wrap(std::move(plan)), wrap(std::move(positions)));
+    const int64_t pitch = 2 * ((seq_q + 127) / 128 * 128);
+    at::Tensor first, end;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        first = plan.as_strided({batch, seq_q}, {pitch, 2}, 0);
+        end = plan.as_strided({batch, seq_q}, {pitch, 2}, seq_q > 0 && batch > 0 ? 1 : 0);
+    }
+    return py::make_tuple(wrap(std::move(plan)), wrap(std::move(positions)), wrap(std::move(first)), wrap(std::move(end)));
 }
 
 }  // namespace

@@ -501,7 +501,7 @@ def flash_attention_v100_with_rules(
     if key_ranges is None:
         key_ranges = build_key_ranges(q.shape[1], k.shape[1], batch=1 if key_lengths is None else q.shape[0], causal=causal,
                                       key_lengths=key_lengths, query_offsets=shift, device=q.device)
-    o, lse = RuledAttentionFunction.apply(q, k, v, scale, cap, slopes, key_ranges.plan, key_ranges.batch)
+    o, lse = RuledAttentionFunction.apply(q, k, v, scale, cap, slopes, key_ranges.plan, key_ranges.batch, key_ranges.max_keys)
     if profile:
         end.record(torch.cuda.current_stream(q.device))
         end.synchronize()

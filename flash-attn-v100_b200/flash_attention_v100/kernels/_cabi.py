@@ -94,7 +94,7 @@ class RangesParams(ctypes.Structure):
 
 class RuleParams(ctypes.Structure):
     _fields_ = [("struct_bytes", ctypes.c_size_t), ("plan", ctypes.c_void_p), ("plan_batch", ctypes.c_int32),
-                ("score_cap", ctypes.c_float), ("slopes", ctypes.c_void_p)]
+                ("score_cap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("max_keys", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 class RotaryParams(ctypes.Structure):
@@ -181,7 +181,7 @@ def load():
         lib.fa_b200_key_ranges.restype = ctypes.c_int
         lib.fa_b200_fwd_with_rules.argtypes = [pp, rp, ctypes.c_void_p, ctypes.c_size_t]
         lib.fa_b200_fwd_with_rules.restype = ctypes.c_int
-        lib.fa_b200_fwd_rules_workspace_bytes.argtypes = [pp]
+        lib.fa_b200_fwd_rules_workspace_bytes.argtypes = [pp, rp]
         lib.fa_b200_fwd_rules_workspace_bytes.restype = ctypes.c_size_t
         lib.fa_b200_bwd_with_rules.argtypes = [pp, rp]
         lib.fa_b200_bwd_with_rules.restype = ctypes.c_int

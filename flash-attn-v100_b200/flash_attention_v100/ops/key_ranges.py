@@ -28,23 +28,29 @@ class KeyRanges:
     first, end: (batch, seq_q) int32, row i of entry b sees keys [first, end) (0, 0: none)
     positions:  (batch, seq_q) int32, the row's place within its document, for rotary_embedding
     """
-    __slots__ = ("plan", "positions", "batch", "seq_q", "seq_k")
+    __slots__ = ("plan", "positions", "batch", "seq_q", "seq_k", "max_keys", "_first", "_end")
 
-    def __init__(self, plan: torch.Tensor, positions: torch.Tensor, batch: int, seq_q: int, seq_k: int):
+    def __init__(self, plan: torch.Tensor, positions: torch.Tensor, batch: int, seq_q: int, seq_k: int, max_keys: int = 0,
+                 first: Optional[torch.Tensor] = None, end: Optional[torch.Tensor] = None):
         self.plan, self.positions = plan, positions
         self.batch, self.seq_q, self.seq_k = batch, seq_q, seq_k
+        self.max_keys = max_keys                # most keys a row sees (0: not known), for how the work is divided
+        self._first, self._end = first, end
 
     @property
     def device(self) -> torch.device:
         return self.plan.device
 
+    def _column(self, at: int) -> torch.Tensor:
+        return self.plan.as_strided((self.batch, self.seq_q), (2 * _ceil128(self.seq_q), 2), at if self.batch and self.seq_q else 0)
+
     @property
     def first(self) -> torch.Tensor:
-        return self.plan.as_strided((self.batch, self.seq_q), (2 * _ceil128(self.seq_q), 2), 0)
+        return self._column(0) if self._first is None else self._first
 
     @property
     def end(self) -> torch.Tensor:
-        return self.plan.as_strided((self.batch, self.seq_q), (2 * _ceil128(self.seq_q), 2), 1)
+        return self._column(1) if self._end is None else self._end
 
 
 def _lengths(name: str, t: Optional[torch.Tensor], shapes, device: torch.device) -> Optional[torch.Tensor]:
@@ -63,6 +69,10 @@ def _lengths(name: str, t: Optional[torch.Tensor], shapes, device: torch.device)
     if t.dtype != torch.int32:
         t = t.to(torch.int32)
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _most(causal: bool, window: Optional[int]) -> int:
+    return 0 if window is None else min(window if causal else 2 * window - 1, _INT32_MAX)
 
 
 def _device_index(device, *tensors) -> Optional[int]:
@@ -109,7 +119,7 @@ def build_key_ranges(seq_q: int, seq_k: int, *, batch: int = 1, causal: bool = F
         if index is not None:
             result = _cabi.load_op().key_ranges(seq_q, seq_k, batch, bool(causal), window or 0, document_offsets, prefix_lengths, key_lengths, starts, start, index)
             if result is not None:
-                return KeyRanges(result[0], result[1], batch, seq_q, seq_k)
+                return KeyRanges(result[0], result[1], batch, seq_q, seq_k, _most(causal, window), result[2], result[3])
     if seq_q < 0 or seq_k < 0 or batch < 0:
         raise ValueError(f"sizes must not be negative (seq_q {seq_q}, seq_k {seq_k}, batch {batch})")
     if window is not None and not 1 <= window <= _INT32_MAX:
@@ -141,11 +151,12 @@ def build_key_ranges(seq_q: int, seq_k: int, *, batch: int = 1, causal: bool = F
     nbytes = lib.fa_b200_key_ranges_bytes(batch, seq_q, seq_k)
     if out is None:
         out = KeyRanges(torch.empty(nbytes // 4, dtype=torch.int32, device=device),
-                        torch.empty((batch, seq_q), dtype=torch.int32, device=device), batch, seq_q, seq_k)
+                        torch.empty((batch, seq_q), dtype=torch.int32, device=device), batch, seq_q, seq_k, _most(causal, window))
     else:
         if (out.batch, out.seq_q, out.seq_k) != (batch, seq_q, seq_k) or out.device != device:
             raise ValueError(f"out is for batch {out.batch}, {out.seq_q} rows and {out.seq_k} keys on {out.device}")
         torch.autograd.graph.increment_version([out.plan, out.positions])
+        out.max_keys = _most(causal, window)
     p = _cabi.RangesParams(
         _RANGES_BYTES, out.plan.data_ptr(), nbytes, out.positions.data_ptr(), given.data_ptr() if given is not None else None,
         offsets.data_ptr() if offsets is not None else None, prefixes.data_ptr() if prefixes is not None else None,

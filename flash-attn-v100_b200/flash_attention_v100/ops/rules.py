@@ -19,8 +19,8 @@ from .key_ranges import KeyRanges
 _RULES_BYTES = ctypes.sizeof(_cabi.RuleParams)
 
 
-def _rules(cap: float, slopes: Optional[torch.Tensor], plan: torch.Tensor, plan_batch: int) -> _cabi.RuleParams:
-    return _cabi.RuleParams(_RULES_BYTES, plan.data_ptr(), plan_batch, cap, slopes.data_ptr() if slopes is not None else None)
+def _rules(cap: float, slopes: Optional[torch.Tensor], plan: torch.Tensor, plan_batch: int, max_keys: int = 0) -> _cabi.RuleParams:
+    return _cabi.RuleParams(_RULES_BYTES, plan.data_ptr(), plan_batch, cap, slopes.data_ptr() if slopes is not None else None, max_keys)
 
 
 def check_rules(q: torch.Tensor, k: torch.Tensor, score_cap: Optional[float], slopes: Optional[torch.Tensor],
@@ -57,10 +57,10 @@ def native_call_rules(q, k, v, scale, score_cap, slopes, ranges: KeyRanges):
     """(o, lse) by the native operator, or None where it does not serve the call (as attention.native_call)."""
     if torch.compiler.is_compiling() or getattr(_variant_override, "value", _cabi.VARIANT_AUTO) != _cabi.VARIANT_AUTO:
         return None
-    return _cabi.load_op().attention_rules(q, k, v, scale, score_cap, slopes, ranges.plan, ranges.batch, ranges.seq_q, ranges.seq_k)
+    return _cabi.load_op().attention_rules(q, k, v, scale, score_cap, slopes, ranges.plan, ranges.batch, ranges.seq_q, ranges.seq_k, ranges.max_keys)
 
 
-def launch_forward_rules(q, k, v, scale, cap, slopes, plan, plan_batch, o_residual=None, split_keys=False):
+def launch_forward_rules(q, k, v, scale, cap, slopes, plan, plan_batch, o_residual=None, split_keys=False, max_keys=0):
     """(o, lse) <- fa_b200_fwd_with_rules; arguments as launch_forward's."""
     B, Nq, H, _ = q.shape
     o = q.new_empty(q.shape)
@@ -73,9 +73,9 @@ def launch_forward_rules(q, k, v, scale, cap, slopes, plan, plan_batch, o_residu
     if o_residual is not None:
         p.o_lo = _tensor4(o_residual)
     lib = _cabi.load()
-    nbytes = int(lib.fa_b200_fwd_rules_workspace_bytes(ctypes.byref(p))) if split_keys else 0
+    r = _rules(cap, slopes, plan, plan_batch, max_keys)
+    nbytes = int(lib.fa_b200_fwd_rules_workspace_bytes(ctypes.byref(p), ctypes.byref(r))) if split_keys else 0
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    r = _rules(cap, slopes, plan, plan_batch)
     rc = lib.fa_b200_fwd_with_rules(ctypes.byref(p), ctypes.byref(r), ws.data_ptr() if nbytes else None, nbytes)
     _cabi.raise_for_status(rc, "fa_b200_fwd_with_rules")
     return o, lse
@@ -103,10 +103,10 @@ class RuledAttentionFunction(torch.autograd.Function):
     """(o, lse) of q, k, v under rules; the lse is not differentiable."""
 
     @staticmethod
-    def forward(ctx, q, k, v, scale, cap, slopes, plan, plan_batch):
+    def forward(ctx, q, k, v, scale, cap, slopes, plan, plan_batch, max_keys):
         needs_grad = any(ctx.needs_input_grad[:3])
         o_lo = torch.empty(q.shape, dtype=q.dtype, device=q.device) if needs_grad and saves_output_residual(q.dtype) else None
-        o, lse = launch_forward_rules(q, k, v, scale, cap, slopes, plan, plan_batch, o_residual=o_lo, split_keys=not needs_grad)
+        o, lse = launch_forward_rules(q, k, v, scale, cap, slopes, plan, plan_batch, o_residual=o_lo, split_keys=not needs_grad, max_keys=max_keys)
         ctx.save_for_backward(q, k, v, o, lse, slopes, plan, o_lo)
         ctx.how = (scale, cap, plan_batch)
         ctx.mark_non_differentiable(lse)
@@ -119,9 +119,9 @@ class RuledAttentionFunction(torch.autograd.Function):
         q, k, v, o, lse, slopes, plan, o_lo = ctx.saved_tensors
         scale, cap, plan_batch = ctx.how
         if grad_o is None:
-            return (None,) * 8
+            return (None,) * 9
         grads = launch_backward_rules(grad_o, q, k, v, o, lse, scale, cap, slopes, plan, plan_batch, o_residual=o_lo)
-        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 5
+        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 6
 
 
 __all__ = ["RuledAttentionFunction", "check_rules", "launch_forward_rules", "launch_backward_rules"]

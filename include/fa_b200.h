@@ -372,11 +372,13 @@ typedef struct fa_b200_rules {
     int32_t        plan_batch;         /* batch entries it was built for: B, or 1 for all */
     float          score_cap;          /* 0: none */
     const float*   slopes;             /* optional, H */
+    int32_t        max_keys;           /* a hint for how the work is divided: most keys a row sees, e.g. the window (0: not known) */
+    int32_t        reserved;
 } fa_b200_rules;
 
 /* Forward; scratch as for fa_b200_fwd_with_workspace. */
 int fa_b200_fwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r, void* workspace, size_t workspace_bytes);
-size_t fa_b200_fwd_rules_workspace_bytes(const fa_b200_params* p);
+size_t fa_b200_fwd_rules_workspace_bytes(const fa_b200_params* p, const fa_b200_rules* r);
 /* Backward, deterministic; p->workspace holds at least fa_b200_bwd_rules_workspace_bytes(p) bytes. */
 int fa_b200_bwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r);
 size_t fa_b200_bwd_rules_workspace_bytes(const fa_b200_params* p);
