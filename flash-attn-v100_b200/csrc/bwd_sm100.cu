@@ -334,6 +334,7 @@ __device__ __forceinline__ BwdItem make_item(const BwdArgs& a, const CtaWork& cw
     m.rot = 0;
     if (KS) {
         m.tile = cw.tile_rank;                        // key tile: the first one sees the most query tiles
+        if (RULES) m.tile = min(max(a.rules.k_order[m.b * a.rules.k_tiles_b + cw.tile_rank], 0), (int)gridDim.x - 1);      // the longest first
         m.head_kv = cw.head;
         // first query tile that sees this key tile: query i sees key j iff j <= i + shift
         m.it0 = a.causal ? (m.tile * kTile > a.shift ? (m.tile * kTile - a.shift) / kTile : 0) : 0;
@@ -352,7 +353,8 @@ __device__ __forceinline__ BwdItem make_item(const BwdArgs& a, const CtaWork& cw
         // staggered already).
         if (FUSED && !a.causal && m.n_per_head > 0) m.rot = m.tile % m.n_per_head;
     } else {
-        m.tile = a.causal || RULES ? (int)gridDim.x - 1 - cw.tile_rank : cw.tile_rank;     // query tile, heavy first
+        m.tile = a.causal ? (int)gridDim.x - 1 - cw.tile_rank : cw.tile_rank;     // query tile, heavy first
+        if (RULES) m.tile = min(max(a.rules.q_order[m.b * a.rules.q_tiles_b + cw.tile_rank], 0), (int)gridDim.x - 1);
         m.head_kv = cw.head / a.group;
         m.it0 = 0;
         int kv_end = m.nk;

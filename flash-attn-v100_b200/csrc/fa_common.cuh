@@ -101,9 +101,13 @@ constexpr int kVariantPair = 16;
 //                                     largest first, least end of all rows below Nq (2^31 - 1, 0 if one sees nothing)
 //   q_parts  [B][nq_pad / 16]   int2  the same hull for 16 rows
 //   k_tiles  [B][nk_pad / 128]  int2  first and end of the query tiles whose hull meets the key tile ((0, 0): none)
+//   q_order, p_order, k_order         [B][nq_pad / 128], [B][pairs of them], [B][nk_pad / 128]: query tiles, pairs of them and
+//                                     key tiles with those that meet most of the others first (in their order beyond
+//                                     kMostOrdered tiles)
 //   origin   [B]                      position of row 0
+constexpr int kMostOrdered = 512;
 struct RangesLayout {
-    int64_t q_tiles, q_parts, k_tiles, origin, total;          // in int32; rows are at 0
+    int64_t q_tiles, q_parts, k_tiles, q_order, p_order, k_order, origin, total;          // in int32; rows are at 0
     int nq_pad, nk_pad;
 };
 static inline __host__ __device__ RangesLayout ranges_layout(int64_t B, int Nq, int Nk) {
@@ -113,14 +117,18 @@ static inline __host__ __device__ RangesLayout ranges_layout(int64_t B, int Nq, 
     l.q_tiles = B * l.nq_pad * 2;
     l.q_parts = l.q_tiles + B * (l.nq_pad / 128) * 4;
     l.k_tiles = l.q_parts + B * (l.nq_pad / 16) * 2;
-    l.origin = l.k_tiles + B * (l.nk_pad / 128) * 2;
+    l.q_order = l.k_tiles + B * (l.nk_pad / 128) * 2;
+    l.p_order = l.q_order + B * (l.nq_pad / 128);
+    l.k_order = l.p_order + B * ((l.nq_pad / 128 + 1) / 2);
+    l.origin = l.k_order + B * (l.nk_pad / 128);
     l.total = l.origin + (B + 3) / 4 * 4;
     return l;
 }
 // The rules of a call as its kernels read them (rows = nullptr: none).  Strides over the batch, 0 where one plan serves all.
 struct Rules {
-    const int2* rows; const int4* q_tiles; const int2* q_parts; const int2* k_tiles; const int32_t* origin;
-    int64_t rows_b, q_tiles_b, q_parts_b, k_tiles_b, origin_b;
+    const int2* rows; const int4* q_tiles; const int2* q_parts; const int2* k_tiles;
+    const int32_t *q_order, *p_order, *k_order, *origin;
+    int64_t rows_b, q_tiles_b, q_parts_b, k_tiles_b, p_order_b, origin_b;         // (q_order as q_tiles, k_order as k_tiles)
     const float* slopes;           // optional, one per head
     float cap;                     // 0: none
     int max_keys;                  // most keys a row sees (0: not known); a hint
@@ -131,7 +139,9 @@ static inline Rules make_rules(const fa_b200_rules& r, int Nq, int Nk) {
     const bool shared = r.plan_batch == 1;
     Rules u;
     u.rows = (const int2*)base; u.q_tiles = (const int4*)(base + l.q_tiles); u.q_parts = (const int2*)(base + l.q_parts);
-    u.k_tiles = (const int2*)(base + l.k_tiles); u.origin = base + l.origin;
+    u.k_tiles = (const int2*)(base + l.k_tiles);
+    u.q_order = base + l.q_order; u.p_order = base + l.p_order; u.k_order = base + l.k_order; u.p_order_b = shared ? 0 : (l.nq_pad / 128 + 1) / 2;
+    u.origin = base + l.origin;
     u.rows_b = shared ? 0 : l.nq_pad; u.q_tiles_b = shared ? 0 : l.nq_pad / 128; u.q_parts_b = shared ? 0 : l.nq_pad / 16;
     u.k_tiles_b = shared ? 0 : l.nk_pad / 128; u.origin_b = shared ? 0 : 1;
     u.slopes = r.slopes; u.cap = r.score_cap; u.max_keys = r.max_keys;

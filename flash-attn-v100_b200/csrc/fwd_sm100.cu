@@ -373,8 +373,8 @@ template <> struct WorkLoop<0, 0> {       // whole pairs, round robin
 };
 // Whole pairs with rules: what a pair costs is on the device, so pairs are not dealt out beforehand.  The grid has a block a
 // pair; a CTA starts with its own and goes on with blocks not yet launched (clusterlaunchcontrol, as in the backward).
-// The order: groups of columns whose K and V stay in L2, in a group the last pair of all columns first, which under a
-// causal mask is the longest, then the one before it.  The producer asks (Dealer) and leaves the pair's number in one of two
+// The order: groups of columns whose K and V stay in L2, in a group the longest pair of every column first, then the second
+// (the plan's p_order).  The producer asks (Dealer) and leaves the pair's number in one of two
 // slots for the other roles (WorkLoop).  Round robin: B4 N4096 H32 D128 bf16 with 8 documents a row 317 us.
 struct Deal {                              // in shared memory, at RangeStart's place; 16-byte aligned answer
     int w[2], pad[2];
@@ -386,9 +386,9 @@ __device__ __forceinline__ void dealt_stretch(const FwdArgs& a, int w, Stretch& 
     const int group = w / per_group, at = w - group * per_group;
     const int here = min(a.cols_per_group, cols - group * a.cols_per_group);
     const int col = group * a.cols_per_group + at % here;
-    s.pair = a.n_pairs - 1 - at / here;
     s.h = col % a.H;
     s.b = col / a.H;
+    s.pair = min(max(a.rules.p_order[s.b * a.rules.p_order_b + at / here], 0), a.n_pairs - 1);
     stretch_blocks<RULES>(a, kBlockM, s);
     s.j0 = s.jb;
     s.j1 = s.n[0] > s.n[1] ? s.n[0] : s.n[1];

@@ -70,7 +70,7 @@ __device__ __forceinline__ int2 row_of(const RangesArgs& a, int b, int i, int64_
 
 // A block makes the 128 rows of a query tile.
 __global__ void __launch_bounds__(128) key_rows_kernel(const RangesArgs a) {
-    ptx::grid_launch_dependents();                 // key_tiles_kernel, which waits for this grid's end
+    ptx::grid_launch_dependents();                 // key_orders_kernel or key_tiles_kernel, which waits for this grid's end
     const RangesLayout l = ranges_layout(a.B, a.Nq, a.Nk);
     __shared__ int4 part[4];
     const int tile = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -114,30 +114,90 @@ __global__ void __launch_bounds__(128) key_rows_kernel(const RangesArgs a) {
         __syncthreads();
         const int4 whole = part[0];
         int2* k_tiles = (int2*)(a.plan + l.k_tiles) + (int64_t)b * (l.nk_pad / 128);
-        for (int j = threadIdx.x; j < l.nk_pad / 128; j += 128)
+        int32_t* k_order = a.plan + l.k_order + (int64_t)b * (l.nk_pad / 128);
+        for (int j = threadIdx.x; j < l.nk_pad / 128; j += 128) {
             k_tiles[j] = make_int2(0, whole.x < j * 128 + 128 && whole.y > j * 128 ? 1 : 0);
+            k_order[j] = j;
+        }
+        if (threadIdx.x == 0) { a.plan[l.q_order + b] = 0; a.plan[l.p_order + b] = 0; }
     }
 }
 
-// A warp makes a key tile's list: the first and the last query tile whose hull meets it.
+// Key tiles' lists; the orders as they come.  For many tiles: a warp a key tile, all over the GPU.
 __global__ void __launch_bounds__(256) key_tiles_kernel(const RangesArgs a) {
     ptx::grid_dependency_wait();
     const RangesLayout l = ranges_layout(a.B, a.Nq, a.Nk);
     const int j = (int)blockIdx.x * 8 + (int)(threadIdx.x >> 5), b = blockIdx.y, lane = threadIdx.x & 31;
-    if (j >= l.nk_pad / 128) return;
-    const int n = l.nq_pad / 128;
+    const int n = l.nq_pad / 128, nk = l.nk_pad / 128, np = (n + 1) / 2;
+    for (int i = (int)(blockIdx.x * blockDim.x + threadIdx.x); i < n; i += (int)(gridDim.x * blockDim.x)) {
+        a.plan[l.q_order + (int64_t)b * n + i] = n - 1 - i;
+        if (i < np) a.plan[l.p_order + (int64_t)b * np + i] = np - 1 - i;
+    }
+    if (j >= nk) return;
     const int4* q_tiles = (const int4*)(a.plan + l.q_tiles) + (int64_t)b * n;
     int lo = INT_MAX, hi = 0;
     for (int t = lane; t < n; t += 32) {
         const int4 h = q_tiles[t];
         if (h.x < j * 128 + 128 && h.y > j * 128) { lo = min(lo, t); hi = t + 1; }
     }
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) {
+        ((int2*)(a.plan + l.k_tiles))[(int64_t)b * nk + j] = hi > 0 ? make_int2(lo, hi) : make_int2(0, 0);
+        a.plan[l.k_order + (int64_t)b * nk + j] = j;
     }
-    if (lane == 0) ((int2*)(a.plan + l.k_tiles))[(int64_t)b * (l.nk_pad / 128) + j] = hi > 0 ? make_int2(lo, hi) : make_int2(0, 0);
+}
+// The same for at most kMostOrdered tiles, a block a batch entry, and the orders: a tile's place is the number of tiles that
+// meet more others, or as many and come first (later ones first for queries, where a causal mask makes them the longer ones).
+__global__ void __launch_bounds__(1024) key_orders_kernel(const RangesArgs a) {
+    __shared__ int4 hulls[kMostOrdered];
+    __shared__ __align__(16) int cost[3][kMostOrdered];
+    const RangesLayout l = ranges_layout(a.B, a.Nq, a.Nk);
+    const int b = blockIdx.x, n = l.nq_pad / 128, nk = l.nk_pad / 128, np = (n + 1) / 2;
+    for (int i = threadIdx.x; i < 3 * kMostOrdered; i += 1024) (&cost[0][0])[i] = -1;        // (places behind the last tile: no place taken)
+    ptx::grid_dependency_wait();
+    for (int t = threadIdx.x; t < n; t += 1024) hulls[t] = ((const int4*)(a.plan + l.q_tiles))[(int64_t)b * n + t];
+    __syncthreads();
+    auto tiles_of = [](int x, int y) { return y > x ? (y + 127) / 128 - x / 128 : 0; };
+    static_assert(2 * kMostOrdered == 1024, "half of the threads for the keys, half for the queries");
+    if (threadIdx.x < kMostOrdered) {
+        // a thread a key tile, which all look at the same query tile
+        const int j = threadIdx.x;
+        if (j < nk) {
+            int lo = INT_MAX, hi = 0;
+#pragma unroll 4
+            for (int t = 0; t < n; ++t) {
+                const int4 h = hulls[t];
+                if (h.x < j * 128 + 128 && h.y > j * 128) { lo = min(lo, t); hi = t + 1; }
+            }
+            const int2 r = hi > 0 ? make_int2(lo, hi) : make_int2(0, 0);
+            ((int2*)(a.plan + l.k_tiles))[(int64_t)b * nk + j] = r;
+            cost[0][j] = r.y - r.x;
+        }
+    } else {
+        const int t = threadIdx.x - kMostOrdered;
+        if (t < n) {
+            const int4 h = hulls[t];
+            cost[1][t] = tiles_of(h.x, h.y);
+            if (t % 2 == 0) {
+                const int4 g = t + 1 < n ? hulls[t + 1] : make_int4(0, 0, 0, 0);
+                cost[2][t / 2] = h.y <= 0 ? tiles_of(g.x, g.y) : (g.y <= 0 ? tiles_of(h.x, h.y) : tiles_of(min(h.x, g.x), max(h.y, g.y)));
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < nk + n + np; i += 1024) {
+        const int o = i < nk ? 0 : (i < nk + n ? 1 : 2), count = o == 0 ? nk : (o == 1 ? n : np), me = i - (o == 0 ? 0 : (o == 1 ? nk : nk + n));
+        const int mine = cost[o][me];
+        int place = 0;
+        for (int e = 0; e < count; e += 4) {
+            const int4 c = *reinterpret_cast<const int4*>(&cost[o][e]);
+            auto ahead = [&](int x, int at) { return x > mine || (x == mine && (o == 0 ? at < me : at > me)); };
+            place += ahead(c.x, e) + ahead(c.y, e + 1) + ahead(c.z, e + 2) + ahead(c.w, e + 3);
+        }
+        const int64_t base = o == 0 ? l.k_order + (int64_t)b * nk : (o == 1 ? l.q_order + (int64_t)b * n : l.p_order + (int64_t)b * np);
+        a.plan[base + place] = me;
+    }
 }
 
 }  // namespace
@@ -184,16 +244,17 @@ int fa_b200_key_ranges(const fa_b200_ranges_params* p) {
     key_rows_kernel<<<dim3((unsigned)(l.nq_pad / 128), (unsigned)p->B), 128, 0, st>>>(a);
     FA_CUDA_CHECK(cudaGetLastError());
     if (l.nq_pad > 128 && l.nk_pad > 0) {
+        const bool ordered = l.nq_pad / 128 <= kMostOrdered && l.nk_pad / 128 <= kMostOrdered;
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)((l.nk_pad / 128 + 7) / 8), (unsigned)p->B);
-        cfg.blockDim = dim3(256);
+        cfg.gridDim = ordered ? dim3((unsigned)p->B) : dim3((unsigned)((l.nk_pad / 128 + 7) / 8), (unsigned)p->B);
+        cfg.blockDim = dim3(ordered ? 1024 : 256);
         cfg.stream = st;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        FA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, key_tiles_kernel, a));
+        FA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ordered ? key_orders_kernel : key_tiles_kernel, a));
     }
     return FA_OK;
 }

@@ -202,7 +202,7 @@ void ruled_backward(at::Tensor d_o, const at::Tensor& q, const at::Tensor& k, co
 struct RuledAttention : torch::autograd::Function<RuledAttention> {
     static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const Ruled& r) {
         at::Tensor o, lse, o_lo;
-        ruled_forward(q, k, v, r, false, q.scalar_type() == at::kBFloat16, o, lse, o_lo);
+        ruled_forward(q, k, v, r, false, q.scalar_type() != at::kFloat, o, lse, o_lo);
         ctx->save_for_backward({q, k, v, o, lse, r.plan, o_lo, r.slopes});
         ctx->saved_data["scale"] = r.scale;
         ctx->saved_data["cap"] = r.cap;

@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from ..kernels import _cabi
-from .attention import _base_params, _tensor4, _variant_override, saves_output_residual
+from .attention import _base_params, _tensor4, _variant_override
 from ..utils import _last_dim_contiguous
 from .key_ranges import KeyRanges
 
@@ -104,8 +104,9 @@ class RuledAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, scale, cap, slopes, plan, plan_batch, max_keys):
+        # what rounding o to 16 bits dropped goes to the backward: without it half of the error of fp16 dQ and dK was delta's
         needs_grad = any(ctx.needs_input_grad[:3])
-        o_lo = torch.empty(q.shape, dtype=q.dtype, device=q.device) if needs_grad and saves_output_residual(q.dtype) else None
+        o_lo = torch.empty(q.shape, dtype=q.dtype, device=q.device) if needs_grad and q.dtype != torch.float32 else None
         o, lse = launch_forward_rules(q, k, v, scale, cap, slopes, plan, plan_batch, o_residual=o_lo, split_keys=not needs_grad, max_keys=max_keys)
         ctx.save_for_backward(q, k, v, o, lse, slopes, plan, o_lo)
         ctx.how = (scale, cap, plan_batch)

@@ -70,6 +70,21 @@ def check(r, Nq, Nk, batch, host):
         for n in range(nk):
             meets = ((tiles[:, 0] < n * 128 + 128) & (tiles[:, 1] > n * 128)).nonzero()
             assert keys[n].tolist() == ([int(meets.min()), int(meets.max()) + 1] if len(meets) else [0, 0]), (b, n)
+        # the orders: every tile once, those that meet most first
+        at = r.batch * (nq * 276 + nk * 2)
+        for count, cost in ((nq, lambda t: -(-int(tiles[t, 1]) // 128) - int(tiles[t, 0]) // 128),
+                            ((nq + 1) // 2, lambda p: _pair_cost(tiles[2 * p:2 * p + 2])), (nk, lambda n: int(keys[n, 1] - keys[n, 0]))):
+            order = hull[at + b * count:at + (b + 1) * count].tolist()
+            at += r.batch * count
+            assert sorted(order) == list(range(count))
+            costs = [cost(i) for i in order]
+            if nq > 1 and max(nq, nk) <= 512:
+                assert costs == sorted(costs, reverse=True), (b, costs)
+
+
+def _pair_cost(tiles):
+    some = tiles[tiles[:, 1] > 0]
+    return -(-int(some[:, 1].max()) // 128) - int(some[:, 0].min()) // 128 if len(some) else 0
 
 
 @pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=["int32", "int64"])

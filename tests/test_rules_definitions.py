@@ -145,8 +145,8 @@ def test_bad_range_parameters_are_refused_before_any_cuda_call(change, code):
     assert lib.fa_b200_key_ranges(ctypes.byref(p)) == code
     assert lib.fa_b200_key_ranges(None) == _cabi.FA_EINVAL
     assert lib.fa_b200_key_ranges_bytes(-1, 4, 4) == 0
-    # rows, 128-row hulls, 16-row hulls, key tiles, origins
-    assert lib.fa_b200_key_ranges_bytes(2, 129, 300) == 4 * (2 * 256 * 2 + 2 * 2 * 4 + 2 * 16 * 2 + 2 * 3 * 2 + 4)
+    # rows, 128-row hulls, 16-row hulls, key tiles, three orders, origins
+    assert lib.fa_b200_key_ranges_bytes(2, 129, 300) == 4 * (2 * 256 * 2 + 2 * 2 * 4 + 2 * 16 * 2 + 2 * 3 * 2 + 2 * (2 + 1 + 3) + 4)
 
 
 @pytest.mark.parametrize("change,code", [
