@@ -22,13 +22,15 @@ the kernels underneath:
 from __future__ import annotations
 
 import warnings
-from typing import Any, Dict, Optional, Tuple
+from typing import Any, Dict, Optional, Tuple, Union
 
 import torch
 from torch import nn
 
-from .interface import flash_attention_v100
+from .interface import flash_attention_v100, flash_attention_v100_with_rules
 from .kernels import _cabi
+from .ops.key_ranges import KeyRanges
+from .ops.rotary import rotary_embedding, rotary_frequencies
 
 
 def masks_to_bias(attn_mask: Optional[torch.Tensor], key_padding_mask: Optional[torch.Tensor],
@@ -122,14 +124,29 @@ def _rows_can_be_moved(k: torch.Tensor, v: torch.Tensor, mask: torch.Tensor) -> 
             k.shape[0] * k.shape[1] * (row // 16) < 1 << 32)
 
 
+def _warn_no_weights() -> None:
+    warnings.warn("need_weights=True: attention weights are never materialised by these kernels; "
+                  "None is returned for them.", UserWarning, stacklevel=3)
+
+
 class EnhancedMultiHeadAttention(nn.Module):
     def __init__(self, embed_dim: int, num_heads: int, dropout: float = 0.0, bias: bool = True,
                  batch_first: bool = True, optimization_strategy: str = "balanced",
                  enable_multi_gpu: bool = True, enable_gradient_checkpointing: bool = False,
-                 enable_performance_monitoring: bool = False):
+                 enable_performance_monitoring: bool = False, rotary_base: Optional[float] = None,
+                 rotary_dim: Optional[int] = None, score_cap: Optional[float] = None,
+                 distance_slopes: Optional[torch.Tensor] = None):
+        """After the reference's arguments, for language models: rotary_base turns q and k by their positions
+        (rotary_embedding, rotary_dim columns of a head, default all); score_cap and distance_slopes ((num_heads,)) are
+        flash_attention_v100_with_rules'.  None of them has parameters or an entry in the state dict; a layer with a cap or
+        slopes takes neither masks as tensors nor dropout."""
         super().__init__()
         if embed_dim % num_heads != 0:
             raise ValueError("embed_dim must be divisible by num_heads")
+        if rotary_dim is not None and (rotary_base is None or rotary_dim % 2 or not 0 < rotary_dim <= embed_dim // num_heads):
+            raise ValueError(f"rotary_dim must be even, at most the head size {embed_dim // num_heads}, and come with rotary_base")
+        if distance_slopes is not None and tuple(distance_slopes.shape) != (num_heads,):
+            raise ValueError(f"distance_slopes must have shape ({num_heads},), got {tuple(distance_slopes.shape)}")
         self.embed_dim, self.num_heads = embed_dim, num_heads
         self.head_dim = embed_dim // num_heads
         self.dropout = dropout
@@ -144,6 +161,11 @@ class EnhancedMultiHeadAttention(nn.Module):
         self.v_proj = nn.Linear(embed_dim, embed_dim, bias=bias)
         self.out_proj = nn.Linear(embed_dim, embed_dim, bias=bias)
         self.forward_count = 0
+        self.score_cap = None if score_cap is None else float(score_cap)
+        # (64 bits, which a module's conversion to a floating type would round: built where it is used)
+        self.rotary = None if rotary_base is None else (rotary_dim or self.head_dim, float(rotary_base))
+        self._inv_freq: Dict[torch.device, torch.Tensor] = {}
+        self.register_buffer("distance_slopes", None if distance_slopes is None else distance_slopes.detach().float(), persistent=False)
         self.reset_parameters()
 
     def reset_parameters(self) -> None:
@@ -156,9 +178,13 @@ class EnhancedMultiHeadAttention(nn.Module):
                 value: Optional[torch.Tensor] = None, key_padding_mask: Optional[torch.Tensor] = None,
                 attn_mask: Optional[torch.Tensor] = None, need_weights: bool = False,
                 average_attn_weights: bool = True, is_causal: bool = False,
-                key_lengths: Optional[torch.Tensor] = None
-                ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-        """Reference signature plus key_lengths (B,): for right-padded batches, the number of real keys
+                key_lengths: Optional[torch.Tensor] = None, key_ranges: Optional[KeyRanges] = None,
+                positions: Union[torch.Tensor, int, None] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+        """key_ranges (build_key_ranges) says which keys each query sees, in the place of all masks; positions are those of the
+        queries and keys for a rotary layer (default: key_ranges' positions where there are as many queries as keys, else
+        0, 1, ...; queries and keys of different lengths need a layer without rotary).
+
+        Reference signature plus key_lengths (B,): for right-padded batches, the number of real keys
         of each batch entry; the call stays on the tensor-core kernels and skips the padding's key
         blocks.  A boolean key_padding_mask alone (no attn_mask, is_causal False) gets there too, by moving
         the kept keys to the front (compact_keys); combined with other masks, or as a float mask, it
@@ -175,6 +201,24 @@ class EnhancedMultiHeadAttention(nn.Module):
         q = self.q_proj(query).view(batch, seq_q, self.num_heads, self.head_dim)
         k = self.k_proj(key).view(batch, seq_k, self.num_heads, self.head_dim)
         v = self.v_proj(value).view(batch, seq_k, self.num_heads, self.head_dim)
+        if self.rotary is not None:
+            if seq_q != seq_k:
+                raise ValueError("a rotary layer needs as many keys as queries: turn them before, with rotary_embedding")
+            if positions is None and key_ranges is not None:
+                positions = key_ranges.positions
+            q, k = rotary_embedding(q, k, inv_freq=self._frequencies(q.device), positions=positions)
+        elif positions is not None:
+            raise ValueError("positions are for a layer with rotary_base")
+        if key_ranges is not None or self.score_cap is not None or self.distance_slopes is not None:
+            if attn_mask is not None or key_padding_mask is not None or (self.training and self.dropout):
+                raise ValueError("key_ranges, score_cap and distance_slopes cannot be combined with mask tensors or dropout")
+            if need_weights:
+                _warn_no_weights()
+            self.forward_count += 1
+            out = flash_attention_v100_with_rules(q, k, v, causal=is_causal, score_cap=self.score_cap, distance_slopes=self.distance_slopes,
+                                                  key_ranges=key_ranges, key_lengths=key_lengths,
+                                                  enable_profiling=self.enable_performance_monitoring)
+            return self._project(out, batch, seq_q), None
         if key_padding_mask is not None and key_padding_mask.dtype == torch.bool and attn_mask is None \
                 and not is_causal and key_lengths is None:
             if tuple(key_padding_mask.shape) != (batch, seq_k):
@@ -186,17 +230,22 @@ class EnhancedMultiHeadAttention(nn.Module):
             key_padding_mask = None
         bias = masks_to_bias(attn_mask, key_padding_mask, batch, seq_q, seq_k)
         if need_weights:
-            warnings.warn("need_weights=True: attention weights are never materialised by these kernels; "
-                          "None is returned for them.", UserWarning)
+            _warn_no_weights()
         self.forward_count += 1
         out = flash_attention_v100(q, k, v, causal=is_causal, dropout_p=self.dropout if self.training else 0.0,
                                    bias=bias, optimization_strategy=self.optimization_strategy,
                                    enable_multi_gpu=self.enable_multi_gpu,
                                    enable_profiling=self.enable_performance_monitoring, key_lengths=key_lengths)
+        return self._project(out, batch, seq_q), None
+
+    def _project(self, out: torch.Tensor, batch: int, seq_q: int) -> torch.Tensor:
         out = self.out_proj(out.reshape(batch, seq_q, self.embed_dim))
-        if not self.batch_first:
-            out = out.transpose(0, 1)
-        return out, None
+        return out if self.batch_first else out.transpose(0, 1)
+
+    def _frequencies(self, device: torch.device) -> torch.Tensor:
+        if device not in self._inv_freq:
+            self._inv_freq[device] = rotary_frequencies(self.rotary[0], self.rotary[1], device=device)[0]
+        return self._inv_freq[device]
 
     def get_performance_stats(self) -> Optional[Dict[str, Any]]:
         """Reference :252-256.  Only the call count is kept here; time the layer with CUDA events."""
