@@ -100,7 +100,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // inputs' own format and every accumulating MMA is issued for both, so they keep 17 (bf16) or 22 (fp16) significant
 // bits and no operand is converted.  2: the same with the step's 128 x 128 bias tile brought to shared memory by TMA
 // (see the forward; here the key-stationary kernel would read a value, the other one 16 bytes of 32 lines, per load).
-template <int D, int MODE, int DROP, int PREC>
+template <int D, int MODE, int DROP, int PREC, int RULES = 0>
 struct BwdCfg {
     static constexpr int kNBox = D / 64;
     static constexpr int kTileBytes = kNBox * kBoxBytes;
@@ -148,13 +148,15 @@ struct BwdCfg {
     // two slots of lse[128] | delta[128]; MODE 1: the rows' lse[128] | delta[128] | exponents[128], pairs: later a partial
     // sum of each row from every warpgroup
     static constexpr int kVecBytes = MODE != 1 ? 2 * 1024 : (PREC ? 128 * 4 * kNWG : 3 * 512);
+    // rules, key-stationary: which rows of the key tile a step's queries see, two bytes a query, with the vectors' slots
+    static constexpr int kSeesBytes = RULES != 0 && MODE == 0 ? 2 * 256 : 0;
     static constexpr int kDsBytes = 128 * 128 * 2;               // fused kernel: dS^T tile for the dQ MMA
     static constexpr int kBarBytes = (kNumBars * 8 + 15) / 16 * 16;
     // behind the barriers: TMEM slot, abort flag and wait limit (16 bytes), the answer to a request for a block (16),
     // two BwdItem
     static constexpr int kCtlBytes = 32 + 2 * 48;
     // bytes used from the 1024-aligned base: X, Y, U ring, W ring, [dS], [vectors], barriers, control words, [masks]
-    static constexpr int kUsedBytes = (2 + kUStages + kWStages) * kTileBytes + kBiasBytes + (kFused ? kDsBytes : 0) + kVecBytes +
+    static constexpr int kUsedBytes = (2 + kUStages + kWStages) * kTileBytes + kBiasBytes + (kFused ? kDsBytes : 0) + kVecBytes + kSeesBytes +
                                       kBarBytes + kCtlBytes + (kMasks ? kMaskBytes : 0);
     static constexpr int kMaxSmem = 232448;                      // 227 KB: the most one CTA can ask for
     static_assert(128 * kNWG + 128 == 32 * tile::kBwdWarps, "thread count and table disagree");
@@ -203,6 +205,9 @@ struct BwdArgs {
     // Calls with rules (RULES != 0):
     Rules rules;
     float cap_in, cap_out;         // u = S * cap_in, x = tanh(u) * cap_out (log2 units)
+    // dK/dV kernel: a block is a key tile and one query head, its sums go here in fp32 (bwd_heads_kernel adds them up):
+    // [B*H][key tiles][dK, dV][D / 4][128 rows][4]; nullptr: a key tile and all query heads of its K/V head
+    float* part;
 };
 
 __device__ __forceinline__ void bulk_load_1d(void* smem_dst, const void* gsrc, uint32_t bytes, uint64_t* bar) {
@@ -322,7 +327,8 @@ struct BwdItem {
     int n_iter;                        // steps in all; -1: no block any more
     int rot;                           // FUSED: see q_tile_of
     float range[2];                    // max |dO|, max |V| of the column
-    int head_kv, pad;
+    int head_kv;
+    int head_q0;                       // rules, key-stationary: first query head
 };
 static_assert(sizeof(BwdItem) == 48, "kCtlBytes");
 template <bool KS, bool FUSED, bool DS, int RULES>
@@ -348,6 +354,12 @@ __device__ __forceinline__ BwdItem make_item(const BwdArgs& a, const CtaWork& cw
             m.n_per_head = max(min(seen.y, nq_tiles) - m.it0, 0);
         }
         m.n_iter = m.n_per_head * a.group;
+        m.head_q0 = cw.head * a.group;
+        if (RULES && a.part) {
+            m.head_q0 = cw.head;
+            m.head_x = m.head_kv = cw.head / a.group;
+            m.n_iter = m.n_per_head;
+        }
         // The fused kernel without a causal mask starts each key tile's walk at a different query tile, so that the CTAs
         // of one head, which run at the same time, add to different dQ tiles (under a causal mask the walks are
         // staggered already).
@@ -389,7 +401,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                  const __grid_constant__ CUtensorMap map_out1, const __grid_constant__ CUtensorMap map_out2,
                  const __grid_constant__ CUtensorMap map_aux, const __grid_constant__ CUtensorMap map_bias,
                  const __grid_constant__ CUtensorMap map_ds, const BwdArgs a) {
-    using Cfg = BwdCfg<D, MODE, DROP, PREC>;
+    using Cfg = BwdCfg<D, MODE, DROP, PREC, RULES>;
     constexpr bool KS = (MODE != 1);        // key-stationary: K, V stay, query tiles stream
     constexpr bool FUSED = (MODE == 2);     // key-stationary and dQ too
     constexpr bool CONV = BF16 && PREC == 0;    // every MMA runs f16 x f16: bf16 tiles are converted
@@ -415,7 +427,8 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     uint8_t* sBias = sW + WST * TILE;               // PREC = 2
     uint8_t* sDs = sBias + Cfg::kBiasBytes;         // fused kernel only
     float* sVec = (float*)(sDs + (FUSED ? Cfg::kDsBytes : 0));      // key-stationary: 2 x (lse[128] | delta[128]); see kVecBytes
-    uint64_t* bars = (uint64_t*)((uint8_t*)sVec + Cfg::kVecBytes);
+    [[maybe_unused]] uint8_t* sSees = (uint8_t*)sVec + Cfg::kVecBytes;      // [2][128][2]
+    uint64_t* bars = (uint64_t*)(sSees + Cfg::kSeesBytes);
     uint32_t* tmem_slot = (uint32_t*)((uint8_t*)bars + Cfg::kBarBytes);
     volatile uint32_t* abort_flag = (volatile uint32_t*)(tmem_slot + 1);
     uint32_t* clc_answer = tmem_slot + 4;
@@ -447,7 +460,8 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     constexpr int kAllThreads = 128 * NWG + kExtraThreads;
     if (warp == kTmaWarp) {
         // the producer's warp sets the barriers up, so that the first loads need not wait for the other warps
-        constexpr uint32_t kReaders = 4u * NWG + 2u + ((STREAM_CONV || PREC == 2) ? 1u : 0u);
+        constexpr bool SEES = RULED && KS;        // warp 18 adds what a step's queries see to its vectors
+        constexpr uint32_t kReaders = 4u * NWG + 2u + ((STREAM_CONV || PREC == 2 || SEES) ? 1u : 0u);
         for (int i = lane; i < Cfg::kNumBars; i += 32) {
             const bool wide = (i == Cfg::kPReady || i == Cfg::kDsReady || i == Cfg::kMask || i == Cfg::kEpi || i == Cfg::kRowEmpty ||
                                i == Cfg::kXConv || i == Cfg::kYConv ||
@@ -458,6 +472,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             if (i == Cfg::kSchedEmpty || i == Cfg::kSchedEmpty + 1) count = kReaders;
             if (i == Cfg::kXEmpty && K_COPY) count = 2u;              // the MMAs and the copy of K
             if (i == Cfg::kYEmpty && ROW_MAX) count = 1u + 4u * NWG;
+            if (SEES && (i == Cfg::kVFull || i == Cfg::kVFull + 1)) count = 2u;
             mbar_init(&bars[i], count);
         }
         if (lane == 0) wait_control_init(abort_flag, a.wait_limit_ms);
@@ -533,6 +548,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 volatile BwdItem* d = sched + slot;
                 d->tile = m.tile; d->head_x = m.head_x; d->b = m.b; d->nk = m.nk; d->it0 = m.it0; d->n_per_head = m.n_per_head;
                 d->n_iter = m.n_iter; d->rot = m.rot; d->range[0] = rg.x; d->range[1] = rg.y; d->head_kv = m.head_kv;
+                if (RULED && KS) d->head_q0 = m.head_q0;
                 mbar_arrive(&bars[Cfg::kSchedFull + slot]);
             };
             for (int k = 0; ok; ++k) {
@@ -549,7 +565,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 int qi = 0, hg = 0;
                 for (int it = 0; it < m.n_iter; ++it) {
                     int head_u, row_u;
-                    if (KS) { head_u = m.head_x * a.group + hg; row_u = q_tile_of(m.it0, m.n_per_head, m.rot, qi) * kTile; }
+                    if (KS) { head_u = (RULED ? m.head_q0 : m.head_x * a.group) + hg; row_u = q_tile_of(m.it0, m.n_per_head, m.rot, qi) * kTile; }
                     else    { head_u = m.head_kv; row_u = ((RULED ? m.it0 : 0) + k_tile_of(m.n_per_head, it)) * kTile; }
                     ok = mbar_wait(&bars[Cfg::kUEmpty + us], (uph & 1u) ^ 1u, abort_flag);
                     if (!ok) break;
@@ -863,7 +879,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             if (stores && mbar_wait(&bars[Cfg::kEpi], (uint32_t)items & 1u, abort_flag, kIdleNs, (uint32_t)n_iter + 1u)) {
                 const int su = (steps - 1) % UST, sw = (steps - 1) % WST;
 #pragma unroll
-                for (int bx = 0; bx < Cfg::kNBox; ++bx) {
+                for (int bx = 0; bx < (RULED && KS && a.part ? 0 : Cfg::kNBox); ++bx) {
                     tma_store_4d(&map_out1, sU + su * TILE + bx * kBoxBytes, bx * 64, head, row0, b);
                     if (KS) tma_store_4d(&map_out2, sW + sw * TILE + bx * kBoxBytes, bx * 64, head, row0, b);
                 }
@@ -874,6 +890,38 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             }
             __syncwarp();
             ++items;
+        }
+      } else if (RULED && KS && warp == kTmaWarp + 1) {
+        // ---------------------------------------------------------------- warp 18: what the steps' queries see of the key tile
+        // (read by the threads themselves, from global memory behind the wait for a step's first product, the masked steps of
+        // short documents took 3.3 us where whole ones take 2.1)
+        int v = 0;
+        bool ok = true;
+        for (int k = 0; ok; ++k) {
+            ok = __all_sync(0xffffffffu, item_there(k));
+            if (!ok) break;
+            const volatile BwdItem* m = sched + (k & 1);
+            const int n_iter = m->n_iter, n_per_head = m->n_per_head, it0 = m->it0, tile = m->tile, b = m->b;
+            mbar_arrive_warp(&bars[Cfg::kSchedEmpty + (k & 1)]);
+            if (n_iter < 0) break;
+            int qi = 0;
+            for (int it = 0; it < n_iter; ++it, ++v) {
+                const int row = q_tile_of(it0, n_per_head, 0, qi) * kTile + lane * 4;
+                const int4* rows = reinterpret_cast<const int4*>(a.rules.rows + b * a.rules.rows_b + row);
+                const int4 x = rows[0], y = rows[1];
+                auto pair = [&](int first, int end, int q) {
+                    // rows of the tile, a byte each (128: none); a row of no query has no P whatever it sees
+                    if (q >= a.Nq) return (uint32_t)kTile << 8;
+                    return (uint32_t)min(max(first - tile * kTile, 0), kTile) | (uint32_t)min(max(end - tile * kTile, 0), kTile) << 8;
+                };
+                const uint2 w = make_uint2(pair(x.x, x.y, row) | pair(x.z, x.w, row + 1) << 16, pair(y.x, y.y, row + 2) | pair(y.z, y.w, row + 3) << 16);
+                ok = mbar_wait(&bars[Cfg::kVEmpty + (v & 1)], ((uint32_t)(v >> 1) & 1u) ^ 1u, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                *reinterpret_cast<uint2*>(sSees + (v & 1) * 256 + lane * 8) = w;
+                mbar_arrive_warp(&bars[Cfg::kVFull + (v & 1)]);
+                if (++qi == n_per_head) qi = 0;
+            }
         }
       } else if (PREC == 2 && warp == kTmaWarp + 1) {
         // ---------------------------------------------------------------- warp 18: the steps' bias tiles
@@ -960,6 +1008,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         const int tile = m->tile, head_x = m->head_x, b = m->b, nk = m->nk, it0 = m->it0, n_per_head = m->n_per_head, n_iter = m->n_iter;
         [[maybe_unused]] const int sum_steps = DS ? n_per_head : 0;
         [[maybe_unused]] const int rot = FUSED ? m->rot : 0;
+        [[maybe_unused]] const int head_q0 = RULED && KS ? m->head_q0 : 0;
         if (n_iter < 0) break;
         if (XY_CONV && KS && n_iter > 0) {
             ok = convert_xy(1, (count >> 2) & 1u);
@@ -1062,7 +1111,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             const int it = g - g0;          // (query-stationary)
             const int strm_tile = (KS) ? q_tile_of(it0, n_per_head, rot, qi) : (RULED ? it0 : 0) + k_tile_of(n_per_head, it);     // query tile (0) / key tile (1)
             const int col_g0 = strm_tile * kTile + cb;                          // global index of my first column
-            const int head_q = (KS) ? head_x * a.group + hg : head_x;
+            const int head_q = (KS) ? (RULED ? head_q0 : head_x * a.group) + hg : head_x;
             const uint32_t bh = dropout_column(a.rng, b, head_q);
             [[maybe_unused]] const float* bias_h = PREC ? a.bias + b * a.bias_sb + head_q * a.bias_sh : nullptr;
             // key-stationary: -lse*log2(e) and -delta of this step's 128 queries (slot g & 1)
@@ -1135,31 +1184,26 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 #pragma unroll
                     for (int k = 0; k < 2; ++k) kwr[h][k] = w[16 * h + 8 * k];
             }
-            // rules: whether some query of the step does not see my whole key tile, and then, for my eight query columns, the
-            // tile's rows they see: first and end of columns 8j + 2lq + {0, 1}, a byte each (128: none)
-            [[maybe_unused]] bool partial = false;
-            [[maybe_unused]] uint32_t sees[4];
             [[maybe_unused]] float slope = 0.f;
-            if constexpr (RULED) {
-                const int4 hull = a.rules.q_tiles[b * a.rules.q_tiles_b + strm_tile];
+            if constexpr (RULED)
                 if (a.rules.slopes) slope = -a.rules.slopes[head_q] * kLog2e;
-                partial = hull.z > tile * kTile || hull.w < tile * kTile + kTile;
-                if (partial) {
-                    const int4* rows = reinterpret_cast<const int4*>(a.rules.rows + b * a.rules.rows_b + col_g0 + 2 * lq);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int4 x = rows[4 * j];
-                        auto in_tile = [&](int key) { return (uint32_t)min(max(key - tile * kTile, 0), kTile); };
-                        sees[j] = in_tile(x.x) | in_tile(x.y) << 8 | in_tile(x.z) << 16 | in_tile(x.w) << 24;
-                    }
-                }
-            }
             ok = mbar_wait(&bars[Cfg::kT1Full], (uint32_t)g & 1u, abort_flag);
             if (ok) ok = mbar_wait(&bars[Cfg::kVFull + (g & 1)], (uint32_t)(g >> 1) & 1u, abort_flag);
             if (PREC == 2 && ok) ok = mbar_wait(&bars[Cfg::kBiasFull], (uint32_t)g & 1u, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after_sync();
+            // rules: the tile's rows that my eight query columns see, first and end of columns 8j + 2lq + {0, 1}, a byte each
+            [[maybe_unused]] uint32_t sees[4];
+            [[maybe_unused]] bool partial = false;
+            if constexpr (RULED) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    sees[j] = *reinterpret_cast<const uint32_t*>(sSees + (g & 1) * 256 + (cb + 8 * j + 2 * lq) * 2);
+                    partial |= sees[j] != 0x80008000u;
+                }
+                partial = __any_sync(0xffffffffu, partial);
+            }
             const uint32_t t_lo = lane_off + cb, t_hi = lane_off + (16u << 16) + cb;
             // element (h, j, k, e): row rbase + 16h + 8k, column 8j + 2lq + e, register [h][4j + 2k + e]
             uint32_t pf[2][16];
@@ -1846,6 +1890,16 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 if constexpr (kCols == 32) tmem_ld_32x32(tacc, acc);
                 else                       tmem_ld_32x16(tacc, acc);
                 tmem_wait_ld();
+                if (RULED && KS && a.part) {
+                    // neighbouring lanes are neighbouring rows: 512 bytes a warp and instruction
+                    float* dst = a.part + (((int64_t)m->b * a.H + m->head_q0) * ((a.Nk + kTile - 1) / kTile) + m->tile) * (2 * kTile * D) + o * kTile * D;
+#pragma unroll
+                    for (int q = 0; q < kCols / 4; ++q)
+                        *reinterpret_cast<float4*>(dst + ((wg * (kCols / 4) + q) * kTile + r) * 4) =
+                            make_float4(__uint_as_float(acc[4 * q]) * mul, __uint_as_float(acc[4 * q + 1]) * mul, __uint_as_float(acc[4 * q + 2]) * mul,
+                                        __uint_as_float(acc[4 * q + 3]) * mul);
+                    continue;
+                }
 #pragma unroll
                 for (int q = 0; q < kCols / 8; ++q) {
                     uint4 v4;
@@ -1860,7 +1914,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             tc_fence_before_sync();                        // (the next block's first hand-off lets them be overwritten)
             fence_proxy_async_smem();
             mbar_arrive_warp(&bars[Cfg::kEpi]);
-        } else if (m->tile * kTile + r < (KS ? a.Nk : a.Nq)) {
+        } else if (m->tile * kTile + r < (KS ? a.Nk : a.Nq) && !(RULED && KS && a.part)) {
             // no query sees this key tile
             const int64_t row = m->tile * kTile + r;
             uint16_t* dst1 = (uint16_t*)a.out1 + m->b * a.o1_sb + row * a.o1_sn + m->head_x * a.o1_sh;
@@ -2040,6 +2094,28 @@ bwd_dq_convert_kernel(const float* __restrict__ acc, T* __restrict__ dq, int Nq,
     }
 }
 
+// Rules: dK and dV of a key tile, summed over the query heads of its K/V head in their order, from what the dK/dV kernel's
+// blocks of one query head each have left (BwdArgs.part).  A thread eight columns of a row; memory bounds it.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) bwd_heads_kernel(const BwdArgs a, int n_tiles) {
+    const int tile = blockIdx.x % n_tiles, hk = blockIdx.y, b = blockIdx.z, row = threadIdx.x & 127, key = tile * kTile + row;
+    const int e = (int)(blockIdx.x / n_tiles) * 2 + (int)(threadIdx.x >> 7), o = e / (D / 8), c8 = e % (D / 8);
+    if (key >= a.Nk || c8 * 8 >= a.d) return;
+    const int2 seen = a.rules.k_tiles[b * a.rules.k_tiles_b + tile];
+    const int64_t step = (int64_t)n_tiles * 2 * kTile * D;
+    const float* s = a.part + ((int64_t)b * a.H + (int64_t)hk * a.group) * step + (int64_t)(tile * 2 + o) * kTile * D + (2 * c8 * kTile + row) * 4;
+    float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+#pragma unroll 4
+    for (int h = 0; h < (seen.y > seen.x ? a.group : 0); ++h, s += step) {           // (a tile that nobody sees has left nothing)
+        const float4 x = *reinterpret_cast<const float4*>(s), y = *reinterpret_cast<const float4*>(s + kTile * 4);
+        lo.x += x.x; lo.y += x.y; lo.z += x.z; lo.w += x.w;
+        hi.x += y.x; hi.y += y.y; hi.z += y.z; hi.w += y.w;
+    }
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    T* out = o == 0 ? (T*)a.out1 + b * a.o1_sb + (int64_t)key * a.o1_sn + hk * a.o1_sh : (T*)a.out2 + b * a.o2_sb + (int64_t)key * a.o2_sn + hk * a.o2_sh;
+    *reinterpret_cast<uint4*>(out + c8 * 8) = make_uint4(pack2<BF16>(lo.x, lo.y), pack2<BF16>(lo.z, lo.w), pack2<BF16>(hi.x, hi.y), pack2<BF16>(hi.z, hi.w));
+}
+
 // INLINE: bf16 call without room for the fp16 copies (the workspace-free entry point): the main kernels
 // convert their tiles themselves.
 // the kernel instance and its shared memory for a dropout form (0 none, 1 drawn in the kernel, 2 loaded;
@@ -2053,8 +2129,9 @@ auto pick_kernel(int drop) {
     else return drop ? bwd_sm100_kernel<D, BF16, MODE, kNWG, 1, INLINE, PREC, DS> : bwd_sm100_kernel<D, BF16, MODE, kNWG, 0, INLINE, PREC, DS>;
     }
 }
-template <int D, int MODE, int PREC>
+template <int D, int MODE, int PREC, int RULES = 0>
 int pick_smem(int drop) {
+    if constexpr (RULES != 0) return BwdCfg<D, MODE, 0, PREC, RULES>::kSmemBytes;
     if constexpr (PREC == 2) return drop ? BwdCfg<D, MODE, 2, PREC>::kSmemBytes : BwdCfg<D, MODE, 0, PREC>::kSmemBytes;
     else return drop == 2 ? BwdCfg<D, MODE, 2, PREC>::kSmemBytes
                      : (drop ? BwdCfg<D, MODE, 1, PREC>::kSmemBytes : BwdCfg<D, MODE, 0, PREC>::kSmemBytes);
@@ -2134,7 +2211,9 @@ int launch(const fa_b200_params& p, const BwdWorkspace& ws, const Rules* rules =
     BwdArgs a;
     a.rules = Rules{};
     a.cap_in = a.cap_out = 0.f;
+    a.part = nullptr;
     if constexpr (RULES != 0) {
+        if (ws.part_bytes) a.part = (float*)(wsp + ws.part_off);
         a.rules = *rules;
         if (RULES == 2) { a.cap_in = (float)((double)p.scale / rules->cap); a.cap_out = rules->cap * kLog2e; }
     }
@@ -2192,7 +2271,7 @@ int launch(const fa_b200_params& p, const BwdWorkspace& ws, const Rules* rules =
     static std::mutex smem_mu;             // per (D, dtype, INLINE) instance of this function
     static uint64_t smem_done[9] = {};     // [kernel mode x dropout form] -> devices whose limit is set
     constexpr int kThreads = 128 * kNWG + kExtraThreads;
-    const dim3 grid_kv((p.Nk + kTile - 1) / kTile, p.Hkv, p.B);
+    const dim3 grid_kv((p.Nk + kTile - 1) / kTile, RULES != 0 && ws.part_bytes ? p.H : p.Hkv, p.B);
     const dim3 grid_q((p.Nq + kTile - 1) / kTile, p.H, p.B);
     if constexpr (D == 64 && PREC == 0 && RULES == 0) if (fused) {
         // one key-stationary kernel for dK, dV and the fp32 dQ sums, then the conversion of dQ
@@ -2216,7 +2295,7 @@ int launch(const fa_b200_params& p, const BwdWorkspace& ws, const Rules* rules =
     auto k0 = pick_kernel<D, BF16, 0, INLINE, PREC, false, RULES>(drop);
     auto k1 = pick_kernel<D, BF16, 1, INLINE, PREC, false, RULES>(drop);
     if constexpr (PREC != 0) if (p.d_scores) k1 = pick_kernel<D, BF16, 1, INLINE, PREC, true>(drop);
-    const int smem0 = pick_smem<D, 0, PREC>(drop), smem1 = pick_smem<D, 1, PREC>(drop);
+    const int smem0 = pick_smem<D, 0, PREC, RULES>(drop), smem1 = pick_smem<D, 1, PREC, RULES>(drop);
     FA_CUDA_CHECK(set_smem_limit_once(k0, smem0, p.device, &smem_done[drop], &smem_mu));
     FA_CUDA_CHECK(set_smem_limit_once(k1, smem1, p.device, &smem_done[(PREC && p.d_scores ? 6 : 3) + drop], &smem_mu));
     if (phases & 2) {
@@ -2249,6 +2328,11 @@ int launch(const fa_b200_params& p, const BwdWorkspace& ws, const Rules* rules =
         outputs(p.dq, p.dq);
         FA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k1, mq16, mg, mk16, mv, mdq, mdq, mdq, mb, mds, a));
     }
+    if constexpr (RULES != 0) if ((phases & 2) && a.part) {
+        outputs(p.dk, p.dv);
+        bwd_heads_kernel<T, D><<<dim3(grid_kv.x * (D / 8), p.Hkv, p.B), 256, 0, st>>>(a, (int)grid_kv.x);
+        FA_CUDA_CHECK(cudaGetLastError());
+    }
     return FA_OK;
 }
 
@@ -2259,6 +2343,18 @@ template <int RULES>
 int bwd_by_type(const fa_b200_params& p, const BwdWorkspace& ws, const Rules& rules) {
     if (p.dtype == FA_B200_BF16) return p.D > 64 ? launch<128, true, false, 0, RULES>(p, ws, &rules) : launch<64, true, false, 0, RULES>(p, ws, &rules);
     return p.D > 64 ? launch<128, false, false, 0, RULES>(p, ws, &rules) : launch<64, false, false, 0, RULES>(p, ws, &rules);
+}
+// A block of the dK/dV kernel walks its key tile's query tiles for every query head of its K/V head.  With fewer blocks than
+// SMs some do nothing and the longest walk (a causal call's first key tile: every query tile) is the kernel's time; then a
+// block takes one query head, and a further launch adds the heads up in fp32.  Causal bf16 backwards, all heads -> one, us:
+// 64 blocks (B1 N2048 H16 Hkv4 D128) 170 -> 106, 64 (B1 N2048 H8 Hkv4 D128) 122 -> 114, 8 (B1 N512 H8 Hkv2 D64) 69 -> 54;
+// with more blocks than SMs what a block costs beside its steps is paid once a head: 256 (B4 N2048 H16 Hkv4 D64) 224 -> 250,
+// 512 (B8 N1024 H32 Hkv8 D128) 384 -> 390.
+size_t sm100_rules_bwd_part_bytes(const fa_b200_params& p) {
+    const int sms = sm_count(p.device), D = p.D > 64 ? 128 : 64;
+    const int64_t nk = ((int64_t)p.Nk + kTile - 1) / kTile;
+    if (p.H == p.Hkv || (int64_t)p.B * p.Hkv * nk >= sms) return 0;
+    return (size_t)p.B * p.H * nk * 2 * kTile * D * sizeof(float);
 }
 int sm100_rules_bwd(const fa_b200_params& p, const BwdWorkspace& ws, const Rules& rules) {
     return rules.cap > 0.f ? bwd_by_type<2>(p, ws, rules) : bwd_by_type<1>(p, ws, rules);

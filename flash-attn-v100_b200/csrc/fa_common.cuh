@@ -87,6 +87,7 @@ struct BwdWorkspace {
     size_t do16_off, do16_bytes;
     size_t k16_off, k16_bytes;
     size_t dq_off, dq_bytes;
+    size_t part_off, part_bytes;     // calls with rules whose dK and dV are summed over a K/V head's query heads at the end
     size_t total;
 };
 BwdWorkspace bwd_workspace_layout(const fa_b200_params& p, int variant, bool inline_conversion = false);
@@ -180,6 +181,7 @@ bool sm100_pair_supports(const fa_b200_params& p, bool backward, const char** wh
 int sm100_rules_fwd(const fa_b200_params& p, const Rules& rules, void* ws, size_t ws_bytes);
 size_t sm100_rules_fwd_workspace_bytes(const fa_b200_params& p, int max_keys);
 int sm100_rules_bwd(const fa_b200_params& p, const BwdWorkspace& ws, const Rules& rules);
+size_t sm100_rules_bwd_part_bytes(const fa_b200_params& p);
 // fp32 forward on the tensor cores (fwd_tf32_sm100.cu): TF32 products taken three times
 int sm100_tf32_fwd(const fa_b200_params& p);
 bool sm100_tf32_fwd_supports(const fa_b200_params& p, const char** why);

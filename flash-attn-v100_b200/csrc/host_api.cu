@@ -382,7 +382,11 @@ int validate_rules(const fa_b200_params* p, const fa_b200_rules* r) {
 BwdWorkspace rules_workspace(const fa_b200_params& p) {
     fa_b200_params q = p;
     q.D = p.D > 64 ? 128 : 64;
-    return bwd_workspace_layout(q, FA_B200_VARIANT_TCGEN05_2PASS);
+    BwdWorkspace w = bwd_workspace_layout(q, FA_B200_VARIANT_TCGEN05_2PASS);
+    w.part_off = w.total;
+    w.part_bytes = sm100_rules_bwd_part_bytes(p);
+    w.total = align_up(w.total + w.part_bytes, 256);
+    return w;
 }
 // Kernel family of a call with rules.
 int choose_rules_variant(const fa_b200_params& p, bool backward, int* variant) {

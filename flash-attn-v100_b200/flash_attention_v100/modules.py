@@ -162,10 +162,10 @@ class EnhancedMultiHeadAttention(nn.Module):
         self.out_proj = nn.Linear(embed_dim, embed_dim, bias=bias)
         self.forward_count = 0
         self.score_cap = None if score_cap is None else float(score_cap)
-        # (64 bits, which a module's conversion to a floating type would round: built where it is used)
         self.rotary = None if rotary_base is None else (rotary_dim or self.head_dim, float(rotary_base))
-        self._inv_freq: Dict[torch.device, torch.Tensor] = {}
-        self.register_buffer("distance_slopes", None if distance_slopes is None else distance_slopes.detach().float(), persistent=False)
+        self.distance_slopes = None if distance_slopes is None else distance_slopes.detach().float().clone()
+        # frequencies (64 bits) and slopes (32) where they are used: as buffers a module's conversion to bf16 would round them
+        self._tables: Dict[Tuple[str, torch.device], torch.Tensor] = {}
         self.reset_parameters()
 
     def reset_parameters(self) -> None:
@@ -206,7 +206,7 @@ class EnhancedMultiHeadAttention(nn.Module):
                 raise ValueError("a rotary layer needs as many keys as queries: turn them before, with rotary_embedding")
             if positions is None and key_ranges is not None:
                 positions = key_ranges.positions
-            q, k = rotary_embedding(q, k, inv_freq=self._frequencies(q.device), positions=positions)
+            q, k = rotary_embedding(q, k, inv_freq=self._table("frequencies", q.device), positions=positions)
         elif positions is not None:
             raise ValueError("positions are for a layer with rotary_base")
         if key_ranges is not None or self.score_cap is not None or self.distance_slopes is not None:
@@ -215,7 +215,7 @@ class EnhancedMultiHeadAttention(nn.Module):
             if need_weights:
                 _warn_no_weights()
             self.forward_count += 1
-            out = flash_attention_v100_with_rules(q, k, v, causal=is_causal, score_cap=self.score_cap, distance_slopes=self.distance_slopes,
+            out = flash_attention_v100_with_rules(q, k, v, causal=is_causal, score_cap=self.score_cap, distance_slopes=self._table("slopes", q.device),
                                                   key_ranges=key_ranges, key_lengths=key_lengths,
                                                   enable_profiling=self.enable_performance_monitoring)
             return self._project(out, batch, seq_q), None
@@ -242,10 +242,13 @@ class EnhancedMultiHeadAttention(nn.Module):
         out = self.out_proj(out.reshape(batch, seq_q, self.embed_dim))
         return out if self.batch_first else out.transpose(0, 1)
 
-    def _frequencies(self, device: torch.device) -> torch.Tensor:
-        if device not in self._inv_freq:
-            self._inv_freq[device] = rotary_frequencies(self.rotary[0], self.rotary[1], device=device)[0]
-        return self._inv_freq[device]
+    def _table(self, name: str, device: torch.device) -> Optional[torch.Tensor]:
+        if name == "slopes" and self.distance_slopes is None:
+            return None
+        if (name, device) not in self._tables:
+            self._tables[name, device] = (rotary_frequencies(self.rotary[0], self.rotary[1], device=device)[0] if name == "frequencies"
+                                          else self.distance_slopes.to(device))
+        return self._tables[name, device]
 
     def get_performance_stats(self) -> Optional[Dict[str, Any]]:
         """Reference :252-256.  Only the call count is kept here; time the layer with CUDA events."""
