@@ -98,8 +98,8 @@ constexpr int kVariantPair = 16;
 // ---- key ranges (key_ranges.cu) ------------------------------------------------
 // A plan's regions, int32, one after the other, each for all batch entries:
 //   rows     [B][nq_pad]        int2  first, end of a row ((0, 0): sees nothing; so the padding rows)
-//   q_tiles  [B][nq_pad / 128]  int4  of a tile's rows: least first and largest end of those that see keys (0, 0: none),
-//                                     largest first, least end of all rows below Nq (2^31 - 1, 0 if one sees nothing)
+//   q_tiles  [B][nq_pad / 128]  int4  of a tile's rows: least first, largest end, largest first and least end of those that see
+//                                     keys (0, 0, 0, 2^31 - 1: none)
 //   q_parts  [B][nq_pad / 16]   int2  the same hull for 16 rows
 //   k_tiles  [B][nk_pad / 128]  int2  first and end of the query tiles whose hull meets the key tile ((0, 0): none)
 //   q_order, p_order, k_order         [B][nq_pad / 128], [B][pairs of them], [B][nk_pad / 128]: query tiles, pairs of them and

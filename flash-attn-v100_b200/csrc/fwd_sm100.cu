@@ -119,7 +119,8 @@ struct FwdCfg {
     static constexpr int kNumBars = kDealt ? (kClc + 2) & ~1 : kClc;      // (even: what lies behind them is 16-byte aligned)
     static constexpr int kMlBytes = SCHED == 2 ? kBlockM * 8 : 0;
     static constexpr int kWalkBytes = SCHED ? 8 * 40 : 0;  // a WalkRecord per softmax warp
-    static constexpr int kSmemBytes = (kQTiles + 2 * kStages) * kTileBytes + kBiasBytes + kNumBars * 8 + 64 + kMlBytes + kWalkBytes + 1024;
+    static constexpr int kDealBytes = kDealt ? 144 : 0;                // a Deal behind the 64 bytes of control words
+    static constexpr int kSmemBytes = (kQTiles + 2 * kStages) * kTileBytes + kBiasBytes + kNumBars * 8 + 64 + kMlBytes + kWalkBytes + kDealBytes + 1024;
     static_assert(kSmemBytes <= 232448, "shared-memory plan does not fit");
 };
 
@@ -172,6 +173,7 @@ struct FwdArgs {
 // (0: no rows); count(t): how many of them lie in this stretch.  With rules a tile's blocks begin at s[t], a pair's at jb.
 struct Stretch {
     int pair, h, b, nk, j0, j1, n[2], jb, s[2];
+    int2 seen, all[2];             // dealt pairs: keys that rows of the pair see, keys that all rows of a tile see (that see any)
     __device__ __forceinline__ int first(int t) const { return j0 > s[t] ? j0 : s[t]; }
     __device__ __forceinline__ int count(int t) const { const int f = first(t), e = n[t] < j1 ? n[t] : j1; return e > f ? e - f : 0; }
     __device__ __forceinline__ bool whole() const { return j0 == jb && j1 >= n[0] && j1 >= n[1]; }
@@ -376,9 +378,9 @@ template <> struct WorkLoop<0, 0> {       // whole pairs, round robin
 // The order: groups of columns whose K and V stay in L2, in a group the longest pair of every column first, then the second
 // (the plan's p_order).  The producer asks (Dealer) and leaves the pair's number in one of two
 // slots for the other roles (WorkLoop).  Round robin: B4 N4096 H32 D128 bf16 with 8 documents a row 317 us.
-struct Deal {                              // in shared memory, at RangeStart's place; 16-byte aligned answer
-    int w[2], pad[2];
-    uint32_t answer[4];
+struct Deal {                              // in shared memory; what a role needs of a pair comes from here, not from the plan in memory
+    uint32_t answer[4];                    // 16-byte aligned
+    int4 slot[2][4];                       // number (-1: no more), pair, head, batch | jb, n, n | s, s, seen | all, all
 };
 template <int RULES>
 __device__ __forceinline__ void dealt_stretch(const FwdArgs& a, int w, Stretch& s) {
@@ -392,6 +394,16 @@ __device__ __forceinline__ void dealt_stretch(const FwdArgs& a, int w, Stretch& 
     stretch_blocks<RULES>(a, kBlockM, s);
     s.j0 = s.jb;
     s.j1 = s.n[0] > s.n[1] ? s.n[0] : s.n[1];
+    const int2 h0 = tile_hull(a, s.b, kBlockM, s.pair, 0), h1 = tile_hull(a, s.b, kBlockM, s.pair, 1);
+    s.seen = h0.y == 0 ? h1 : (h1.y == 0 ? h0 : make_int2(min(h0.x, h1.x), max(h0.y, h1.y)));
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        s.all[t] = make_int2(0, 0x7fffffff);
+        if ((s.pair * 2 + t) * kBlockM < a.Nq) {
+            const int4 h = a.rules.q_tiles[s.b * a.rules.q_tiles_b + s.pair * 2 + t];
+            s.all[t] = make_int2(h.z, h.w);
+        }
+    }
 }
 template <int RULES> struct WorkLoop<0, RULES> {
     static constexpr int kSub = 1;
@@ -399,18 +411,25 @@ template <int RULES> struct WorkLoop<0, RULES> {
     uint64_t* bars;                        // kSchedFull[2], kSchedEmpty[2], kClc
     volatile uint32_t* abort_flag;
     bool warp;                             // a warp reads, not a thread
-    int k, w;
-    __device__ __forceinline__ WorkLoop(volatile Deal* d, uint64_t* b, volatile uint32_t* f, bool wp) : deal(d), bars(b), abort_flag(f), warp(wp), k(0), w(-1) {}
+    int k;
+    __device__ __forceinline__ WorkLoop(volatile Deal* d, uint64_t* b, volatile uint32_t* f, bool wp) : deal(d), bars(b), abort_flag(f), warp(wp), k(0) {}
     __device__ __forceinline__ bool more(const FwdArgs&) {
         bool there = mbar_wait(&bars[k & 1], (uint32_t)(k >> 1) & 1u, abort_flag);
         if (warp) there = __all_sync(0xffffffffu, there);
-        w = there ? deal->w[k & 1] : -1;
-        if (there) { if (warp) mbar_arrive_warp(&bars[2 + (k & 1)]); else mbar_arrive(&bars[2 + (k & 1)]); }
-        ++k;
-        return w >= 0;
+        return there && ((volatile int*)deal->slot[k & 1])[0] >= 0;
     }
     __device__ __forceinline__ void advance() {}
-    __device__ __forceinline__ bool get(const FwdArgs& a, int, Stretch& s) const { dealt_stretch<RULES>(a, w, s); return true; }
+    __device__ __forceinline__ bool get(const FwdArgs& a, int, Stretch& s) {
+        const volatile int* x = (const volatile int*)deal->slot[k & 1];
+        s.pair = x[1]; s.h = x[2]; s.b = x[3]; s.jb = s.j0 = x[4]; s.n[0] = x[5]; s.n[1] = x[6]; s.s[0] = x[7]; s.s[1] = x[8];
+        s.seen = make_int2(x[9], x[10]);
+        s.all[0] = make_int2(x[11], x[12]); s.all[1] = make_int2(x[13], x[14]);
+        s.j1 = s.n[0] > s.n[1] ? s.n[0] : s.n[1];
+        s.nk = a.Nk;
+        if (warp) mbar_arrive_warp(&bars[2 + (k & 1)]); else mbar_arrive(&bars[2 + (k & 1)]);
+        ++k;
+        return true;
+    }
 };
 // The producer's side of it (one thread).
 template <int RULES> struct Dealer {
@@ -419,10 +438,19 @@ template <int RULES> struct Dealer {
     uint64_t* bars;
     volatile uint32_t* abort_flag;
     int k, w, asked;
-    __device__ __forceinline__ Dealer(volatile Deal* d, uint64_t* b, volatile uint32_t* f) : deal(d), bars(b), abort_flag(f), k(0), w(blockIdx.x), asked(0) { leave(); }
-    __device__ __forceinline__ void leave() {
+    Stretch st;
+    const FwdArgs* args;
+    __device__ __forceinline__ Dealer(const FwdArgs& a, volatile Deal* d, uint64_t* b, volatile uint32_t* f)
+        : deal(d), bars(b), abort_flag(f), k(0), w(blockIdx.x), asked(0), args(&a) { leave(a); }
+    __device__ __forceinline__ void leave(const FwdArgs& a) {
+        if (w >= 0) dealt_stretch<RULES>(a, w, st);
         if (!mbar_wait(&bars[2 + (k & 1)], ((uint32_t)(k >> 1) & 1u) ^ 1u, abort_flag)) { w = -1; return; }
-        deal->w[k & 1] = w;
+        volatile int* x = (volatile int*)deal->slot[k & 1];
+        x[0] = w;
+        if (w >= 0) {
+            x[1] = st.pair; x[2] = st.h; x[3] = st.b; x[4] = st.jb; x[5] = st.n[0]; x[6] = st.n[1]; x[7] = st.s[0]; x[8] = st.s[1];
+            x[9] = st.seen.x; x[10] = st.seen.y; x[11] = st.all[0].x; x[12] = st.all[0].y; x[13] = st.all[1].x; x[14] = st.all[1].y;
+        }
         mbar_arrive(&bars[k & 1]);
     }
     __device__ __forceinline__ void ask() {
@@ -436,9 +464,9 @@ template <int RULES> struct Dealer {
         w = clc_answer_block((const uint32_t*)deal->answer, block) ? (int)block.x : -1;
         fence_proxy_async_smem();          // read before the next answer is written
         ++k;
-        leave();
+        leave(*args);
     }
-    __device__ __forceinline__ bool get(const FwdArgs& a, int, Stretch& s) const { dealt_stretch<RULES>(a, w, s); return true; }
+    __device__ __forceinline__ bool get(const FwdArgs&, int, Stretch& s) const { s = st; return true; }
     __device__ __forceinline__ void unwind() const {
         for (int spin = 0; spin < 4096 && asked > 0 && !mbar_try_wait(&bars[4], (uint32_t)(asked - 1) & 1u); ++spin) {}
     }
@@ -546,10 +574,11 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     [[maybe_unused]] float2* sMl = (float2*)((uint8_t*)(bars + Cfg::kNumBars) + 64);      // SCHED = 2: [128]
     volatile RangeStart* range = (volatile RangeStart*)(tmem_slot + 4);      // seven words of the 64 bytes behind the barriers
     constexpr bool DEALT = Cfg::kDealt;
-    static_assert(!DEALT || (Cfg::kNumBars % 2 == 0 && sizeof(Deal) <= 48), "the answer to a request is 16-byte aligned");
+    static_assert(!DEALT || (Cfg::kNumBars % 2 == 0 && sizeof(Deal) == Cfg::kDealBytes), "the answer to a request is 16-byte aligned");
+    [[maybe_unused]] volatile Deal* deal = (volatile Deal*)(tmem_slot + 16);
     // a role's walk (WorkLoop); `by_warp`: the role is a warp, not one thread
     auto walk_of = [&](bool by_warp) {
-        if constexpr (DEALT) return WorkLoop<SCHED, RULES>((volatile Deal*)(tmem_slot + 4), bars + Cfg::kSchedFull, abort_flag, by_warp);
+        if constexpr (DEALT) return WorkLoop<SCHED, RULES>(deal, bars + Cfg::kSchedFull, abort_flag, by_warp);
         else return WorkLoop<SCHED, RULES>(a, range);
     };
 
@@ -594,7 +623,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             bool ok = true;
             const uint32_t q_bytes = FREE ? (uint32_t)(Cfg::kNBox * 128 * pack * q_per_tile) : TILE;
             auto dealer = [&] {
-                if constexpr (DEALT) return Dealer<RULES>((volatile Deal*)(tmem_slot + 4), bars + Cfg::kSchedFull, abort_flag);
+                if constexpr (DEALT) return Dealer<RULES>(a, deal, bars + Cfg::kSchedFull, abort_flag);
                 else return WorkLoop<SCHED, RULES>(a, range);
             };
             auto wl = dealer();
@@ -835,7 +864,8 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 Stretch st;
                 if (!wl.get(a, u, st)) continue;
                 int2 seen = make_int2(0, 0);                // keys that rows of the pair see
-                if constexpr (RULED) {
+                if constexpr (DEALT) seen = st.seen;
+                else if constexpr (RULED) {
                     const int2 h0 = tile_hull(a, st.b, q_per_tile, st.pair, 0), h1 = tile_hull(a, st.b, q_per_tile, st.pair, 1);
                     seen = h0.y == 0 ? h1 : (h1.y == 0 ? h0 : make_int2(min(h0.x, h1.x), max(h0.y, h1.y)));
                 }
@@ -909,7 +939,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 
         if (FREE && threadIdx.x == 0) a.part_meta[blockIdx.x] = make_int4(0, 0, 0, 0);
         auto my_walk = [&] {
-            if constexpr (DEALT) return SoftmaxLoop<SCHED, RULES>((volatile Deal*)(tmem_slot + 4), bars + Cfg::kSchedFull, abort_flag, true);
+            if constexpr (DEALT) return SoftmaxLoop<SCHED, RULES>(deal, bars + Cfg::kSchedFull, abort_flag, true);
             else return SoftmaxLoop<SCHED, RULES>(a, range, walk);
         };
         for (auto wl = my_walk(); wl.more(a) && ok; wl.advance()) {
@@ -959,9 +989,14 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         if (a.rules.slopes) slope = a.rules.slopes[h] * kLog2e;
                     }
                     at = i + a.rules.origin[st.b * a.rules.origin_b];
-                    all_from = __reduce_max_sync(0xffffffffu, keys.x);
-                    all_to = __reduce_min_sync(0xffffffffu, keys.y);
-                    ahead = __any_sync(0xffffffffu, row_ok() && !dead && at < keys.y - 1);
+                    if constexpr (DEALT) {
+                        all_from = st.all[t].x;            // (nothing waits for the row's own range before a block has to be masked)
+                        all_to = st.all[t].y;
+                    } else {
+                        all_from = __reduce_max_sync(0xffffffffu, keys.x);
+                        all_to = __reduce_min_sync(0xffffffffu, keys.y);
+                    }
+                    if (a.rules.slopes) ahead = __any_sync(0xffffffffu, row_ok() && !dead && at < keys.y - 1);
                 }
                 // my row of the bias (a row beyond Nq, whose results nobody keeps, reads the last one)
                 const float* brow = nullptr;
@@ -1108,11 +1143,17 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                                 }
                             }
                         }
-                        if (col0 < all_from || col0 + kBlockN > all_to) {
-                            const int lo = keys.x - col0, hi = keys.y - col0;         // the columns my row sees
+                        if (col0 < all_from) {                     // (a block on one of a range's ends is seldom on the other)
+                            const int lo = keys.x - col0;
 #pragma unroll
                             for (int c = 0; c < 128; ++c)
-                                if (c < lo || c >= hi) SSET(c, -INFINITY);
+                                if (c < lo) SSET(c, -INFINITY);
+                        }
+                        if (col0 + kBlockN > all_to) {
+                            const int hi = keys.y - col0;
+#pragma unroll
+                            for (int c = 0; c < 128; ++c)
+                                if (c >= hi) SSET(c, -INFINITY);
                         }
                     }
                     const bool need_mask = !RULED && ((a.causal && col0 + kBlockN - 1 > tile * q_per_tile + a.shift) || (col0 + kBlockN > nk));

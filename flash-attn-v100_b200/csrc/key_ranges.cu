@@ -87,8 +87,8 @@ __global__ void __launch_bounds__(128) key_rows_kernel(const RangesArgs a) {
     int4 h;                                        // least first, largest end; largest first, least end
     h.x = sees ? r.x : INT_MAX;
     h.y = sees ? r.y : 0;
-    h.z = i < a.Nq ? (sees ? r.x : INT_MAX) : 0;
-    h.w = i < a.Nq ? (sees ? r.y : 0) : INT_MAX;
+    h.z = sees ? r.x : 0;
+    h.w = sees ? r.y : INT_MAX;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
         h.x = min(h.x, __shfl_xor_sync(0xffffffffu, h.x, off));

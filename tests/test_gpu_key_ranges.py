@@ -61,12 +61,9 @@ def check(r, Nq, Nk, batch, host):
                 want_hull = [int(seen.min()), int(seen.max()) + 1] if len(seen) else [0, 0]
                 assert got_hull[n].tolist() == want_hull, (b, rows, n)
         for n in range(nq):
-            rows = want[n * 128:(n + 1) * 128]
-            f, e = first[b][n * 128:(n + 1) * 128], end[b][n * 128:(n + 1) * 128]
-            if rows.any(dim=1).all():
-                assert tiles[n, 2:].tolist() == [int(f.max()), int(e.min())]
-            else:
-                assert tiles[n, 2:].tolist() == [2 ** 31 - 1, 0]
+            some = want[n * 128:(n + 1) * 128].any(dim=1)
+            f, e = first[b][n * 128:(n + 1) * 128][some], end[b][n * 128:(n + 1) * 128][some]
+            assert tiles[n, 2:].tolist() == ([int(f.max()), int(e.min())] if some.any() else [0, 2 ** 31 - 1])
         for n in range(nk):
             meets = ((tiles[:, 0] < n * 128 + 128) & (tiles[:, 1] > n * 128)).nonzero()
             assert keys[n].tolist() == ([int(meets.min()), int(meets.max()) + 1] if len(meets) else [0, 0]), (b, n)
