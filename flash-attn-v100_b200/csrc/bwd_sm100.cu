@@ -408,6 +408,9 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     constexpr bool P_BF16 = BF16 && PREC != 0;  // ... except that pairs of bf16 need no conversion
     static_assert(PREC == 0 || (MODE != 2 && !INLINE), "the pair instances are the two-pass form");
     constexpr bool RULED = RULES != 0, ANY_D = PREC != 0 || RULED;
+    // dS as hi + lo fp16 where the results are fp16: rounded once, dS was half of the error of dQ and dK (3.2e-4 against the 2.1e-4
+    // of their own rounding); bf16 results do not show it.
+    constexpr bool DS_PAIR = RULED && !BF16;
     static_assert(!RULED || (PREC == 0 && DROP == 0 && MODE != 2 && !INLINE && !DS), "rules come without bias and dropout, in two passes");
     constexpr bool STREAM_CONV = CONV && INLINE;             // ... the streamed ones by warps 18 and 19
     constexpr bool XY_CONV = CONV && (KS || INLINE);         // ... the stationary ones (X; key-stationary also Y), too
@@ -673,7 +676,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             // every warpgroup's slice: K-steps kk = hf, hf + 2, hf + 4, hf + 6.  A holds 16-bit pairs: the group
             // that owns columns [g*CPT, (g+1)*CPT) of T wrote its CPT values packed into columns
             // [g*CPT, g*CPT + CPT/2); with pairs their low parts follow in [g*CPT + CPT/2, (g+1)*CPT).
-            auto issue_acc_half = [&](uint32_t d_tmem, uint32_t a_tmem, uint32_t strm_u, bool acc, int hf) {
+            auto issue_acc_half = [&](uint32_t d_tmem, uint32_t a_tmem, uint32_t strm_u, bool acc, int hf, bool pair = PREC != 0) {
                 static_assert(CPT == 32, "one K-step of 16 per half slice");
                 const uint64_t b0 = dmn_major + (uint64_t)(strm_u >> 4);
 #pragma unroll
@@ -682,7 +685,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                     const uint32_t a_col = (uint32_t)q * CPT + (uint32_t)hf * 8u;
                     mma_ts_f16(d_tmem, a_tmem + a_col, b0 + (uint64_t)((kk * 2048) >> 4), idesc_acc,
                                (acc || hf > 0 || q > 0) ? 1u : 0u);
-                    if (PREC) mma_ts_f16(d_tmem, a_tmem + a_col + CPT / 2, b0 + (uint64_t)((kk * 2048) >> 4), idesc_acc, 1u);
+                    if (pair) mma_ts_f16(d_tmem, a_tmem + a_col + CPT / 2, b0 + (uint64_t)((kk * 2048) >> 4), idesc_acc, 1u);
                 }
             };
 
@@ -787,11 +790,11 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                     if (!ok) break;
                     tc_fence_after_sync();
                     const bool acc = !DS || it >= sum_steps;                       // (no dS in the steps that only sum)
-                    if (acc) issue_acc_half(tAcc1, tDs, cur_u, it > sum_steps, 0);   // dK += dS^T Q  /  dQ += dS K
+                    if (acc) issue_acc_half(tAcc1, tDs, cur_u, it > sum_steps, 0, PREC != 0 || DS_PAIR);   // dK += dS^T Q  /  dQ += dS K
                     ok = mbar_wait(&bars[b_ready], ds_par, abort_flag);
                     if (!ok) break;
                     tc_fence_after_sync();
-                    if (acc) issue_acc_half(tAcc1, tDs, cur_u, it > sum_steps, 1);
+                    if (acc) issue_acc_half(tAcc1, tDs, cur_u, it > sum_steps, 1, PREC != 0 || DS_PAIR);
                     // last reader of U(it); a block's last U and W tiles' places take its results first
                     mma_commit(&bars[more ? Cfg::kUEmpty + us : Cfg::kAccDone]);
                     if (FUSED) {
@@ -1446,8 +1449,8 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                                     if (col < lim) d0 = 0.f;
                                     if (col + 1 < lim) d1 = 0.f;
                                 }
-                                if (PREC) pack2_pair<P_BF16>(d0, d1, pk[h][2 * jj + k], pl[h][2 * jj + k]);
-                                else      pk[h][2 * jj + k] = pack2<false>(d0, d1);
+                                if (PREC || DS_PAIR) pack2_pair<P_BF16>(d0, d1, pk[h][2 * jj + k], pl[h][2 * jj + k]);
+                                else                 pk[h][2 * jj + k] = pack2<false>(d0, d1);
                             }
                     }
                     if (drop && hf == 1) {
@@ -1457,7 +1460,7 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                     }
                     tmem_st_16x128b_x2(tT2 + t_lo + hf * 8, pk[0]);
                     tmem_st_16x128b_x2(tT2 + t_hi + hf * 8, pk[1]);
-                    if (PREC) {
+                    if (PREC || DS_PAIR) {
                         tmem_st_16x128b_x2(tT2 + t_lo + 16 + hf * 8, pl[0]);
                         tmem_st_16x128b_x2(tT2 + t_hi + 16 + hf * 8, pl[1]);
                     }
@@ -1796,13 +1799,17 @@ bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                                         if (col_g0 + c + 3 < a.Nk) dst[3] = d3 * ds_mul;
                                     }
                                 }
+                            } else if constexpr (DS_PAIR) {
+                                const int e = (c4 - hf * (CPT / 8)) * 2;
+                                pack2_pair<false>(d0, d1, pk[e], pl[e]);
+                                pack2_pair<false>(d2v, d3, pk[e + 1], pl[e + 1]);
                             } else {
                                 pk[(c4 - hf * (CPT / 8)) * 2 + 0] = pack2<false>(d0, d1);
                                 pk[(c4 - hf * (CPT / 8)) * 2 + 1] = pack2<false>(d2v, d3);
                             }
                         }
                         tmem_st_32x8(tD + lane_off + cb + hf * (CPT / 4), pk);
-                        if (PREC) tmem_st_32x8(tD + lane_off + cb + CPT / 2 + hf * (CPT / 4), pl);
+                        if (PREC || DS_PAIR) tmem_st_32x8(tD + lane_off + cb + CPT / 2 + hf * (CPT / 4), pl);
                         if (FUSED) {
                             // the same dS^T values as a shared-memory tile [key row][query], 64-query boxes with
                             // the 128-byte swizzle: the A operand (MN-major) of the dQ MMA.  The previous

@@ -59,6 +59,17 @@ __device__ __forceinline__ RowRule row_rule(const Rules& u, int b, int i, int Nq
     }
     return r;
 }
+// Keys that rows of a 64-row query tile see ((0, 0): none).
+__device__ __forceinline__ int2 hull_of(const Rules& u, int b, int tile) {
+    const int2* parts = u.q_parts + b * u.q_parts_b + tile * (BM / 16);
+    int2 r = make_int2(0x7fffffff, 0);
+#pragma unroll
+    for (int e = 0; e < BM / 16; ++e) {
+        const int2 h = parts[e];
+        if (h.y > 0) { r.x = min(r.x, h.x); r.y = max(r.y, h.y); }
+    }
+    return r.y > 0 ? r : make_int2(0, 0);
+}
 // x of a score s = scale q.k, and the derivative of x by s
 __device__ __forceinline__ float ruled_score(const Rules& u, float slope, float s, int position, int key, float& dx) {
     dx = 1.f;
@@ -121,8 +132,8 @@ __global__ void __launch_bounds__(NT) simt_fwd_kernel(SimtArgs a) {
     float slope = 0.f;
     RowRule rule[4];
     if (RULES) {
-        const int4 hull = a.rules.q_tiles[b * a.rules.q_tiles_b + m0 / 128];
-        from = hull.x; to = kv_end = hull.y;
+        const int2 hull = hull_of(a.rules, b, mt);
+        from = max(hull.x, 0); to = kv_end = min(hull.y, a.Nk);
         if (a.rules.slopes) slope = a.rules.slopes[h];
 #pragma unroll
         for (int r = 0; r < 4; ++r) rule[r] = row_rule(a.rules, b, m0 + ty * 4 + r, a.Nq);
@@ -328,7 +339,7 @@ __global__ void __launch_bounds__(NT) simt_bwd_kernel(SimtArgs a) {
             it_end = (a.Nq + BM - 1) / BM;
             if (RULES) {
                 const int2 seen = a.rules.k_tiles[b * a.rules.k_tiles_b + tile * BN / 128];
-                it_begin = seen.x * (128 / BM);
+                it_begin = max(seen.x, 0) * (128 / BM);
                 it_end = min(it_end, seen.y * (128 / BM));
             }
         } else {
@@ -336,9 +347,9 @@ __global__ void __launch_bounds__(NT) simt_bwd_kernel(SimtArgs a) {
             if (a.causal && tile * BM + BM + a.shift < kv_end) kv_end = tile * BM + BM + a.shift;
             it_begin = 0;
             if (RULES) {
-                const int4 hull = a.rules.q_tiles[b * a.rules.q_tiles_b + tile * BM / 128];
-                it_begin = hull.x / BN;
-                kv_end = hull.y;
+                const int2 hull = hull_of(a.rules, b, tile);
+                it_begin = max(hull.x, 0) / BN;
+                kv_end = min(hull.y, a.Nk);
             }
             it_end = (kv_end + BN - 1) / BN;
         }
@@ -357,6 +368,10 @@ __global__ void __launch_bounds__(NT) simt_bwd_kernel(SimtArgs a) {
         for (int it = it_begin; it < it_end; ++it) {
             const int m0 = (MODE == 0) ? it * BM : tile * BM;
             const int n0 = (MODE == 0) ? tile * BN : it * BN;
+            if (RULES && MODE == 0) {              // (the list holds all tiles between the first and the last that meet this one's 128 keys)
+                const int2 hull = hull_of(a.rules, b, it);
+                if (hull.x >= n0 + BN || hull.y <= n0) continue;
+            }
             __syncthreads();
             if (MODE == 0) {
                 load_tile<T>(Qs, ld, qb, a.q.stride_n, m0, a.Nq, D, BM);
