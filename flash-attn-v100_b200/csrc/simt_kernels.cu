@@ -47,7 +47,8 @@ struct SimtArgs {
     Rules rules;         // RULES instances only
 };
 
-// RULES instances: scores bent by a cap, moved by a distance, hidden outside a row's range (fa_b200_rules).  Rows of K and V
+// RULES instances (DC: the head size, known when compiling, where fp32 calls mostly have it: B2 N500 H4 D64, five documents, forward
+// and backward 79 + 249 -> 61 + 157 us; 0: any): scores bent by a cap, moved by a distance, hidden outside a row's range (fa_b200_rules).  Rows of K and V
 // outside the hull of the query tile's ranges are read as zeros, so that memory nobody sees may hold anything.
 struct RowRule { int first, end, position; };
 __device__ __forceinline__ RowRule row_rule(const Rules& u, int b, int i, int Nq) {
@@ -91,10 +92,10 @@ __device__ __forceinline__ void load_tile(float* dst, int ld, const T* base, int
     }
 }
 
-template <typename T, bool RULES>
+template <typename T, bool RULES, int DC = 0>
 __global__ void __launch_bounds__(NT) simt_fwd_kernel(SimtArgs a) {
     extern __shared__ float smem[];
-    const int D = a.D, ld = D + 1;
+    const int D = DC ? DC : a.D, ld = D + 1;
     float* Qs = smem;
     float* Ks = Qs + BM * ld;
     float* Vs = Ks + BN * ld;
@@ -286,10 +287,10 @@ __global__ void __launch_bounds__(256) simt_delta_kernel(SimtArgs a) {
 }
 
 // MODE 0: key-stationary, writes dK and dV.  MODE 1: query-stationary, writes dQ.
-template <typename T, int MODE, bool RULES>
+template <typename T, int MODE, bool RULES, int DC = 0>
 __global__ void __launch_bounds__(NT) simt_bwd_kernel(SimtArgs a) {
     extern __shared__ float smem[];
-    const int D = a.D, ld = D + 1;
+    const int D = DC ? DC : a.D, ld = D + 1;
     float* Qs = smem;
     float* Gs = Qs + BM * ld;    // dO tile
     float* Ks = Gs + BM * ld;
@@ -635,10 +636,12 @@ template <typename T, bool RULES>
 int launch_fwd(const fa_b200_params& p, const Rules* rules) {
     SimtArgs a = make_args(p, nullptr, rules);
     size_t smem = ((size_t)(BM + 2 * BN) * (p.D + 1) + (size_t)BM * SLD + 3 * BM) * sizeof(float);
-    int rc = set_smem(simt_fwd_kernel<T, RULES>, smem);
+    auto kernel = simt_fwd_kernel<T, RULES>;
+    if constexpr (RULES) kernel = p.D == 64 ? simt_fwd_kernel<T, true, 64> : (p.D == 32 ? simt_fwd_kernel<T, true, 32> : kernel);
+    int rc = set_smem(kernel, smem);
     if (rc) return rc;
     dim3 grid((p.Nq + BM - 1) / BM, p.H, p.B);
-    simt_fwd_kernel<T, RULES><<<grid, NT, smem, (cudaStream_t)p.stream>>>(a);
+    kernel<<<grid, NT, smem, (cudaStream_t)p.stream>>>(a);
     FA_CUDA_CHECK(cudaGetLastError());
     return FA_OK;
 }
@@ -655,18 +658,23 @@ int launch_bwd(const fa_b200_params& p, const BwdWorkspace& ws, const Rules* rul
         FA_CUDA_CHECK(cudaGetLastError());
     }
     size_t smem = ((size_t)(2 * BM + 2 * BN) * (p.D + 1) + (size_t)2 * BM * SLD + 2 * BM) * sizeof(float);
-    int rc = set_smem(simt_bwd_kernel<T, 0, RULES>, smem);
+    auto k0 = simt_bwd_kernel<T, 0, RULES>, k1 = simt_bwd_kernel<T, 1, RULES>;
+    if constexpr (RULES) {
+        if (p.D == 64) { k0 = simt_bwd_kernel<T, 0, true, 64>; k1 = simt_bwd_kernel<T, 1, true, 64>; }
+        if (p.D == 32) { k0 = simt_bwd_kernel<T, 0, true, 32>; k1 = simt_bwd_kernel<T, 1, true, 32>; }
+    }
+    int rc = set_smem(k0, smem);
     if (rc) return rc;
-    rc = set_smem(simt_bwd_kernel<T, 1, RULES>, smem);
+    rc = set_smem(k1, smem);
     if (rc) return rc;
     if (phases & 2) {
         dim3 grid_kv((p.Nk + BN - 1) / BN, p.Hkv, p.B);
-        simt_bwd_kernel<T, 0, RULES><<<grid_kv, NT, smem, st>>>(a);
+        k0<<<grid_kv, NT, smem, st>>>(a);
         FA_CUDA_CHECK(cudaGetLastError());
     }
     if (phases & 4) {
         dim3 grid_q((p.Nq + BM - 1) / BM, p.H, p.B);
-        simt_bwd_kernel<T, 1, RULES><<<grid_q, NT, smem, st>>>(a);
+        k1<<<grid_q, NT, smem, st>>>(a);
         FA_CUDA_CHECK(cudaGetLastError());
     }
     return FA_OK;
