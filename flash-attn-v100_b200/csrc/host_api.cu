@@ -8,6 +8,7 @@
 #include "fa_common.cuh"
 #include "sm100_ptx.cuh"
 #include "tile_config.cuh"
+#include <math.h>
 #include <stdarg.h>
 #include <string.h>
 #include <mutex>
@@ -370,7 +371,7 @@ int validate_rules(const fa_b200_params* p, const fa_b200_rules* r) {
         return FA_EINVAL;
     }
     if (!(r->score_cap >= 0.f) || r->score_cap > 1e30f) { set_error("score_cap must be 0 or positive and finite"); return FA_EINVAL; }
-    if (r->score_cap > 0.f && !(p->scale * p->scale < 1e30f * r->score_cap)) { set_error("scale is too large for the cap"); return FA_EINVAL; }
+    if (r->score_cap > 0.f && !(fabs((double)p->scale) <= 1e30 * (double)r->score_cap)) { set_error("scale is too large for the cap"); return FA_EINVAL; }
     if (p->B > 0 && p->Nq > 0) {
         if (r->plan_batch != 1 && r->plan_batch != p->B) { set_error("the plan is for a batch of %d, the call has %d", r->plan_batch, p->B); return FA_EINVAL; }
         if (!r->plan) { set_error("the plan is null"); return FA_EINVAL; }

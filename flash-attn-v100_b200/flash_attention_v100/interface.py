@@ -481,8 +481,8 @@ def flash_attention_v100_with_rules(
         causal, key_lengths, causal_alignment: without key_ranges, as flash_attention_v100's (counts below 1 hide all keys
             of an entry); ranges for them are built by the call.  position_i is i, with the bottom-right alignment i + Nk - Nq
 
-    Keys and values behind an entry's counts (or outside every range) may be unwritten memory in a call without gradients; in
-    a training step they have to be numbers.  Gradients are bit-reproducible.  One GPU: that of the tensors.
+    Keys and values before the first and behind the last key that an entry's queries see may be unwritten memory in a call
+    without gradients; those between, and all in a training step, have to be numbers.  Gradients are bit-reproducible.  One GPU: that of the tensors.
     """
     manager = get_flash_attention_manager()
     profile = manager.enable_profiling or enable_profiling

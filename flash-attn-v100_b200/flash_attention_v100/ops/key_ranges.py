@@ -67,7 +67,7 @@ def _lengths(name: str, t: Optional[torch.Tensor], shapes, device: torch.device)
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected one of {shapes}")
     t = t.detach()
     if t.dtype != torch.int32:
-        t = t.to(torch.int32)
+        t = t.clamp(-_INT32_MAX, _INT32_MAX).to(torch.int32)         # (a length beyond 32 bits means all there is)
     return t if t.is_contiguous() else t.contiguous()
 
 

@@ -177,6 +177,8 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, inv_f
         for x in xs:
             if x.numel() and (x.stride(3) != 1 or any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape))):
                 raise ValueError("inplace=True needs tensors with a contiguous head dimension and rows of their own")
+        if k is not None and q.numel() and k.numel() and q.data_ptr() == k.data_ptr():
+            raise ValueError("inplace=True needs q and k that do not share memory")
         ys = xs
         if not all(x.numel() == 0 for x in xs):
             _launch(xs, ys, positions, offset, inv_freq, interleaved, float(attention_factor), False)

@@ -362,8 +362,8 @@ int fa_b200_key_ranges(const fa_b200_ranges_params* p);
  * with softmax, output, lse and gradients of x.  A row that sees nothing has an output of zeros, an lse of -inf and no
  * gradient.  Positions are those of the plan's query offsets.  In fa_b200_params causal, causal_shift, bias, kv_lengths,
  * d_scores, dropout_p and the rng_* fields have to be zero; the plan says what they would.
- * Keys and values that no row of a call's batch entry sees may hold anything in a forward (an unwritten cache); in a
- * backward, and where other rows see them, they have to be numbers.
+ * Keys and values before the first and behind the last key that rows of a call's batch entry see may hold anything in a
+ * forward (an unwritten cache); those between, and all in a backward, have to be numbers.
  * No counterpart in the reference.
  */
 typedef struct fa_b200_rules {

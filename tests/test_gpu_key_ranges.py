@@ -146,3 +146,27 @@ def test_on_another_stream(device):
         r = fa.build_key_ranges(200, 200, causal=True, key_lengths=lengths)
     side.synchronize()
     check(r, 200, 200, 1, dict(causal=True, lengths=[77]))
+
+
+def test_lengths_beyond_32_bits_mean_all(device):
+    r = fa.build_key_ranges(3, 50, key_lengths=torch.tensor([2 ** 40], device=device))
+    assert r.end.tolist() == [[50, 50, 50]]
+    r = fa.build_key_ranges(2, 50, rows=torch.tensor([[[3, 2 ** 33], [-2 ** 33, 7]]], device=device))
+    assert r.first.tolist() == [[3, 0]] and r.end.tolist() == [[50, 7]]
+
+
+def test_more_tiles_than_are_put_in_order(device):
+    """Beyond 512 tiles the lists come from another launch and the orders are the tiles' own."""
+    N, w = 66000, 700
+    r = fa.build_key_ranges(N, N, causal=True, window=w, device=device)
+    t = torch.arange(N)
+    assert torch.equal(r.first[0].cpu(), (t - w + 1).clamp(min=0).int()) and torch.equal(r.end[0].cpu(), (t + 1).int())
+    n = -(-N // 128)
+    plan = r.plan.cpu()
+    keys = plan[n * 276:][:2 * n].view(n, 2)
+    first = torch.arange(n)
+    last = ((first * 128 + 127 + w - 1).clamp(max=N - 1)) // 128
+    assert torch.equal(keys, torch.stack([first, last + 1], dim=1).int())
+    at = n * 278
+    assert sorted(plan[at:at + n].tolist()) == list(range(n)) and sorted(plan[at + n:at + n + (n + 1) // 2].tolist()) == list(range((n + 1) // 2))
+    assert sorted(plan[at + n + (n + 1) // 2:at + 2 * n + (n + 1) // 2].tolist()) == list(range(n))

@@ -115,6 +115,7 @@ def test_refusals(device):
         ("int32 or int64", lambda: fa.rotary_embedding(x, inv_freq=f, positions=torch.zeros(4, device=device))),
         ("without gradients", lambda: fa.rotary_embedding(x.clone().requires_grad_(True), inv_freq=f, inplace=True)),
         ("rows of their own", lambda: fa.rotary_embedding(x[:, :1].expand(1, 4, 2, 64), inv_freq=f, inplace=True)),
+        ("share memory", lambda: fa.rotary_embedding(x, x, inv_freq=f, inplace=True)),
         ("Unsupported dtype", lambda: fa.rotary_embedding(x.double(), inv_freq=f)),
     ]:
         with pytest.raises(ValueError, match=match):

@@ -355,3 +355,104 @@ def test_gradient_of_a_gradient_is_refused(device):
     d, = torch.autograd.grad(o.float().square().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(d.sum(), q)
+
+
+def test_a_long_window_of_many_tiles(device):
+    """More tiles than the plan puts in order: every row against its own few keys, in 64 bits."""
+    N, w, D = 66000, 200, 64
+    q, k, v, g = _inputs(1, N, N, 1, 1, D, torch.bfloat16, device)
+    r = fa.build_key_ranges(N, N, causal=True, window=w, device=device)
+    o, lse, dq, dk, dv = _step(q, k, v, g, score_cap=6.0, key_ranges=r)
+    pad = lambda t: torch.nn.functional.pad(t[0, :, 0].double(), (0, 0, w - 1, 0)).unfold(0, w, 1)      # (N, D, w): a row's keys
+    for rows in (slice(0, 3000), slice(30000, 33000), slice(63000, 66000)):
+        x = torch.einsum("nd,ndw->nw", q[0, rows, 0].detach().double(), pad(k.detach())[rows]) * D ** -0.5
+        t = torch.tanh(x / 6.0)
+        at = torch.arange(N, device=device)[rows]
+        x = (6.0 * t).masked_fill(at.view(-1, 1) - (w - 1) + torch.arange(w, device=device) < 0, float("-inf"))
+        p = torch.softmax(x, dim=1)
+        vw, go = pad(v.detach())[rows], g[0, rows, 0].double()
+        want = torch.einsum("nw,ndw->nd", p, vw)
+        dp = torch.einsum("nd,ndw->nw", go, vw)
+        ds = p * (dp - (p * dp).sum(dim=1, keepdim=True)) * (1 - t * t) * D ** -0.5
+        assert rel(o[0, rows, 0], want) <= TOLERANCE[torch.bfloat16] and rel(lse[0, 0, rows], torch.logsumexp(x, dim=1)) <= TOLERANCE[torch.bfloat16]
+        assert rel(dq[0, rows, 0], torch.einsum("nw,ndw->nd", ds, pad(k.detach())[rows])) <= TOLERANCE[torch.bfloat16]
+        # a key's gradients come from the rows behind it: those whose rows all lie in the slice
+        n = rows.stop - rows.start - w + 1
+        i = torch.arange(n, device=device).view(-1, 1) + torch.arange(w, device=device)                 # rows that see key n
+        j = w - 1 - torch.arange(w, device=device)                                                      # ... at this place of theirs
+        assert rel(dv[0, rows.start:rows.start + n, 0], torch.einsum("nw,nwd->nd", p[i, j], go[i])) <= TOLERANCE[torch.bfloat16]
+        assert rel(dk[0, rows.start:rows.start + n, 0], torch.einsum("nw,nwd->nd", ds[i, j], q[0, rows, 0].detach().double()[i])) <= TOLERANCE[torch.bfloat16]
+
+
+@pytest.mark.parametrize("dtype,H,Hkv,D", [("bf16", 4, 2, 64), ("fp16", 2, 2, 128), ("fp32", 2, 1, 64)])
+def test_a_training_step_in_a_graph(device, dtype, H, Hkv, D):
+    """Ranges, rotary, attention and all gradients, captured once, replayed on new documents and new inputs."""
+    t = TYPES[dtype]
+    N = 260
+    q, k, v, g = (x.requires_grad_(n < 3) for n, x in enumerate(_inputs(1, N, N, H, Hkv, D, t, device)))
+    f = fa.rotary_frequencies(D, device=device)[0]
+    offsets = torch.tensor([0, 100, N], dtype=torch.int32, device=device)
+
+    def step(r=None):
+        r = fa.build_key_ranges(N, N, causal=True, document_offsets=offsets, out=r)
+        qr, kr = fa.rotary_embedding(q, k, inv_freq=f, positions=r.positions)
+        o = fa.flash_attention_v100_with_rules(qr, kr, v, score_cap=12.0, key_ranges=r)
+        return r, (o,) + torch.autograd.grad(o, (q, k, v), g)
+
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(side):
+        r, _ = step()
+    torch.cuda.current_stream(device).wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, got = step(r)
+    for seed, cuts in ((3, [0, 30, 200]), (4, [0, 259, 260])):
+        with torch.no_grad():
+            for x, y in zip((q, k, v, g), _inputs(1, N, N, H, Hkv, D, t, device, seed=seed)):
+                x.copy_(y)
+        offsets.copy_(torch.tensor(cuts, dtype=torch.int32))
+        graph.replay()
+        _, want = step()
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+
+
+def test_two_streams_at_once(device):
+    """Calls on two streams share nothing: a split forward and a backward beside each other, many times."""
+    q, k, v, g = _inputs(2, 300, 300, 4, 2, 64, torch.bfloat16, device)
+    r, _, _ = _ranges(300, 300, 2, dict(causal=True, offsets=[[0, 90, 300], [0, 1, 250]]), device)
+    q1, k1, v1, _ = _inputs(3, 1, 1200, 8, 2, 128, torch.float16, device)
+    r1, _, _ = _ranges(1, 1200, 3, dict(lengths=[1200, 7, 600]), device)
+    decode = lambda: fa.flash_attention_v100_with_rules(q1, k1, v1, score_cap=5.0, key_ranges=r1)
+    train = lambda: _step(q, k, v, g, score_cap=5.0, key_ranges=r)
+    want = (decode(),) + train()
+    a, b = torch.cuda.Stream(device), torch.cuda.Stream(device)
+    for s in (a, b):
+        s.wait_stream(torch.cuda.current_stream(device))
+    outs = []
+    for _ in range(10):
+        with torch.cuda.stream(a):
+            x = decode()
+        with torch.cuda.stream(b):
+            y = train()
+        outs.append((x,) + y)
+    torch.cuda.synchronize()
+    for got in outs:
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("Nq,H,Hkv", [(1, 48, 1), (1, 17, 1), (3, 40, 2), (16, 1, 1), (17, 1, 1), (2, 8, 1), (9, 2, 1), (200, 12, 1)])
+def test_groups_of_any_size(device, Nq, H, Hkv):
+    """Rows of a K/V head on either side of what a decoding block takes (16), groups that do not divide a tile."""
+    lengths = [700, 130]
+    host = dict(causal=True, lengths=lengths, starts=[max(n - Nq, 0) for n in lengths])
+    for dtype, D in ((torch.bfloat16, 128), (torch.float16, 72)):
+        q, k, v, _ = _inputs(2, Nq, 700, H, Hkv, D, dtype, device, std=2.0)
+        r, see, at = _ranges(Nq, 700, 2, host, device)
+        want = attention64(q, k, v, see, at, D ** -0.5, 10.0, _slopes(H, device))
+        with torch.no_grad():
+            got = fa.flash_attention_v100_with_rules(q, k, v, score_cap=10.0, distance_slopes=_slopes(H, device), key_ranges=r, return_softmax_lse=True)
+        _check(got, want, dtype, ("o", "lse"))

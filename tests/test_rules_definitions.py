@@ -121,7 +121,7 @@ def test_masks_of_a_call_with_rules_are_the_plans(field, value):
     (dict(struct_bytes=8), _cabi.FA_EINVAL, b"struct_bytes"), (dict(plan=None), _cabi.FA_EINVAL, b"null"),
     (dict(plan=8), _cabi.FA_EALIGN, b"aligned"), (dict(plan_batch=3), _cabi.FA_EINVAL, b"batch"),
     (dict(score_cap=-1.0), _cabi.FA_EINVAL, b"score_cap"), (dict(score_cap=float("nan")), _cabi.FA_EINVAL, b"score_cap"),
-    (dict(score_cap=float("inf")), _cabi.FA_EINVAL, b"score_cap")])
+    (dict(score_cap=float("inf")), _cabi.FA_EINVAL, b"score_cap"), (dict(score_cap=1e-40), _cabi.FA_EINVAL, b"too large")])
 def test_bad_rules_are_refused_before_any_cuda_call(rule, code, word):
     lib, p = _cabi.load(), _params()
     r = _cabi.RuleParams(ctypes.sizeof(_cabi.RuleParams), 256, 1, 0.0, None)
