@@ -3,11 +3,13 @@
 //
 // What bounds it is reading K and V once; a tcgen05 tile would have 128 rows, of which a decoding call uses 1 to 16, all in one
 // warp's lanes of tensor memory, and that warp's 128 exponentials a row would be the step (32 requests of 2048-8192 keys,
-// H32 Hkv8 D128 bf16, cap and distances: 207 us, 106 at the copy rate).  So the small matrix instruction instead: each
-// of eight warps takes 16 keys of a 128-key block, S (16 x 16) = Q K^T with Q in registers and K by ldmatrix from the tile TMA
-// has brought, its own running maximum and sum, O (16 x D) += P V in registers.  A warp never waits for another one until a
-// stretch ends, when the eight are put together through shared memory.  P is fp16, or for bf16 calls a pair of bf16 hi + lo (two
-// products), so that its rounding stays below the output's.
+// H32 Hkv8 D128 bf16, cap and distances: 207 us, here 124 to 139 from one GPU to another, 106 at the copy rate).  So the
+// small matrix instruction instead: each of eight warps takes 16 keys of a 128-key block, S (16 x 16) = Q K^T with Q in
+// registers and K by ldmatrix from the tile TMA has brought, its own running maximum and sum, O (16 x D) += P V in registers.
+// A warp never waits for another one until a stretch ends, when the eight are put together through shared memory.  P is fp16,
+// or for bf16 calls a pair of bf16 hi + lo (two products), so that its rounding stays below the output's.
+// Sixteen warps (registers then spill: 202 us), 8-row registers (no change) and, at D 64, two blocks a warp at once (no
+// change) brought nothing; D 64 gets 62 % of D 128's rate out of a cache whose heads lie side by side, 128 bytes a head.
 #pragma once
 
 template <int D>
@@ -276,7 +278,7 @@ fwd_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                         o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
                     }
                     if (!st.whole()) {
-                        a.part_o[(slot * (D / 4) + col / 4) * (int64_t)a.part_rows + r] = o;
+                        a.part_o[(slot * a.part_rows + r) * (D / 4) + col / 4] = o;
                         if (col == 0) a.part_ml[slot * a.part_rows + r] = make_float2(big, sum);
                     } else {
                         const int i = r / a.pack, h = st.h * a.pack + r % a.pack;
@@ -293,4 +295,55 @@ fwd_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     }
     __syncthreads();
     if (threadIdx.x == 0 && *abort_flag) report_status(a.status, 1);
+}
+
+// Put together what ranges cut: block (c, r) takes row r of the pair that starts in CTA c's range and goes on in others.  A
+// thread holds four columns and every U-th part, so that a few parts are under way at once; the U sums are added in
+// their order, which does not depend on which CTA finished first.  What bounds it is the latency of its loads (a lane a row, all
+// parts one after another, as fwd_merge_kernel has it for tiles: 16 us for the 18 parts of one request's 4096 keys, H32 Hkv8 D128 bf16;
+// the call 31 -> 18 us, with 16384 keys 43 -> 31).
+template <int D, bool BF16>
+__global__ void __launch_bounds__(128) fwd_decode_merge_kernel(const FwdArgs a) {
+    using T16 = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+    constexpr int C = D / 4, U = 128 / C;
+    __shared__ float4 sum_o[U][C];
+    __shared__ float sum_l[U];
+    const int c = blockIdx.x, r = blockIdx.y, u = threadIdx.x / C, col = threadIdx.x % C;
+    auto at = [&](int k) { return (2 * ((int64_t)c + k) + (k == 0 ? 1 : 0)) * a.part_rows + r; };
+    grid_dependency_wait();
+    const int4 meta = a.part_meta[c];
+    // (read before the record is there: a part that is none is not used)
+    const int64_t first = at(c + u < (int)gridDim.x ? u : 0);
+    const float2 ml0 = a.part_ml[first];
+    const float4 o0 = a.part_o[first * C + col];
+    if (meta.w == 0) return;
+    float m = -INFINITY, l = 0.f;
+    for (int k = threadIdx.x & 31; k < meta.w; k += 32) m = fmaxf(m, a.part_ml[at(k)].x);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float2 ml, const float4 o) {
+        const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+        l = fmaf(w, ml.y, l);
+        acc.x = fmaf(w, o.x, acc.x); acc.y = fmaf(w, o.y, acc.y); acc.z = fmaf(w, o.z, acc.z); acc.w = fmaf(w, o.w, acc.w);
+    };
+    if (u < meta.w) add(ml0, o0);
+#pragma unroll 4
+    for (int k = u + U; k < meta.w; k += U) add(a.part_ml[at(k)], a.part_o[at(k) * C + col]);
+    sum_o[u][col] = acc;
+    if (col == 0) sum_l[u] = l;
+    __syncthreads();
+    if (u != 0) return;
+#pragma unroll
+    for (int x = 1; x < U; ++x) {
+        const float4 o = sum_o[x][col];
+        acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
+        l += sum_l[x];
+    }
+    const int i = r / a.pack, h = meta.y * a.pack + r % a.pack;
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    if (col * 4 < a.d)
+        *reinterpret_cast<uint2*>(reinterpret_cast<T16*>(a.o) + meta.x * a.o_sb + i * a.o_sn + h * a.o_sh + col * 4) =
+            make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+    if (col == 0) a.lse[((int64_t)meta.x * a.H + h) * a.Nq + i] = kLn2 * ((m - kPShift) + log2f(l));
 }

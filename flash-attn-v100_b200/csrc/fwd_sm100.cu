@@ -1611,7 +1611,7 @@ FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, bool r
         pl.meta_off = pl.ml_off + align_up(slots * sizeof(float2), 256);
         pl.bytes = pl.meta_off + align_up((size_t)pl.ctas * sizeof(int4), 256);
     };
-    if (ruled && (int64_t)p.Nq * group <= kDecodeRows) {
+    if (ruled && (int64_t)p.Nq * group <= kDecodeRows && !p.o_lo.ptr) {
         // the rows of a K/V head together, a range of its key blocks a CTA; a pair's end (the warps' sums) takes about a block's time
         const int64_t units = (int64_t)p.B * p.Hkv * ((p.Nk + kBlockN - 1) / kBlockN);
         if (units < (1 << 28)) {
@@ -1769,15 +1769,23 @@ int launch(const fa_b200_params& p, void* ws, size_t ws_bytes, const Rules* rule
     }
     if constexpr (PREC == 0) if (plan.sched) {
         cudaLaunchConfig_t cfg = {};
+        auto merge = fwd_merge_kernel<D, BF16, RULES != 0>;
         cfg.gridDim = dim3((unsigned)plan.ctas, (unsigned)(plan.part_rows / 32));
         cfg.blockDim = dim3(256);
+#ifdef FA_RULES_INSTANCES
+        if (plan.sched == 3) {
+            merge = fwd_decode_merge_kernel<D, BF16>;
+            cfg.gridDim.y = (unsigned)(p.Nq * plan.pack);
+            cfg.blockDim = dim3(128);
+        }
+#endif
         cfg.stream = (cudaStream_t)p.stream;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        FA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fwd_merge_kernel<D, BF16, RULES != 0>, a));
+        FA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, merge, a));
     }
     return FA_OK;
 }
