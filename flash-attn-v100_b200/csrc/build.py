@@ -14,7 +14,7 @@ OUT_DIR = os.path.join(os.path.dirname(HERE), "flash_attention_v100", "lib")
 OUT = os.path.join(OUT_DIR, "libfa_b200.so")
 OP_OUT = os.path.join(OUT_DIR, "fa_b200_torch.so")
 OP_SOURCE = "torch_op.cpp"
-SOURCES = ["host_api.cu", "simt_kernels.cu", "fwd_sm100.cu", "fwd_tf32_sm100.cu", "bwd_sm100.cu", "bwd_f32_sm100.cu", "combine.cu", "compact.cu",
+SOURCES = ["host_api.cu", "simt_kernels.cu", "simt_rules.cu", "fwd_sm100.cu", "fwd_tf32_sm100.cu", "bwd_sm100.cu", "bwd_f32_sm100.cu", "combine.cu", "compact.cu",
            "fwd_pair_sm100.cu", "bwd_pair_sm100.cu", "key_ranges.cu", "rotary.cu",
            "fwd_rules_sm100.cu", "bwd_rules_sm100.cu"]
 HEADERS = ["fa_common.cuh", "philox.cuh", "sm100_ptx.cuh", "tma_host.cuh", "tile_config.cuh", "score_rules.cuh", "fwd_decode.cuh",
@@ -88,7 +88,7 @@ def build_library(force=False, verbose=False):
         o = os.path.join(OUT_DIR, os.path.basename(s).replace(".cu", ".o"))
         objs.append(o)
         flags = list(NVCC_FLAGS)
-        if os.path.basename(s) in ("simt_kernels.cu", "rotary.cu"):
+        if os.path.basename(s) in ("simt_kernels.cu", "simt_rules.cu", "rotary.cu"):
             flags.remove("--use_fast_math")  # exact expf/logf/division in the fp32 family, sincosf of rotary angles
         cmd = [nvcc] + flags + ["-c", s, "-o", o]
         procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))

@@ -150,9 +150,11 @@ static inline Rules make_rules(const fa_b200_rules& r, int Nq, int Nk) {
 }
 
 // ---- kernel families ---------------------------------------------------------
-// CUDA-core tiles (simt_kernels.cu)
-int simt_fwd(const fa_b200_params& p, const Rules* rules = nullptr);
+// CUDA-core tiles (simt_kernels.cu; calls with rules: simt_rules.cu, which simt_bwd goes to behind delta)
+int simt_fwd(const fa_b200_params& p);
 int simt_bwd(const fa_b200_params& p, const BwdWorkspace& ws, const Rules* rules = nullptr);
+int simt_rules_fwd(const fa_b200_params& p, const Rules& rules);
+int simt_rules_bwd(const fa_b200_params& p, const float* delta, const Rules& rules);
 bool simt_supports(const fa_b200_params& p);
 
 // TMA + tcgen05 (fwd_sm100.cu, bwd_sm100.cu)

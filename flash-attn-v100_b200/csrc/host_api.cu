@@ -424,7 +424,7 @@ int fa_b200_fwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r, void
     GuardDevice g(p->device);
     if (!g.ok) { set_error("cudaSetDevice(%d) failed", p->device); return FA_ECUDA; }
     const Rules u = make_rules(*r, p->Nq, p->Nk);
-    return variant != FA_B200_VARIANT_SIMT ? sm100_rules_fwd(*p, u, workspace, workspace_bytes) : simt_fwd(*p, &u);
+    return variant != FA_B200_VARIANT_SIMT ? sm100_rules_fwd(*p, u, workspace, workspace_bytes) : simt_rules_fwd(*p, u);
 }
 
 size_t fa_b200_bwd_rules_workspace_bytes(const fa_b200_params* p) {

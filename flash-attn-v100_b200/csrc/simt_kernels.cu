@@ -44,58 +44,22 @@ struct SimtArgs {
     float inv_keep;      // 1 / (1 - effective p)
     PhiloxKey key;
     DropoutOrigin rng;
-    Rules rules;         // RULES instances only
 };
-
-// RULES instances (DC: the head size, known when compiling, where fp32 calls mostly have it: B2 N500 H4 D64, five documents, forward
-// and backward 79 + 249 -> 61 + 157 us; 0: any): scores bent by a cap, moved by a distance, hidden outside a row's range (fa_b200_rules).  Rows of K and V
-// outside the hull of the query tile's ranges are read as zeros, so that memory nobody sees may hold anything.
-struct RowRule { int first, end, position; };
-__device__ __forceinline__ RowRule row_rule(const Rules& u, int b, int i, int Nq) {
-    RowRule r = {0, 0, 0};
-    if (i < Nq) {
-        const int2 x = u.rows[b * u.rows_b + i];
-        r.first = x.x; r.end = x.y;
-        r.position = i + u.origin[b * u.origin_b];
-    }
-    return r;
-}
-// Keys that rows of a 64-row query tile see ((0, 0): none).
-__device__ __forceinline__ int2 hull_of(const Rules& u, int b, int tile) {
-    const int2* parts = u.q_parts + b * u.q_parts_b + tile * (BM / 16);
-    int2 r = make_int2(0x7fffffff, 0);
-#pragma unroll
-    for (int e = 0; e < BM / 16; ++e) {
-        const int2 h = parts[e];
-        if (h.y > 0) { r.x = min(r.x, h.x); r.y = max(r.y, h.y); }
-    }
-    return r.y > 0 ? r : make_int2(0, 0);
-}
-// x of a score s = scale q.k, and the derivative of x by s
-__device__ __forceinline__ float ruled_score(const Rules& u, float slope, float s, int position, int key, float& dx) {
-    dx = 1.f;
-    if (u.cap > 0.f) {
-        const float t = tanhf(s / u.cap);
-        s = u.cap * t;
-        dx = 1.f - t * t;
-    }
-    return s - slope * fabsf((float)position - (float)key);
-}
 
 template <typename T>
 __device__ __forceinline__ void load_tile(float* dst, int ld, const T* base, int64_t stride_n,
-                                          int row0, int nrows, int D, int rows_in_tile, int from = 0) {
+                                          int row0, int nrows, int D, int rows_in_tile) {
     for (int idx = threadIdx.x; idx < rows_in_tile * D; idx += NT) {
         int r = idx / D, c = idx - r * D;
         int gr = row0 + r;
-        dst[r * ld + c] = (gr < nrows && gr >= from) ? to_f32<T>(base[(int64_t)gr * stride_n + c]) : 0.f;
+        dst[r * ld + c] = (gr < nrows) ? to_f32<T>(base[(int64_t)gr * stride_n + c]) : 0.f;
     }
 }
 
-template <typename T, bool RULES, int DC = 0>
+template <typename T>
 __global__ void __launch_bounds__(NT) simt_fwd_kernel(SimtArgs a) {
     extern __shared__ float smem[];
-    const int D = DC ? DC : a.D, ld = D + 1;
+    const int D = a.D, ld = D + 1;
     float* Qs = smem;
     float* Ks = Qs + BM * ld;
     float* Vs = Ks + BN * ld;
@@ -129,21 +93,11 @@ __global__ void __launch_bounds__(NT) simt_fwd_kernel(SimtArgs a) {
     const int nk = kv_len_of(a.kv_len, b, a.Nk);      // keys this batch entry attends to
     int kv_end = nk;
     if (a.causal && m0 + BM + a.shift < kv_end) kv_end = m0 + BM + a.shift;
-    int from = 0, to = a.Nk;                          // keys that are read
-    float slope = 0.f;
-    RowRule rule[4];
-    if (RULES) {
-        const int2 hull = hull_of(a.rules, b, mt);
-        from = max(hull.x, 0); to = kv_end = min(hull.y, a.Nk);
-        if (a.rules.slopes) slope = a.rules.slopes[h];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) rule[r] = row_rule(a.rules, b, m0 + ty * 4 + r, a.Nq);
-    }
 
-    for (int n0 = RULES ? from / BN * BN : 0; n0 < kv_end; n0 += BN) {
+    for (int n0 = 0; n0 < kv_end; n0 += BN) {
         __syncthreads();
-        load_tile<T>(Ks, ld, kb, a.k.stride_n, n0, to, D, BN, from);
-        load_tile<T>(Vs, ld, vb, a.v.stride_n, n0, to, D, BN, from);
+        load_tile<T>(Ks, ld, kb, a.k.stride_n, n0, a.Nk, D, BN);
+        load_tile<T>(Vs, ld, vb, a.v.stride_n, n0, a.Nk, D, BN);
         __syncthreads();
 
         float acc[4][4];
@@ -169,14 +123,8 @@ __global__ void __launch_bounds__(NT) simt_fwd_kernel(SimtArgs a) {
             for (int c = 0; c < 4; ++c) {
                 int j = n0 + tx + 16 * c;
                 float s = acc[r][c] * a.scale;
-                if constexpr (RULES) {
-                    float dx;
-                    s = ruled_score(a.rules, slope, s, rule[r].position, j, dx);
-                    if (j < rule[r].first || j >= rule[r].end) s = -INFINITY;
-                } else {
-                    if (bias_b && i < a.Nq && j < nk) s += bias_b[(int64_t)i * a.bias.stride_n + j];
-                    if (j >= nk || (a.causal && j > i + a.shift)) s = -INFINITY;
-                }
+                if (bias_b && i < a.Nq && j < nk) s += bias_b[(int64_t)i * a.bias.stride_n + j];
+                if (j >= nk || (a.causal && j > i + a.shift)) s = -INFINITY;
                 Ss[(ty * 4 + r) * SLD + tx + 16 * c] = s;
             }
         }
@@ -243,7 +191,6 @@ __global__ void __launch_bounds__(NT) simt_fwd_kernel(SimtArgs a) {
         int row = ty * 4 + r, i = m0 + row;
         if (i < a.Nq) {
             float inv = 1.f / row_l[row];
-            if (RULES && row_l[row] == 0.f) inv = 0.f;        // a row that sees nothing
 #pragma unroll
             for (int c = 0; c < MAXC; ++c) {
                 int col = tx + 16 * c;
@@ -287,10 +234,10 @@ __global__ void __launch_bounds__(256) simt_delta_kernel(SimtArgs a) {
 }
 
 // MODE 0: key-stationary, writes dK and dV.  MODE 1: query-stationary, writes dQ.
-template <typename T, int MODE, bool RULES, int DC = 0>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(NT) simt_bwd_kernel(SimtArgs a) {
     extern __shared__ float smem[];
-    const int D = DC ? DC : a.D, ld = D + 1;
+    const int D = a.D, ld = D + 1;
     float* Qs = smem;
     float* Gs = Qs + BM * ld;    // dO tile
     float* Ks = Gs + BM * ld;
@@ -338,23 +285,12 @@ __global__ void __launch_bounds__(NT) simt_bwd_kernel(SimtArgs a) {
         if (MODE == 0) {
             it_begin = (a.causal && tile * BN > a.shift) ? (tile * BN - a.shift) / BM : 0;
             it_end = (a.Nq + BM - 1) / BM;
-            if (RULES) {
-                const int2 seen = a.rules.k_tiles[b * a.rules.k_tiles_b + tile * BN / 128];
-                it_begin = max(seen.x, 0) * (128 / BM);
-                it_end = min(it_end, seen.y * (128 / BM));
-            }
         } else {
             int kv_end = nk;
             if (a.causal && tile * BM + BM + a.shift < kv_end) kv_end = tile * BM + BM + a.shift;
             it_begin = 0;
-            if (RULES) {
-                const int2 hull = hull_of(a.rules, b, tile);
-                it_begin = max(hull.x, 0) / BN;
-                kv_end = min(hull.y, a.Nk);
-            }
             it_end = (kv_end + BN - 1) / BN;
         }
-        const float slope = RULES && a.rules.slopes ? a.rules.slopes[h] : 0.f;
         if (MODE == 1) {
             __syncthreads();
             load_tile<T>(Qs, ld, qb, a.q.stride_n, tile * BM, a.Nq, D, BM);
@@ -369,10 +305,6 @@ __global__ void __launch_bounds__(NT) simt_bwd_kernel(SimtArgs a) {
         for (int it = it_begin; it < it_end; ++it) {
             const int m0 = (MODE == 0) ? it * BM : tile * BM;
             const int n0 = (MODE == 0) ? tile * BN : it * BN;
-            if (RULES && MODE == 0) {              // (the list holds all tiles between the first and the last that meet this one's 128 keys)
-                const int2 hull = hull_of(a.rules, b, it);
-                if (hull.x >= n0 + BN || hull.y <= n0) continue;
-            }
             __syncthreads();
             if (MODE == 0) {
                 load_tile<T>(Qs, ld, qb, a.q.stride_n, m0, a.Nq, D, BM);
@@ -417,26 +349,20 @@ __global__ void __launch_bounds__(NT) simt_bwd_kernel(SimtArgs a) {
             for (int r = 0; r < 4; ++r) {
                 const int row = ty * 4 + r, i = m0 + row;
                 const float lse_i = lse_s[row], del_i = del_s[row];
-                RowRule rule;
-                if (RULES) rule = row_rule(a.rules, b, i, a.Nq);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const int col = tx + 16 * c, j = n0 + col;
                     float p = 0.f, z = 1.f;
-                    float dx = 1.f;
                     bool visible = (i < a.Nq) && (j < nk) && !(a.causal && j > i + a.shift);
-                    if (RULES) visible = j >= rule.first && j < rule.end;
                     if (visible) {
                         float s = s_acc[r][c] * a.scale;
-                        if (RULES) s = ruled_score(a.rules, slope, s, rule.position, j, dx);
-                        else if (bias_b) s += bias_b[(int64_t)i * a.bias.stride_n + j];
+                        if (bias_b) s += bias_b[(int64_t)i * a.bias.stride_n + j];
                         p = expf(s - lse_i);
                     }
                     if (a.drop_thr)
                         z = dropout_keep(a.key, bh, (uint32_t)i, (uint32_t)j, a.drop_thr) ? a.inv_keep : 0.f;
                     Ps[row * SLD + col] = p * z;
-                    float ds = p * (p_acc[r][c] * z - del_i);
-                    if (RULES) ds = visible ? ds * dx : 0.f;
+                    const float ds = p * (p_acc[r][c] * z - del_i);
                     Ds[row * SLD + col] = ds;
                     if (MODE == 1 && ds_b && visible) ds_b[(int64_t)i * a.Nk + j] = ds;
                 }
@@ -610,9 +536,8 @@ dropout_bits_kernel(PhiloxKey key, uint32_t thr, DropoutOrigin rng, int H, int N
     }
 }
 
-SimtArgs make_args(const fa_b200_params& p, float* delta, const Rules* rules) {
+SimtArgs make_args(const fa_b200_params& p, float* delta) {
     SimtArgs a;
-    a.rules = rules ? *rules : Rules{};
     a.q = p.q; a.k = p.k; a.v = p.v; a.o = p.o; a.d_o = p.d_o; a.dq = p.dq; a.dk = p.dk; a.dv = p.dv;
     a.o_lo = p.o_lo;
     a.lse = p.lse; a.delta = delta;
@@ -632,24 +557,22 @@ int set_smem(K kernel, size_t bytes) {
     return FA_OK;
 }
 
-template <typename T, bool RULES>
-int launch_fwd(const fa_b200_params& p, const Rules* rules) {
-    SimtArgs a = make_args(p, nullptr, rules);
+template <typename T>
+int launch_fwd(const fa_b200_params& p) {
+    SimtArgs a = make_args(p, nullptr);
     size_t smem = ((size_t)(BM + 2 * BN) * (p.D + 1) + (size_t)BM * SLD + 3 * BM) * sizeof(float);
-    auto kernel = simt_fwd_kernel<T, RULES>;
-    if constexpr (RULES) kernel = p.D == 64 ? simt_fwd_kernel<T, true, 64> : (p.D == 32 ? simt_fwd_kernel<T, true, 32> : kernel);
-    int rc = set_smem(kernel, smem);
+    int rc = set_smem(simt_fwd_kernel<T>, smem);
     if (rc) return rc;
     dim3 grid((p.Nq + BM - 1) / BM, p.H, p.B);
-    kernel<<<grid, NT, smem, (cudaStream_t)p.stream>>>(a);
+    simt_fwd_kernel<T><<<grid, NT, smem, (cudaStream_t)p.stream>>>(a);
     FA_CUDA_CHECK(cudaGetLastError());
     return FA_OK;
 }
 
-template <typename T, bool RULES>
+template <typename T>
 int launch_bwd(const fa_b200_params& p, const BwdWorkspace& ws, const Rules* rules) {
     float* delta = (float*)((char*)p.workspace + ws.delta_off);
-    SimtArgs a = make_args(p, delta, rules);
+    SimtArgs a = make_args(p, delta);
     cudaStream_t st = (cudaStream_t)p.stream;
     int64_t rows = (int64_t)p.B * p.H * p.Nq;
     const int phases = p.bwd_phases ? p.bwd_phases : 7;
@@ -657,24 +580,20 @@ int launch_bwd(const fa_b200_params& p, const BwdWorkspace& ws, const Rules* rul
         simt_delta_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(a);
         FA_CUDA_CHECK(cudaGetLastError());
     }
+    if (rules) return simt_rules_bwd(p, delta, *rules);
     size_t smem = ((size_t)(2 * BM + 2 * BN) * (p.D + 1) + (size_t)2 * BM * SLD + 2 * BM) * sizeof(float);
-    auto k0 = simt_bwd_kernel<T, 0, RULES>, k1 = simt_bwd_kernel<T, 1, RULES>;
-    if constexpr (RULES) {
-        if (p.D == 64) { k0 = simt_bwd_kernel<T, 0, true, 64>; k1 = simt_bwd_kernel<T, 1, true, 64>; }
-        if (p.D == 32) { k0 = simt_bwd_kernel<T, 0, true, 32>; k1 = simt_bwd_kernel<T, 1, true, 32>; }
-    }
-    int rc = set_smem(k0, smem);
+    int rc = set_smem(simt_bwd_kernel<T, 0>, smem);
     if (rc) return rc;
-    rc = set_smem(k1, smem);
+    rc = set_smem(simt_bwd_kernel<T, 1>, smem);
     if (rc) return rc;
     if (phases & 2) {
         dim3 grid_kv((p.Nk + BN - 1) / BN, p.Hkv, p.B);
-        k0<<<grid_kv, NT, smem, st>>>(a);
+        simt_bwd_kernel<T, 0><<<grid_kv, NT, smem, st>>>(a);
         FA_CUDA_CHECK(cudaGetLastError());
     }
     if (phases & 4) {
         dim3 grid_q((p.Nq + BM - 1) / BM, p.H, p.B);
-        k1<<<grid_q, NT, smem, st>>>(a);
+        simt_bwd_kernel<T, 1><<<grid_q, NT, smem, st>>>(a);
         FA_CUDA_CHECK(cudaGetLastError());
     }
     return FA_OK;
@@ -684,20 +603,20 @@ int launch_bwd(const fa_b200_params& p, const BwdWorkspace& ws, const Rules* rul
 
 bool simt_supports(const fa_b200_params& p) { return p.D >= 1 && p.D <= 16 * MAXC; }
 
-int simt_fwd(const fa_b200_params& p, const Rules* rules) {
+int simt_fwd(const fa_b200_params& p) {
     switch (p.dtype) {
-        case FA_B200_F16:  return rules ? launch_fwd<__half, true>(p, rules) : launch_fwd<__half, false>(p, nullptr);
-        case FA_B200_BF16: return rules ? launch_fwd<__nv_bfloat16, true>(p, rules) : launch_fwd<__nv_bfloat16, false>(p, nullptr);
-        case FA_B200_F32:  return rules ? launch_fwd<float, true>(p, rules) : launch_fwd<float, false>(p, nullptr);
+        case FA_B200_F16:  return launch_fwd<__half>(p);
+        case FA_B200_BF16: return launch_fwd<__nv_bfloat16>(p);
+        case FA_B200_F32:  return launch_fwd<float>(p);
     }
     return FA_EINVAL;
 }
 
 int simt_bwd(const fa_b200_params& p, const BwdWorkspace& ws, const Rules* rules) {
     switch (p.dtype) {
-        case FA_B200_F16:  return rules ? launch_bwd<__half, true>(p, ws, rules) : launch_bwd<__half, false>(p, ws, nullptr);
-        case FA_B200_BF16: return rules ? launch_bwd<__nv_bfloat16, true>(p, ws, rules) : launch_bwd<__nv_bfloat16, false>(p, ws, nullptr);
-        case FA_B200_F32:  return rules ? launch_bwd<float, true>(p, ws, rules) : launch_bwd<float, false>(p, ws, nullptr);
+        case FA_B200_F16:  return launch_bwd<__half>(p, ws, rules);
+        case FA_B200_BF16: return launch_bwd<__nv_bfloat16>(p, ws, rules);
+        case FA_B200_F32:  return launch_bwd<float>(p, ws, rules);
     }
     return FA_EINVAL;
 }

@@ -104,6 +104,50 @@ def test_caps_and_scores_of_any_size(device, dtype, cap, std):
         assert (a.double() - w).norm() <= (TOLERANCE[t] + 1e-6 * (1 + std)) * w.norm() + 2.0 ** -20 * scale * w.numel() ** 0.5, n
 
 
+@pytest.mark.parametrize("dtype,H,Hkv,D", [("fp32", 2, 2, 128), ("fp32", 4, 2, 32), ("fp32", 2, 1, 20), ("fp32", 2, 2, 96), ("fp32", 3, 3, 33), ("fp32", 2, 2, 1),
+                                           ("fp16", 2, 1, 100), ("bf16", 2, 2, 9)])
+@pytest.mark.parametrize("layout", ["plain", "heads-first", "odd-addresses"])
+def test_cuda_core_tiles(device, dtype, H, Hkv, D, layout):
+    """Every width of tile, rows that can and cannot be copied 16 bytes at a time, K/V heads that several query heads read."""
+    t = TYPES[dtype]
+    host = dict(causal=True, offsets=[[0, 33, 190, 300]], prefixes=[[0, 40, 200]])
+    q, k, v, g = _inputs(1, 310, 310, H, Hkv, D, t, device)
+    if layout == "heads-first":
+        q, k, v, g = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v, g))
+    if layout == "odd-addresses":
+        q, k, v, g = (torch.cat([x[..., :1], x], dim=3)[..., 1:] for x in (q, k, v, g))
+    ranges, see, at = _ranges(310, 310, 1, host, device)
+    want = attention64(q, k, v, see, at, D ** -0.5, 4.0, _slopes(H, device), grad=g)
+    got = _step(q, k, v, g, score_cap=4.0, distance_slopes=_slopes(H, device), key_ranges=ranges)
+    _check(got, want, t, ("o", "lse", "dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(2, 1, 64), (2, 2, 128)])
+def test_cuda_core_tiles_of_long_rows(device, H, Hkv, D):
+    """More tiles of queries than a warp looks through at once, most of which a key tile's window leaves out."""
+    N = 4500
+    for host in (dict(causal=True, window=150), dict(causal=True, offsets=[[0, 100, 2300, 4490]])):
+        q, k, v, g = _inputs(1, N, N, H, Hkv, D, torch.float32, device)
+        ranges, see, at = _ranges(N, N, 1, host, device)
+        want = attention64(q, k, v, see, at, D ** -0.5, None, None, grad=g)
+        _check(_step(q, k, v, g, key_ranges=ranges), want, torch.float32, ("o", "lse", "dq", "dk", "dv"))
+
+
+def test_cuda_core_tiles_rows_of_any_order(device):
+    """Rows that see the first keys or the last ones, in turn: a key tile's list of query tiles has holes."""
+    rows = torch.zeros(1, 700, 2, dtype=torch.int32)
+    i = torch.arange(700)
+    rows[0, :, 0] = torch.where(i // 64 % 3 == 0, 5, 600)
+    rows[0, :, 1] = torch.where(i // 64 % 3 == 0, 90, 641)
+    rows[0, i // 64 % 3 == 2] = 0
+    r = fa.build_key_ranges(700, 650, batch=1, rows=rows.to(device))
+    j = torch.arange(650)
+    see = (j >= rows[..., :1]) & (j < rows[..., 1:])
+    q, k, v, g = _inputs(1, 700, 650, 2, 1, 64, torch.float32, device)
+    want = attention64(q, k, v, see, torch.arange(700).expand(1, 700), 0.125, 5.0, None, grad=g)
+    _check(_step(q, k, v, g, score_cap=5.0, key_ranges=r), want, torch.float32, ("o", "lse", "dq", "dk", "dv"))
+
+
 def test_without_ranges_the_calls_own_masks(device):
     """causal, key_lengths and the alignment build the ranges of the call; without any rule the result is the plain call's."""
     q, k, v, g = _inputs(2, 100, 260, 4, 2, 64, torch.bfloat16, device)
