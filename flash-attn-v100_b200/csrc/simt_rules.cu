@@ -281,8 +281,9 @@ __global__ void __launch_bounds__(NT) ruled_bwd_kernel(const RuledArgs a) {
     int2 hull = make_int2(0, 0);
     if (MODE == 0) {
         const int2 seen = a.rules.k_tiles[b * a.rules.k_tiles_b + x0 / 128];
-        begin = max(seen.x, 0) * (128 / BY);
-        end = min((a.Nq + BY - 1) / BY, seen.y * (128 / BY));
+        const int tiles = (a.Nq + BY - 1) / BY;
+        begin = min(max(seen.x, 0), tiles) * (128 / BY);
+        end = min(tiles, min(seen.y, tiles) * (128 / BY));
     } else {
         hull = hull_of<BX>(a, b, tile);
         begin = hull.x / BY;

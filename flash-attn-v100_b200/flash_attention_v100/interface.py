@@ -474,7 +474,8 @@ def flash_attention_v100_with_rules(
             head size it takes.  fp16 and bf16 with a head size that is a multiple of 8 run on the tensor cores, others on
             the CUDA cores
         score_cap: positive; None leaves the scores as they are
-        distance_slopes: (num_heads,) floating point, no gradient
+        distance_slopes: (num_heads,) floating point, no gradient.  A score x is rounded to 2^-24 |x|, as any 32-bit
+            evaluation has it: 2^-24 slope times distance, where a query is far from all keys it sees
         key_ranges: which keys each query sees (build_key_ranges): packed documents, prefixes, windows, ragged caches; built
             once, read by every layer.  Takes the place of causal, key_lengths and causal_alignment.  A query that sees
             nothing has an output of zeros, an lse of -inf and no gradient.  position_i counts its query offsets
