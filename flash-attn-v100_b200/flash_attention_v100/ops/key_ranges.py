@@ -2,7 +2,7 @@
 
 Packed documents, visible prefixes, sliding windows, causal masks and caches of ragged lengths are all such intervals.
 They are built on the GPU from lengths, once a step, and read by the attention of every layer
-(`flash_attention_v100(..., key_ranges=)`); whole key blocks that no row of a query tile sees are skipped.
+(`flash_attention_v100_with_rules(..., key_ranges=)`); whole key blocks that no row of a query tile sees are skipped.
 The reference expands masks to a dense bias instead (examples/basic_usage.py:228-250).
 """
 from __future__ import annotations
