@@ -72,7 +72,7 @@ __device__ __forceinline__ float ruled_score(float cap, float slope, float u, in
         u = cap * t;
         dx = 1.f - t * t;
     }
-    return u - slope * fabsf((float)position - (float)key);
+    return u - slope * fabsf((float)(position - key));         // (floats of their own would round positions from 2^24 on)
 }
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int bytes) {

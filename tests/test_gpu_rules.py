@@ -148,6 +148,26 @@ def test_cuda_core_tiles_rows_of_any_order(device):
     _check(_step(q, k, v, g, score_cap=5.0, key_ranges=r), want, torch.float32, ("o", "lse", "dq", "dk", "dv"))
 
 
+@pytest.mark.parametrize("dtype,Nq", [("bf16", 1), ("bf16", 40), ("fp32", 40)])
+def test_caches_beyond_32_bits(device, dtype, Nq):
+    """More than 2^31 elements of K and V, positions beyond 2^24: the last keys alone give the same."""
+    N, n, t = 17_000_000, 2000, TYPES[dtype]
+    k, v = (torch.zeros(1, N, 1, 128, device=device, dtype=t) for _ in range(2))
+    q, ks, vs, g = _inputs(1, Nq, n, 2, 1, 128, t, device)
+    k[:, -n:], v[:, -n:] = ks, vs
+    host = dict(causal=True, window=700, starts=n - Nq)
+    see, at = visible(Nq, n, 0, **host).unsqueeze(0), (torch.arange(Nq) + n - Nq).unsqueeze(0)
+    slopes = _slopes(2, device)
+    want = attention64(q, ks, vs, see, at, 0.1, 20.0, slopes, grad=g)
+    r = fa.build_key_ranges(Nq, N, causal=True, window=700, query_offsets=N - Nq, device=device)
+    with torch.no_grad():
+        o, lse = fa.flash_attention_v100_with_rules(q, k, v, scale=0.1, score_cap=20.0, distance_slopes=slopes, key_ranges=r, return_softmax_lse=True)
+    _check((o, lse), want, t, ("o", "lse"))
+    o, lse, dq, dk, dv = _step(q, k, v, g, scale=0.1, score_cap=20.0, distance_slopes=slopes, key_ranges=r)
+    _check((o, lse, dq, dk[:, -n:], dv[:, -n:]), want, t, ("o", "lse", "dq", "dk", "dv"))
+    assert not dk[:, :-n].any() and not dv[:, :-n].any()
+
+
 def test_without_ranges_the_calls_own_masks(device):
     """causal, key_lengths and the alignment build the ranges of the call; without any rule the result is the plain call's."""
     q, k, v, g = _inputs(2, 100, 260, 4, 2, 64, torch.bfloat16, device)
