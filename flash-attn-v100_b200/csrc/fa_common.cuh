@@ -181,7 +181,7 @@ static inline float pair_score_scale(const fa_b200_params& p) {
 bool sm100_pair_supports(const fa_b200_params& p, bool backward, const char** why);
 // The same kernels for calls with rules (fwd_rules_sm100.cu, bwd_rules_sm100.cu): what sm100_pair_supports covers.
 int sm100_rules_fwd(const fa_b200_params& p, const Rules& rules, void* ws, size_t ws_bytes);
-size_t sm100_rules_fwd_workspace_bytes(const fa_b200_params& p, int max_keys);
+size_t sm100_rules_fwd_workspace_bytes(const fa_b200_params& p, bool capped, int max_keys);
 int sm100_rules_bwd(const fa_b200_params& p, const BwdWorkspace& ws, const Rules& rules);
 size_t sm100_rules_bwd_part_bytes(const fa_b200_params& p);
 // fp32 forward on the tensor cores (fwd_tf32_sm100.cu): TF32 products taken three times

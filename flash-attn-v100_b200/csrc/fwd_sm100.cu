@@ -1538,6 +1538,76 @@ __global__ void __launch_bounds__(256) fwd_merge_kernel(const FwdArgs a) {
 }
 
 #ifdef FA_RULES_INSTANCES
+// The same for pairs of many parts (kManyParts): block (c, y, z) takes 32 rows and 16 columns, a warp every eighth part, with a
+// maximum of its own; the warps' sums are added in their order.  bf16, cap, D 128, H 8,
+// one sequence: 17 queries on 16000 keys (19 parts a pair) 65 -> 53 us, on 4096 of them 45 -> 34; H 2, 300 queries on 16000 (37
+// parts) 64 -> 50.  With 9 parts a pair 300 queries on 3000 keys took 48 instead of 43.
+constexpr int kManyParts = 12;                 // ranges a pair, on average
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) fwd_merge_many_kernel(const FwdArgs a) {
+    using T16 = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+    __shared__ float4 sum_o[8][4][32];
+    __shared__ float2 sum_ml[8][32];
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x;
+    const int rr = (int)blockIdx.y * 32 + lane, t = rr / kBlockM, r = rr % kBlockM, c4 = (int)blockIdx.z * 4;
+    auto slot_of = [&](int k) { return 2 * ((int64_t)c + k) + (k == 0 ? 1 : 0); };
+    const int4 meta = a.part_meta[c];
+    const int64_t first = slot_of(c + warp < (int)gridDim.x ? warp : 0);       // (read before the record is there)
+    const float2 ml0 = a.part_ml[first * a.part_rows + rr];
+    float4 o0[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) o0[g] = a.part_o[(first * (D / 4) + c4 + g) * a.part_rows + rr];
+    if (meta.w == 0) return;
+    float m = -INFINITY, l = 0.f;
+    float4 acc[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) acc[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (warp < meta.w) m = ml0.x;
+#pragma unroll 4
+    for (int k = warp + 8; k < meta.w; k += 8) m = fmaxf(m, a.part_ml[slot_of(k) * a.part_rows + rr].x);
+    auto add = [&](const float2 ml, auto&& part) {
+        const float w = ml.y < 0.f || ml.x == -INFINITY ? 0.f : ex2(ml.x - m);       // (below 0: none of the tile's blocks lay in this range)
+        if (w == 0.f) return;
+        l = fmaf(w, ml.y, l);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 x = part(g);
+            acc[g].x = fmaf(w, x.x, acc[g].x); acc[g].y = fmaf(w, x.y, acc[g].y); acc[g].z = fmaf(w, x.z, acc[g].z); acc[g].w = fmaf(w, x.w, acc[g].w);
+        }
+    };
+    if (warp < meta.w) add(ml0, [&](int g) { return o0[g]; });
+#pragma unroll 2
+    for (int k = warp + 8; k < meta.w; k += 8) {
+        const int64_t slot = slot_of(k);
+        add(a.part_ml[slot * a.part_rows + rr], [&](int g) { return a.part_o[(slot * (D / 4) + c4 + g) * a.part_rows + rr]; });
+    }
+    sum_ml[warp][lane] = make_float2(m, l);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) sum_o[warp][g][lane] = acc[g];
+    __syncthreads();
+    const int i = (meta.z * 2 + t) * a.q_per_tile + r / a.pack, h = meta.y * a.pack + r % a.pack, b = meta.x;
+    if (warp >= 4 || r >= a.pack * a.q_per_tile || i >= a.Nq) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, sum_ml[w][lane].x);
+    l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        const float2 ml = sum_ml[w][lane];
+        const float by = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+        const float4 x = sum_o[w][warp][lane];
+        l = fmaf(by, ml.y, l);
+        o.x = fmaf(by, x.x, o.x); o.y = fmaf(by, x.y, o.y); o.z = fmaf(by, x.z, o.z); o.w = fmaf(by, x.w, o.w);
+    }
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    const int col = (c4 + warp) * 4;
+    if (col < a.d)
+        *reinterpret_cast<uint2*>(reinterpret_cast<T16*>(a.o) + (int64_t)b * a.o_sb + (int64_t)i * a.o_sn + (int64_t)h * a.o_sh + col) =
+            make_uint2(pack2<BF16>(o.x * inv, o.y * inv), pack2<BF16>(o.z * inv, o.w * inv));
+    if (col == 0) a.lse[((int64_t)b * a.H + h) * a.Nq + i] = kLn2 * ((m - kPShift) + log2f(l));
+}
 #include "fwd_decode.cuh"
 #endif
 
@@ -1595,9 +1665,11 @@ constexpr int kDecodeRows = 16;        // rows of a K/V head that fwd_decode_ker
 // With rules whole pairs are dealt out as CTAs get done (Dealer), so a round-robin share is what the SMs have on average, one
 // pair at least, and a pair's keys are at most `max_keys` and its own 256 (0: not known).  Ranges cost more there, because a
 // packed tile's hull is read from memory wherever a walk comes to it: 700 queries on 8892 keys, H32 Hkv8 D128 bf16, whole ->
-// ranges, us: all keys 139 -> 133, with a cap 215 -> 172; window 4096 78 -> 90, 113 -> 115; window 1024 35 -> 57, 45 -> 68.
-constexpr int kMergeUnitsRules = 16;
-FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, bool ruled = false, int max_keys = 0) {
+// ranges, us: all keys 139 -> 133, with a cap 215 -> 172; window 4096 82 -> 90, 118 -> 111; window 1024 35 -> 57, 45 -> 68.
+// A block with a cap takes half as long again, so a merge is worth fewer of them.
+constexpr int kMergeUnitsRules = 16, kMergeUnitsCap = 8;
+FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, int rules = 0, int max_keys = 0) {
+    const bool ruled = rules != 0;
     FwdPlan pl;
     memset(&pl, 0, sizeof(pl));
     auto pairs_of = [&](int qpt) { return (int)(((int64_t)p.Nq + 2 * qpt - 1) / (2 * qpt)); };
@@ -1643,7 +1715,7 @@ FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, bool r
     int64_t ranges = (total + pl.ctas - 1) / pl.ctas;
     const bool one_tile = p.Nq <= pl.q_per_tile, counts = p.kv_lengths || ruled;
     if (counts && one_tile) ranges = (3 * ranges + 3) / 4;
-    if (total < (1 << 28) && whole * 9 > (ranges + (ruled ? kMergeUnitsRules : kMergeUnits)) * 10) {
+    if (total < (1 << 28) && whole * 9 > (ranges + (rules == 2 ? kMergeUnitsCap : (ruled ? kMergeUnitsRules : kMergeUnits))) * 10) {
         pl.sched = one_tile ? 2 : 1;
         pl.start_cost = counts && one_tile && ranges >= kLongRange ? 3 : 0;
         const int tiles = (int)(((int64_t)p.Nq + pl.q_per_tile - 1) / pl.q_per_tile);
@@ -1660,8 +1732,8 @@ int launch(const fa_b200_params& p, void* ws, size_t ws_bytes, const Rules* rule
     const int sms = sm_count(p.device);
     if (sms <= 0) { set_error("cannot read the SM count of device %d", p.device); return FA_ECUDA; }
     const int max_keys = rules ? rules->max_keys : 0;
-    FwdPlan plan = plan_schedule(p, D, sms, ws != nullptr, RULES != 0, max_keys);
-    if (ws_bytes < plan.bytes || ((uintptr_t)ws & 255u) != 0) plan = plan_schedule(p, D, sms, false, RULES != 0, max_keys);
+    FwdPlan plan = plan_schedule(p, D, sms, ws != nullptr, RULES, max_keys);
+    if (ws_bytes < plan.bytes || ((uintptr_t)ws & 255u) != 0) plan = plan_schedule(p, D, sms, false, RULES, max_keys);
     const CUtensorMapDataType dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap mq, mk, mv;
     int r;
@@ -1777,6 +1849,9 @@ int launch(const fa_b200_params& p, void* ws, size_t ws_bytes, const Rules* rule
             merge = fwd_decode_merge_kernel<D, BF16>;
             cfg.gridDim.y = (unsigned)(p.Nq * plan.pack);
             cfg.blockDim = dim3(128);
+        } else if (plan.ctas >= kManyParts * p.B * plan.heads * plan.n_pairs && !p.o_lo.ptr) {
+            merge = fwd_merge_many_kernel<D, BF16>;
+            cfg.gridDim.z = D / 16;
         }
 #endif
         cfg.stream = (cudaStream_t)p.stream;
@@ -1802,8 +1877,8 @@ int fwd_by_type(const fa_b200_params& p, const Rules& rules, void* ws, size_t ws
 int sm100_rules_fwd(const fa_b200_params& p, const Rules& rules, void* ws, size_t ws_bytes) {
     return rules.cap > 0.f ? fwd_by_type<2>(p, rules, ws, ws_bytes) : fwd_by_type<1>(p, rules, ws, ws_bytes);
 }
-size_t sm100_rules_fwd_workspace_bytes(const fa_b200_params& p, int max_keys) {
-    return plan_schedule(p, p.D > 64 ? 128 : 64, sm_count(p.device), true, true, max_keys).bytes;
+size_t sm100_rules_fwd_workspace_bytes(const fa_b200_params& p, bool capped, int max_keys) {
+    return plan_schedule(p, p.D > 64 ? 128 : 64, sm_count(p.device), true, capped ? 2 : 1, max_keys).bytes;
 }
 #elif !defined(FA_PAIR_INSTANCES)
 bool tensor_ok(const fa_b200_tensor& t, int64_t B, int64_t N, int64_t H) {

@@ -410,7 +410,7 @@ size_t fa_b200_fwd_rules_workspace_bytes(const fa_b200_params* p, const fa_b200_
     if (p->B <= 0 || p->Nq <= 0 || p->Nk <= 0 || p->H <= 0 || p->Hkv <= 0 || p->D <= 0 || p->H % p->Hkv != 0) return 0;
     int variant;
     if (choose_rules_variant(*p, false, &variant) != FA_OK || variant == FA_B200_VARIANT_SIMT) return 0;
-    return sm100_rules_fwd_workspace_bytes(*p, r->max_keys);
+    return sm100_rules_fwd_workspace_bytes(*p, r->score_cap > 0.f, r->max_keys);
 }
 
 int fa_b200_fwd_with_rules(const fa_b200_params* p, const fa_b200_rules* r, void* workspace, size_t workspace_bytes) {

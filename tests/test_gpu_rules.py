@@ -168,6 +168,25 @@ def test_caches_beyond_32_bits(device, dtype, Nq):
     assert not dk[:, :-n].any() and not dv[:, :-n].any()
 
 
+@pytest.mark.parametrize("dtype,B,Nq,Nk,H,Hkv,D", [("bf16", 1, 17, 16000, 2, 2, 128), ("fp16", 1, 300, 9000, 2, 2, 64), ("bf16", 2, 40, 6000, 4, 2, 80), ("fp16", 3, 33, 5000, 3, 1, 128)])
+@pytest.mark.parametrize("window", [None, 3100])
+def test_few_queries_on_long_caches(device, dtype, B, Nq, Nk, H, Hkv, D, window):
+    """Rows whose keys are cut into many ranges, parts of which, or all, hold nothing for a request with few keys."""
+    t = TYPES[dtype]
+    lengths = [Nk, 200, 0][:B]
+    host = dict(causal=True, window=window, lengths=lengths, starts=[max(n - Nq, 0) for n in lengths])
+    q, k, v, _ = _inputs(B, Nq, Nk, H, Hkv, D, t, device)
+    ranges, see, at = _ranges(Nq, Nk, B, host, device)
+    for cap, slopes in ((None, None), (6.0, _slopes(H, device))):
+        want = attention64(q, k, v, see, at, D ** -0.5, cap, slopes)
+        with torch.no_grad():
+            got = fa.flash_attention_v100_with_rules(q, k, v, score_cap=cap, distance_slopes=slopes, key_ranges=ranges, return_softmax_lse=True)
+            again = fa.flash_attention_v100_with_rules(q, k, v, score_cap=cap, distance_slopes=slopes, key_ranges=ranges)
+        _check(got, want, t, ("o", "lse"))
+        assert torch.equal(got[0], again)
+        assert (got[0].cpu()[~see.any(dim=2)] == 0).all()
+
+
 def test_without_ranges_the_calls_own_masks(device):
     """causal, key_lengths and the alignment build the ranges of the call; without any rule the result is the plain call's."""
     q, k, v, g = _inputs(2, 100, 260, 4, 2, 64, torch.bfloat16, device)
