@@ -187,6 +187,21 @@ def test_few_queries_on_long_caches(device, dtype, B, Nq, Nk, H, Hkv, D, window)
         assert (got[0].cpu()[~see.any(dim=2)] == 0).all()
 
 
+@pytest.mark.parametrize("H,Hkv", [(3, 1), (10, 2), (7, 1), (100, 1)])
+def test_forward_bits_do_not_depend_on_what_memory_held(device, H, Hkv):
+    """Groups of heads that do not divide a tile: the same bits after other kernels have used shared memory."""
+    q, k, v, _ = _inputs(1, 33, 3000, H, Hkv, 128, torch.float16, device)
+    r = fa.build_key_ranges(33, 3000, causal=True, query_offsets=2967, device=device)
+    other = [t * 50 for t in _inputs(1, 300, 900, 8, 8, 128, torch.float16, device)[:3]]
+    first = None
+    with torch.no_grad():
+        for _ in range(40):
+            o = fa.flash_attention_v100_with_rules(q, k, v, score_cap=6.0, distance_slopes=_slopes(H, device), key_ranges=r, return_softmax_lse=True)
+            first = first or o
+            assert torch.equal(o[0], first[0]) and torch.equal(o[1], first[1])
+            fa.flash_attention_v100(*other)
+
+
 def test_without_ranges_the_calls_own_masks(device):
     """causal, key_lengths and the alignment build the ranges of the call; without any rule the result is the plain call's."""
     q, k, v, g = _inputs(2, 100, 260, 4, 2, 64, torch.bfloat16, device)
