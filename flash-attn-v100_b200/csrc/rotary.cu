@@ -4,7 +4,8 @@
 // tokens' cosines and sines into shared memory, a pair's once for all heads of q and k: the angle and its reduction by whole
 // turns in 64 bits (at position 10^6 a float angle would be off by 0.06), sine and cosine of the part of a turn that is left
 // in 32.  A unit is one 16-byte piece of a head, or two of them, u and w, where the halves of the head are paired.  Everything
-// is read once and written once: memory bounds it, and for a token or two the launch.
+// is read once and written once: memory bounds it, and for a token or two the launch.  B4 N4096 H32 on 8 D128 bf16, there and back:
+// 116 us, 0.90 of the rate of a copy; one token of each of 32 requests 8 us.
 #include "fa_common.cuh"
 #include "sm100_ptx.cuh"
 #include <type_traits>
