@@ -261,19 +261,28 @@ fwd_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
                 for (int n = 0; n < D / 8; ++n)
                     *reinterpret_cast<float2*>(mine + ((n * 8 + l2) ^ (r0 * 8 & (D - 1)))) = make_float2(acc[n][2 * y] * by, acc[n][2 * y + 1] * by);
-                meet();
-                // a thread four columns of a row
-                for (int e = threadIdx.x; e < 8 * (D / 4); e += 256) {
-                    const int row = e / (D / 4), col = (e % (D / 4)) * 4, r = row + 8 * y;
-                    if (r >= rows) continue;
-                    float big = -INFINITY, sum = 0.f;
+                // A thread four columns of a row (at D 64 half of the threads).  What it reads of the maxima and sums it reads before
+                // it meets the others: a warp that has nothing to add up here may be through the next stretch, and write its own
+                // maxima there, before this stretch's last sums are formed.  (The sums of O are written behind the next stretch's
+                // first meeting.)
+                static_assert(8 * (D / 4) <= 32 * Cfg::kWarps, "a thread has one piece at most");
+                const int e = threadIdx.x, row = e / (D / 4), col = (e % (D / 4)) * 4, r = row + 8 * y;
+                const bool adds = e < 8 * (D / 4) && r < rows;
+                float big = -INFINITY, sum = 0.f;
+                if (adds) {
 #pragma unroll
                     for (int w = 0; w < Cfg::kWarps; ++w) big = fmaxf(big, sMl[w * 16 + r].x);
-                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                     for (int w = 0; w < Cfg::kWarps; ++w) {
                         const float2 ml = sMl[w * 16 + r];
                         sum = fmaf(ml.x == -INFINITY ? 0.f : ex2(ml.x - big), ml.y, sum);
+                    }
+                }
+                meet();
+                if (adds) {
+                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int w = 0; w < Cfg::kWarps; ++w) {
                         const float4 x = *reinterpret_cast<const float4*>(sO + (w * 8 + row) * D + (col ^ (row * 8 & (D - 1))));
                         o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
                     }
