@@ -984,18 +984,20 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 float m = -INFINITY, l = 0.f;
                 // rules: my row's keys and position, and what a key's distance takes off in log2 units
                 // A row that sees nothing, or is none, takes everything: it would have every block of its warp masked.  The
-                // former's results are put aside at the end.
+                // former's results are put aside at the end, and neither has a say in what its warp does: what it meets may be
+                // unwritten memory, and live rows' roundings would follow it.
                 [[maybe_unused]] int2 keys = make_int2(0, 0x7fffffff);
                 [[maybe_unused]] int at = 0, bend = 0, all_from = 0, all_to = 0;      // keys that all of my warp's rows see
                 [[maybe_unused]] float slope = 0.f;
-                [[maybe_unused]] bool dead = false, ahead = false;                    // ahead: some row of my warp sees keys behind its position
+                [[maybe_unused]] bool live = false, ahead = false;                    // ahead: some row of my warp sees keys behind its position
                 if constexpr (RULED) {
                     if (row_ok()) {
                         const int2 x = a.rules.rows[st.b * a.rules.rows_b + i];
-                        dead = x.x >= x.y;
-                        if (!dead) keys = x;
+                        live = x.x < x.y;
+                        if (live) keys = x;
                         if (a.rules.slopes) slope = a.rules.slopes[h] * kLog2e;
                     }
+                    if (!live) m = INFINITY;                   // (which never grows)
                     at = i + a.rules.origin[st.b * a.rules.origin_b];
                     if constexpr (DEALT) {
                         all_from = st.all[t].x;            // (nothing waits for the row's own range before a block has to be masked)
@@ -1004,7 +1006,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         all_from = __reduce_max_sync(0xffffffffu, keys.x);
                         all_to = __reduce_min_sync(0xffffffffu, keys.y);
                     }
-                    if (a.rules.slopes) ahead = __any_sync(0xffffffffu, row_ok() && !dead && at < keys.y - 1);
+                    if (a.rules.slopes) ahead = __any_sync(0xffffffffu, live && at < keys.y - 1);
                 }
                 // my row of the bias (a row beyond Nq, whose results nobody keeps, reads the last one)
                 const float* brow = nullptr;
@@ -1026,6 +1028,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         continue;
                     }
                     tc_fence_after_sync();
+                    const int col0 = j * kBlockN;
                     uint32_t sr[4][32];                    // the row's 128 scores, then its 128 probabilities
 #define SF(c) __uint_as_float(sr[(c) >> 5][(c) & 31])
 #define SSET(c, x) sr[(c) >> 5][(c) & 31] = __float_as_uint(x)
@@ -1033,7 +1036,6 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     for (int c = 0; c < 4; ++c) tmem_ld_32x32(tS + c * 32, sr[c]);
                     tmem_wait_ld();
 
-                    const int col0 = j * kBlockN;
                     if constexpr (PREC != 0) {
                         // Scores in natural units, the bias added as it is and before the mask: masks of the type's lowest
                         // value, of -1e9 or of its largest have to keep x - m (and, in the backward, x - lse) what the
@@ -1081,7 +1083,9 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     if (PREC == 2 && !ok) break;
                     if constexpr (RULES == 2) {
                         // tanh(u) in the place of u = S scale / cap: by the short polynomial while the scores stay small beside
-                        // the cap, else by the long one, else by the exponential; `bend` is where the last block got to
+                        // the cap, else by the long one, else by the exponential; `bend` is where the last block got to.
+                        // The say have the scores of live rows and of keys that the warp's rows see: keys that nobody sees lie in a tile's
+                        // first and last block, and where the vote goes up there it is taken again without them.
                         auto bent = [&](auto form) {
                             const uint64_t in2 = f2_pack(a.cap_in, a.cap_in);
                             float z0 = 0.f, z1 = 0.f;
@@ -1105,15 +1109,27 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                                 }
                             }
                             const float top = decltype(form)::value ? kTanhLongMax : kTanhShortMax;
-                            return !__any_sync(0xffffffffu, fmaxf(z0, z1) > top * top);
+                            return !__any_sync(0xffffffffu, live && fmaxf(z0, z1) > top * top);
                         };
                         auto again = [&] {
 #pragma unroll
                             for (int c = 0; c < 4; ++c) tmem_ld_32x32(tS + c * 32, sr[c]);
                             tmem_wait_ld();
                         };
-                        if (bend == 0 && !bent(std::false_type{})) { bend = 1; again(); }
-                        if (bend == 1 && !bent(std::true_type{})) { bend = 2; again(); }
+                        auto fails = [&](auto form) {
+                            if (bent(form)) return false;
+                            if (j == first || j == n - 1) {
+                                tmem_clear_32x(tS, 0, min((int)__reduce_min_sync(0xffffffffu, live ? keys.x : 0x7fffffff) - col0, kBlockN));
+                                tmem_clear_32x(tS, max((int)__reduce_max_sync(0xffffffffu, live ? keys.y : 0) - col0, 0), kBlockN);
+                                tmem_wait_st();
+                                again();
+                                if (bent(form)) return false;
+                            }
+                            again();
+                            return true;
+                        };
+                        if (bend == 0 && fails(std::false_type{})) bend = 1;
+                        if (bend == 1 && fails(std::true_type{})) bend = 2;
                         if (bend == 2) {
 #pragma unroll
                             for (int c = 0; c < 128; ++c) SSET(c, tanh_any(SF(c) * a.cap_in));
@@ -1324,7 +1340,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
                 if (!ok) break;
 
-                if (RULED && dead) { m = -INFINITY; l = 0.f; }
+                if (RULED && !live) { m = -INFINITY; l = 0.f; }
                 // ---- epilogue: O_t / l -> 16 bit -> global, straight from registers
                 if constexpr (FREE) {
                     wl.again(a, st);
@@ -1385,7 +1401,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     } else {
                         tmem_wait_ld();
                     }
-                    if (RULED && dead) {               // (0 times what it has summed may be no zero)
+                    if (RULED && !live) {              // (0 times what it has summed may be no zero)
 #pragma unroll
                         for (int c = 0; c < 32; ++c) orr[c] = 0u;
                     }

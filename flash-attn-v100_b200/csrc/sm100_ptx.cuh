@@ -304,6 +304,19 @@ __device__ __forceinline__ void tmem_st_32x8(uint32_t taddr, const uint32_t (&r)
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
         : "memory");
 }
+// zeros in my lane's columns [from, to); the whole warp has the same ones
+__device__ __forceinline__ void tmem_clear_32x(uint32_t taddr, int from, int to) {
+    const uint32_t none[8] = {};
+    for (int c = from; c < to;) {
+        if ((c & 7) == 0 && c + 8 <= to) {
+            tmem_st_32x8(taddr + (uint32_t)c, none);
+            c += 8;
+        } else {
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr + (uint32_t)c), "r"(0u) : "memory");
+            ++c;
+        }
+    }
+}
 __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
