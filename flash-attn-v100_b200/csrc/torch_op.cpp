@@ -127,6 +127,24 @@ void backward(at::Tensor d_o, const at::Tensor& q, const at::Tensor& k, const at
     raise_for_status(fa_b200_bwd(&p), "fa_b200_bwd");
 }
 
+// A gradient computed outside of autograd where its own gradient may be asked for (create_graph): it would look like a constant,
+// and a loss that uses it would lose its part without a word.  A node that throws between it and what it is made of.  (As
+// last_derivative in utils.py.)
+struct LastGradient : torch::autograd::Function<LastGradient> {
+    static at::Tensor forward(AutogradContext*, const at::Tensor& gradient, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&) {
+        return gradient.variable_data();                 // (no view: a caller may write to it)
+    }
+    static variable_list backward(AutogradContext*, variable_list) {
+        TORCH_CHECK(false, "these kernels have no gradient of a gradient: a second derivative through attention is not available");
+    }
+};
+variable_list last_derivative(variable_list out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& d_o) {
+    if (at::GradMode::is_enabled())
+        for (at::Tensor& g : out)
+            if (g.defined()) g = LastGradient::apply(g, q, k, v, d_o);
+    return out;
+}
+
 struct Attention : torch::autograd::Function<Attention> {
     static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const Call& c) {
         at::Tensor o, lse, o_lo;
@@ -216,23 +234,25 @@ struct RuledAttention : torch::autograd::Function<RuledAttention> {
         if (!grads[0].defined()) return out;
         const variable_list kept = ctx->get_saved_variables();
         const Ruled r{ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble(), ctx->saved_data["batch"].toInt(), 0, kept[7], kept[5]};
-        at::Tensor d[3];
-        at::AutoDispatchBelowADInplaceOrView below;
-        ruled_backward(grads[0], kept[0], kept[1], kept[2], kept[3], kept[4], kept[6], r, d[0], d[1], d[2]);
-        for (int i = 0; i < 3; ++i)
-            if (ctx->needs_input_grad(i)) out[i] = d[i];
-        return out;
+        {
+            at::Tensor d[3];
+            at::AutoDispatchBelowADInplaceOrView below;
+            ruled_backward(grads[0], kept[0], kept[1], kept[2], kept[3], kept[4], kept[6], r, d[0], d[1], d[2]);
+            for (int i = 0; i < 3; ++i)
+                if (ctx->needs_input_grad(i)) out[i] = d[i];
+        }
+        return last_derivative(std::move(out), kept[0], kept[1], kept[2], grads[0]);
     }
 };
 
 struct Turn {
     at::Tensor positions, inv_freq;      // positions may be undefined
     int64_t offset;
-    bool interleaved;
+    bool interleaved, inverse;
     double factor;
 };
 
-void turn(const at::Tensor* x, const at::Tensor* y, int n, const Turn& t, bool inverse) {
+void turn(const at::Tensor* x, const at::Tensor* y, int n, const Turn& t) {
     fa_b200_rotary_params p;
     memset(&p, 0, sizeof(p));
     p.struct_bytes = sizeof(p);
@@ -246,7 +266,7 @@ void turn(const at::Tensor* x, const at::Tensor* y, int n, const Turn& t, bool i
     p.position0 = t.offset;
     p.inv_freq = t.inv_freq.const_data_ptr<double>();
     p.B = (int32_t)x[0].size(0); p.N = (int32_t)x[0].size(1); p.D = (int32_t)x[0].size(3); p.half = (int32_t)t.inv_freq.size(0);
-    p.interleaved = t.interleaved; p.inverse = inverse; p.factor = (float)t.factor;
+    p.interleaved = t.interleaved; p.inverse = t.inverse; p.factor = (float)t.factor;
     const auto type = x[0].scalar_type();
     p.dtype = type == at::kHalf ? FA_B200_F16 : (type == at::kBFloat16 ? FA_B200_BF16 : FA_B200_F32);
     p.device = x[0].device().index();
@@ -254,44 +274,53 @@ void turn(const at::Tensor* x, const at::Tensor* y, int n, const Turn& t, bool i
     raise_for_status(fa_b200_rotary(&p), "fa_b200_rotary");
 }
 
+// One or two tensors turned, and their gradients: the turn back, which has a gradient of its own.
 template <int N>
-variable_list turned(AutogradContext* ctx, const at::Tensor (&x)[N], const Turn& t) {
-    at::Tensor y[N];
-    for (int i = 0; i < N; ++i) y[i] = at::empty(x[i].sizes(), x[i].options());
-    turn(x, y, N, t, false);
-    ctx->save_for_backward({t.positions, t.inv_freq});
-    ctx->saved_data["offset"] = t.offset;
-    ctx->saved_data["interleaved"] = t.interleaved;
-    ctx->saved_data["factor"] = t.factor;
-    ctx->set_materialize_grads(false);
-    return variable_list(y, y + N);
-}
+struct Rotary : torch::autograd::Function<Rotary<N>> {
+    template <typename... Tensors>
+    static variable_list forward(AutogradContext* ctx, const Turn& t, const Tensors&... xs) {
+        const at::Tensor x[N] = {xs...};
+        at::Tensor y[N];
+        for (int i = 0; i < N; ++i) y[i] = at::empty(x[i].sizes(), x[i].options());
+        turn(x, y, N, t);
+        ctx->save_for_backward({t.positions, t.inv_freq});
+        ctx->saved_data["offset"] = t.offset;
+        ctx->saved_data["interleaved"] = t.interleaved;
+        ctx->saved_data["inverse"] = t.inverse;
+        ctx->saved_data["factor"] = t.factor;
+        ctx->set_materialize_grads(false);
+        return variable_list(y, y + N);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads);
+};
+variable_list turned(const at::Tensor* x, int n, const Turn& t) { return n == 1 ? Rotary<1>::apply(t, x[0]) : Rotary<2>::apply(t, x[0], x[1]); }
+
 template <int N>
-variable_list turned_back(AutogradContext* ctx, variable_list& grads) {
+variable_list Rotary<N>::backward(AutogradContext* ctx, variable_list grads) {
     const variable_list kept = ctx->get_saved_variables();
-    const Turn t{kept[0], kept[1], ctx->saved_data["offset"].toInt(), ctx->saved_data["interleaved"].toBool(), ctx->saved_data["factor"].toDouble()};
-    at::AutoDispatchBelowADInplaceOrView below;
+    const Turn t{kept[0], kept[1], ctx->saved_data["offset"].toInt(), ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["inverse"].toBool(),
+                 ctx->saved_data["factor"].toDouble()};
     at::Tensor g[N], d[N];
     int which[N], n = 0;
+    bool again = false;                  // (create_graph)
     for (int i = 0; i < N; ++i)
-        if (grads[i].defined() && ctx->needs_input_grad(i)) {
+        if (grads[i].defined() && ctx->needs_input_grad(i)) {          // (counts tensors)
             g[n] = grads[i].stride(3) == 1 ? grads[i] : grads[i].contiguous();
-            d[n] = at::empty(g[n].sizes(), g[n].options());
+            again |= at::GradMode::is_enabled() && g[n].requires_grad();
             which[n++] = i;
         }
-    if (n) turn(g, d, n, t, true);
-    variable_list out(N + 1);
-    for (int i = 0; i < n; ++i) out[which[i]] = d[i];
+    variable_list out(N + 1);            // (counts arguments)
+    if (again) {
+        const variable_list back = turned(g, n, t);
+        for (int i = 0; i < n; ++i) out[which[i] + 1] = back[i];
+    } else if (n) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        for (int i = 0; i < n; ++i) d[i] = at::empty(g[i].sizes(), g[i].options());
+        turn(g, d, n, t);
+        for (int i = 0; i < n; ++i) out[which[i] + 1] = d[i];
+    }
     return out;
 }
-struct Rotary1 : torch::autograd::Function<Rotary1> {
-    static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const Turn& t) { return turned<1>(ctx, {q}, t); }
-    static variable_list backward(AutogradContext* ctx, variable_list grads) { return turned_back<1>(ctx, grads); }
-};
-struct Rotary2 : torch::autograd::Function<Rotary2> {
-    static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const Turn& t) { return turned<2>(ctx, {q, k}, t); }
-    static variable_list backward(AutogradContext* ctx, variable_list grads) { return turned_back<2>(ctx, grads); }
-};
 
 // A plain tensor on a GPU: no subclass, no wrapper, no dual number, no bits to be resolved first.
 bool plain(PyObject* obj, const at::Tensor*& t) {
@@ -426,7 +455,7 @@ py::object rotary(py::handle q_, py::handle k_, py::handle positions_, py::handl
     const at::Tensor *qp, *kp = nullptr, *pp = nullptr, *fp;
     if (watched() || !plain(q_.ptr(), qp) || !plain(inv_freq_.ptr(), fp)) return py::none();
     if (!k_.is_none() && !plain(k_.ptr(), kp)) return py::none();
-    Turn t{{}, *fp, 0, interleaved, factor};
+    Turn t{{}, *fp, 0, interleaved, false, factor};
     if (!positions_.is_none()) {
         if (PyLong_CheckExact(positions_.ptr())) {
             t.offset = PyLong_AsLongLong(positions_.ptr());
@@ -456,13 +485,14 @@ py::object rotary(py::handle q_, py::handle k_, py::handle positions_, py::handl
     at::Tensor y[2];
     unlocked([&] {
         if (wants) {
-            variable_list out = kp ? Rotary2::apply(q, k, t) : Rotary1::apply(q, t);
+            const at::Tensor x[2] = {q, k};
+            variable_list out = turned(x, kp ? 2 : 1, t);
             for (size_t i = 0; i < out.size(); ++i) y[i] = std::move(out[i]);
         } else {
             at::AutoDispatchBelowADInplaceOrView below;
             const at::Tensor x[2] = {q, k};
             for (int i = 0; i < (kp ? 2 : 1); ++i) y[i] = at::empty(x[i].sizes(), x[i].options());
-            turn(x, y, kp ? 2 : 1, t, false);
+            turn(x, y, kp ? 2 : 1, t);
         }
     });
     if (!kp) return wrap(std::move(y[0]));

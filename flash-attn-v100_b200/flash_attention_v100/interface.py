@@ -483,7 +483,8 @@ def flash_attention_v100_with_rules(
             of an entry); ranges for them are built by the call.  position_i is i, with the bottom-right alignment i + Nk - Nq
 
     Keys and values before the first and behind the last key that an entry's queries see may be unwritten memory in a call
-    without gradients; those between, and all in a training step, have to be numbers.  Gradients are bit-reproducible.  One GPU: that of the tensors.
+    without gradients; those between, and all in a training step, have to be numbers.  Gradients are bit-reproducible; a gradient of a
+    gradient raises.  One GPU: that of the tensors.
     """
     manager = get_flash_attention_manager()
     profile = manager.enable_profiling or enable_profiling

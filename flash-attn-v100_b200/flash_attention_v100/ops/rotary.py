@@ -89,35 +89,32 @@ def _unit_last(t: torch.Tensor) -> torch.Tensor:
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, positions, offset, inv_freq, interleaved, factor, *xs):
+    def forward(ctx, positions, offset, inv_freq, interleaved, factor, inverse, *xs):
         xs = [_unit_last(x) for x in xs]
         ys = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
-        _launch(xs, ys, positions, offset, inv_freq, interleaved, factor, False)
+        _launch(xs, ys, positions, offset, inv_freq, interleaved, factor, inverse)
         ctx.save_for_backward(positions, inv_freq)
-        ctx.how = (offset, interleaved, factor)
+        ctx.how = (offset, interleaved, factor, inverse)
         ctx.set_materialize_grads(False)
         return ys
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
+        # the gradient of a turn is the turn back, which has a gradient of its own
         positions, inv_freq = ctx.saved_tensors
-        offset, interleaved, factor = ctx.how
-        wanted = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[5 + i]]
+        offset, interleaved, factor, inverse = ctx.how
+        wanted = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[6 + i]]
         out = [None] * len(grads)
         if wanted:
-            gs = [_unit_last(grads[i]) for i in wanted]
-            ds = [torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in gs]
-            _launch(gs, ds, positions, offset, inv_freq, interleaved, factor, True)
-            for i, d in zip(wanted, ds):
+            for i, d in zip(wanted, _Rotary.apply(positions, offset, inv_freq, interleaved, factor, not inverse, *(grads[i] for i in wanted))):
                 out[i] = d
-        return (None,) * 5 + tuple(out)
+        return (None,) * 6 + tuple(out)
 
 
 def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, inv_freq: torch.Tensor,
                      positions: Union[torch.Tensor, int, None] = None, interleaved: bool = False, attention_factor: float = 1.0,
                      inplace: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
-    """q, or (q, k), turned by position; one launch, and one for the gradients of both.
+    """q, or (q, k), turned by position; one launch, and one for the gradients of both, which have gradients of their own.
 
     The columns of a head are taken in pairs (u, w), the i-th of angle a = position * inv_freq[i]:
         u' = attention_factor (u cos a - w sin a),  w' = attention_factor (w cos a + u sin a)
@@ -184,7 +181,7 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, inv_f
             _launch(xs, ys, positions, offset, inv_freq, interleaved, float(attention_factor), False)
         torch.autograd.graph.increment_version(list(xs))
     elif wants:
-        ys = _Rotary.apply(positions, offset, inv_freq, interleaved, float(attention_factor), *xs)
+        ys = _Rotary.apply(positions, offset, inv_freq, interleaved, float(attention_factor), False, *xs)
     else:
         ins = [_unit_last(x) for x in xs]
         ys = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)

@@ -13,7 +13,7 @@ import torch
 
 from ..kernels import _cabi
 from .attention import _base_params, _tensor4, _variant_override
-from ..utils import _last_dim_contiguous
+from ..utils import _last_dim_contiguous, last_derivative
 from .key_ranges import KeyRanges
 
 _RULES_BYTES = ctypes.sizeof(_cabi.RuleParams)
@@ -115,7 +115,7 @@ class RuledAttentionFunction(torch.autograd.Function):
         return o, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @last_derivative
     def backward(ctx, grad_o, _grad_lse=None):
         q, k, v, o, lse, slopes, plan, o_lo = ctx.saved_tensors
         scale, cap, plan_batch = ctx.how

@@ -8,6 +8,7 @@ call.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -93,4 +94,32 @@ def validate_inputs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return _last_dim_contiguous(q), _last_dim_contiguous(k), _last_dim_contiguous(v), float(scale)
 
 
-__all__ = ["cdiv", "validate_inputs"]
+class _LastGradient(torch.autograd.Function):
+    """The first tensor as it is, with a node that raises between it and the others."""
+
+    @staticmethod
+    def forward(ctx, gradient, *made_of):
+        return gradient.data                     # (no view: a caller may write to it)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("these kernels have no gradient of a gradient: a second derivative through attention is not available")
+
+
+def last_derivative(backward):
+    """Decorates a Function's backward whose results are computed outside of autograd.  With create_graph=True they would look
+    like constants, and a loss that uses them would lose their part without a word: they get a node that raises instead.
+    (torch's once_differentiable does so only where the incoming gradient has a graph, and leads to no input of the call, so
+    that torch.autograd.grad passes it by.)"""
+    @functools.wraps(backward)
+    def wrapped(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        made_of = [t for t in (*ctx.saved_tensors, *grads) if isinstance(t, torch.Tensor) and t.requires_grad]
+        return tuple(g if g is None else _LastGradient.apply(g, *made_of) for g in out)
+    return wrapped
+
+
+__all__ = ["cdiv", "validate_inputs", "last_derivative"]
