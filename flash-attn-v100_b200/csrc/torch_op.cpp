@@ -165,14 +165,16 @@ struct Attention : torch::autograd::Function<Attention> {
         const auto lengths = ctx->saved_data.find("lengths");
         const Call c{ctx->saved_data["scale"].toDouble(), (flags & 1) != 0, (flags & 2) != 0, flags >> 2,
                      lengths == ctx->saved_data.end() ? at::Tensor() : lengths->second.toTensor()};
-        at::Tensor d[3];
-        at::AutoDispatchBelowADInplaceOrView below;          // (allocations and a copy: nothing of this is recorded)
-        if (!grads[0].defined()) grads[0] = at::zeros_like(kept[3]);
-        ::backward(grads[0], kept[0], kept[1], kept[2], kept[3], kept[4], kept.size() > 5 ? kept[5] : at::Tensor(), c, d[0], d[1], d[2]);
         variable_list out(4);
-        for (int i = 0; i < 3; ++i)
-            if (ctx->needs_input_grad(i)) out[i] = d[i];
-        return out;
+        {
+            at::Tensor d[3];
+            at::AutoDispatchBelowADInplaceOrView below;          // (allocations and a copy: nothing of this is recorded)
+            if (!grads[0].defined()) grads[0] = at::zeros_like(kept[3]);
+            ::backward(grads[0], kept[0], kept[1], kept[2], kept[3], kept[4], kept.size() > 5 ? kept[5] : at::Tensor(), c, d[0], d[1], d[2]);
+            for (int i = 0; i < 3; ++i)
+                if (ctx->needs_input_grad(i)) out[i] = d[i];
+        }
+        return last_derivative(std::move(out), kept[0], kept[1], kept[2], grads[0]);
     }
 };
 

@@ -31,6 +31,7 @@ from .interface import flash_attention_v100, flash_attention_v100_with_rules
 from .kernels import _cabi
 from .ops.key_ranges import KeyRanges
 from .ops.rotary import rotary_embedding, rotary_frequencies
+from .utils import last_derivative
 
 
 def masks_to_bias(attn_mask: Optional[torch.Tensor], key_padding_mask: Optional[torch.Tensor],
@@ -111,6 +112,7 @@ class _CompactKeys(torch.autograd.Function):
         return k2, v2, counts
 
     @staticmethod
+    @last_derivative
     def backward(ctx, gk, gv, _):
         order, = ctx.saved_tensors
         return _permute_rows(gk.contiguous(), gv.contiguous(), order, True) + (None,)

@@ -18,7 +18,7 @@ import torch
 
 from ..kernels import _cabi
 from ..kernels.tile_table import dtype_enum
-from ..utils import validate_inputs, _last_dim_contiguous
+from ..utils import _last_dim_contiguous, last_derivative, validate_inputs
 
 # --------------------------------------------------------------------------
 # dropout stream state: (seed, offset) are host integers, never read back from
@@ -444,6 +444,7 @@ class EnhancedFlashAttentionV100Function(torch.autograd.Function):
         return o
 
     @staticmethod
+    @last_derivative
     def backward(ctx, grad_output: torch.Tensor, grad_softmax_lse: Optional[torch.Tensor] = None):
         q, k, v, o, lse, *rest = ctx.saved_tensors
         bias = rest[0] if ctx.has_bias else None

@@ -39,6 +39,7 @@ import torch
 import torch.distributed as dist
 
 from . import attention as _ops
+from ..utils import last_derivative
 
 
 LAYOUTS = ("contiguous", "zigzag")
@@ -251,6 +252,7 @@ class RingAttentionFunction(torch.autograd.Function):
         return o, lse
 
     @staticmethod
+    @last_derivative
     def backward(ctx, grad_o, grad_lse=None):
         q, k, v, o, lse = ctx.saved_tensors
         dq, dk, dv = ring_backward(grad_o, q, k, v, o, lse, ctx.scale, ctx.causal, ctx.ring, ctx.kernels,

@@ -4,7 +4,9 @@ import torch
 from torch.utils._python_dispatch import TorchDispatchMode
 
 import flash_attention_v100 as fa
+from flash_attention_v100.ops import sequence_parallel as sp
 from flash_attention_v100.utils import last_derivative
+from ring_helpers import OracleBlockKernels, run_ring
 from rules_helpers import rel, rotary64
 
 
@@ -126,3 +128,58 @@ def test_one_of_two_rotary_gradients(device):
     back, = torch.autograd.grad(d, w, torch.ones_like(d))
     want = rotary64(torch.ones_like(k), torch.arange(5, device=device).view(1, 5), f, False)
     assert rel(back, want) <= 1e-6
+
+
+def test_a_ring_refuses():
+    def rank(ring):
+        q, k, v = (torch.randn(1, 8, 2, 16, generator=torch.Generator().manual_seed(ring.rank), requires_grad=True) for _ in range(3))
+        o = sp.flash_attention_v100_sequence_parallel(q, k, v, causal=True, ring=ring, kernels=OracleBlockKernels)
+        d = torch.autograd.grad(o.sum(), (q, k, v), create_graph=True)
+        for g, x in zip(d, (q, k, v)):
+            with pytest.raises(RuntimeError, match="second derivative"):
+                torch.autograd.grad(g.square().sum() + x.square().sum(), x, retain_graph=True)
+        return True
+
+    assert all(run_ring(2, rank))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["native", "watched", "bias", "dropout", "fp32"])
+def test_plain_attention_refuses(device, form):
+    g = torch.Generator().manual_seed(0)
+    t = torch.float32 if form == "fp32" else torch.bfloat16
+    q, k, v, w = (torch.randn(1, 70, 2, 64, generator=g).to(t).to(device) for _ in range(4))
+    for x in (q, k, v):
+        x.requires_grad_(True)
+    bias = torch.zeros(1, 2, 70, 70, device=device, requires_grad=True) if form == "bias" else None
+
+    def step():
+        inputs = (q, k, v) + ((bias,) if bias is not None else ())
+        stream = dict(dropout_p=0.2, dropout_stream=(1, 0)) if form == "dropout" else {}
+        call = lambda: fa.flash_attention_v100(q, k, v, causal=True, bias=bias, **stream)
+        plain = torch.autograd.grad(call(), inputs, w)
+        o = call()
+        d = torch.autograd.grad(o, inputs, w, create_graph=True)
+        for a, b, x in zip(d, plain, inputs):
+            assert torch.equal(a, b)
+            with pytest.raises(RuntimeError, match="second derivative"):
+                torch.autograd.grad(o.float().sum() + a.float().square().sum(), x, retain_graph=True)
+
+    if form == "watched":
+        with Watch():
+            step()
+    else:
+        step()
+
+
+@pytest.mark.gpu
+def test_a_layer_with_padding_refuses(device):
+    layer = fa.EnhancedMultiHeadAttention(128, 2).to(device).bfloat16()
+    x = torch.randn(2, 30, 128, device=device).bfloat16().requires_grad_(True)
+    mask = torch.zeros(2, 30, dtype=torch.bool, device=device)
+    mask[0, 20:] = True
+    out = layer(x, key_padding_mask=mask)[0]
+    d = torch.autograd.grad(out.float().sum(), [x, *layer.k_proj.parameters()], create_graph=True)
+    for a in d:
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(a.float().square().sum() + x.float().sum(), x, retain_graph=True)
