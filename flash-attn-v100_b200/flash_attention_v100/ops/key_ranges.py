@@ -8,6 +8,7 @@ The reference expands masks to a dense bias instead (examples/basic_usage.py:228
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import Optional, Union
 
 import torch
@@ -71,6 +72,19 @@ def _lengths(name: str, t: Optional[torch.Tensor], shapes, device: torch.device)
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _start(query_offsets) -> int:
+    """query_offsets where it is no tensor."""
+    if query_offsets is None:
+        return 0
+    try:
+        start = operator.index(query_offsets)
+    except TypeError:
+        raise TypeError(f"query_offsets must be a tensor or a whole number, got {type(query_offsets).__name__}") from None
+    if not -_INT32_MAX - 1 <= start <= _INT32_MAX:
+        raise ValueError(f"query_offsets {start} does not fit 32 bits")
+    return start
+
+
 def _most(causal: bool, window: Optional[int]) -> int:
     return 0 if window is None else min(window if causal else 2 * window - 1, _INT32_MAX)
 
@@ -112,12 +126,13 @@ def build_key_ranges(seq_q: int, seq_k: int, *, batch: int = 1, causal: bool = F
         out: an earlier KeyRanges of the same sizes, written anew in place (a captured graph reads it again).  A backward
             whose forward read its earlier contents raises
     """
+    offset_tensor = query_offsets if isinstance(query_offsets, torch.Tensor) else None
+    start = 0 if offset_tensor is not None else _start(query_offsets)
     if out is None and rows is None and (window is None or window >= 1) and not torch.compiler.is_compiling():
         # (None: a form the native operator does not serve, or one that is refused below)
-        starts, start = (query_offsets, 0) if isinstance(query_offsets, torch.Tensor) else (None, query_offsets or 0)
-        index = _device_index(device, document_offsets, prefix_lengths, key_lengths, starts)
+        index = _device_index(device, document_offsets, prefix_lengths, key_lengths, offset_tensor)
         if index is not None:
-            result = _cabi.load_op().key_ranges(seq_q, seq_k, batch, bool(causal), window or 0, document_offsets, prefix_lengths, key_lengths, starts, start, index)
+            result = _cabi.load_op().key_ranges(seq_q, seq_k, batch, bool(causal), window or 0, document_offsets, prefix_lengths, key_lengths, offset_tensor, start, index)
             if result is not None:
                 return KeyRanges(result[0], result[1], batch, seq_q, seq_k, _most(causal, window), result[2], result[3])
     if seq_q < 0 or seq_k < 0 or batch < 0:
@@ -128,7 +143,6 @@ def build_key_ranges(seq_q: int, seq_k: int, *, batch: int = 1, causal: bool = F
         raise ValueError("prefix_lengths are defined for causal ranges without a window")
     if rows is not None and (causal or window is not None or document_offsets is not None or key_lengths is not None):
         raise ValueError("rows are the ranges: causal, window, document_offsets, prefix_lengths and key_lengths cannot be combined with them")
-    offset_tensor = query_offsets if isinstance(query_offsets, torch.Tensor) else None
     if device is None:
         given = next((t for t in (document_offsets, prefix_lengths, key_lengths, offset_tensor, rows) if t is not None), None)
         device = given.device if given is not None else (out.device if out is not None else torch.device("cuda"))
@@ -163,7 +177,7 @@ def build_key_ranges(seq_q: int, seq_k: int, *, batch: int = 1, causal: bool = F
         lengths.data_ptr() if lengths is not None else None, starts.data_ptr() if starts is not None else None,
         documents + 1 if offsets is not None and offsets.dim() == 2 else 0,
         (documents if prefixes.dim() == 2 else (0 if documents else 1)) if prefixes is not None else 0,
-        documents, query_offsets if isinstance(query_offsets, int) else 0, bool(causal), window or 0,
+        documents, start, bool(causal), window or 0,
         batch, seq_q, seq_k, device.index, torch._C._cuda_getCurrentRawStream(device.index) or None)
     _cabi.raise_for_status(lib.fa_b200_key_ranges(ctypes.byref(p)), "fa_b200_key_ranges")
     return out
