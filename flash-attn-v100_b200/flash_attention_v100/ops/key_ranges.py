@@ -137,6 +137,8 @@ def build_key_ranges(seq_q: int, seq_k: int, *, batch: int = 1, causal: bool = F
                 return KeyRanges(result[0], result[1], batch, seq_q, seq_k, _most(causal, window), result[2], result[3])
     if seq_q < 0 or seq_k < 0 or batch < 0:
         raise ValueError(f"sizes must not be negative (seq_q {seq_q}, seq_k {seq_k}, batch {batch})")
+    if max(seq_q, seq_k, batch) > _INT32_MAX:
+        raise ValueError(f"sizes must be below 2**31 (seq_q {seq_q}, seq_k {seq_k}, batch {batch})")
     if window is not None and not 1 <= window <= _INT32_MAX:
         raise ValueError(f"window must be at least 1, got {window}")
     if prefix_lengths is not None and (not causal or window is not None):

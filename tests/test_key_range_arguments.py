@@ -14,6 +14,12 @@ def test_offsets_that_are_no_whole_numbers_of_32_bits(bad, error):
             fa.build_key_ranges(4, 8, query_offsets=bad, device="cuda:0", **more)
 
 
+@pytest.mark.parametrize("sizes", [dict(seq_q=2 ** 32 + 8, seq_k=4), dict(seq_q=8, seq_k=2 ** 31), dict(seq_q=1, seq_k=1, batch=2 ** 32 + 1)])
+def test_sizes_beyond_32_bits(sizes):
+    with pytest.raises(ValueError, match="below 2"):
+        fa.build_key_ranges(**sizes, device="cuda:0")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("offset", [5, np.int64(5), np.int32(5), np.array(5), np.uint8(5)], ids=lambda o: type(o).__name__)
 def test_offsets_of_any_integer_type(device, offset):
