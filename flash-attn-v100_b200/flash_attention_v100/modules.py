@@ -248,8 +248,10 @@ class EnhancedMultiHeadAttention(nn.Module):
         if name == "slopes" and self.distance_slopes is None:
             return None
         if (name, device) not in self._tables:
-            self._tables[name, device] = (rotary_frequencies(self.rotary[0], self.rotary[1], device=device)[0] if name == "frequencies"
-                                          else self.distance_slopes.to(device))
+            # (kept for training steps too: an inference tensor could not be saved for their backwards)
+            with torch.inference_mode(False):
+                table = rotary_frequencies(self.rotary[0], self.rotary[1], device=device)[0] if name == "frequencies" else self.distance_slopes.to(device)
+                self._tables[name, device] = table.clone() if table.is_inference() else table
         return self._tables[name, device]
 
     def get_performance_stats(self) -> Optional[Dict[str, Any]]:

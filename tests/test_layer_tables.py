@@ -1,0 +1,41 @@
+"""What a layer keeps between calls: frequencies and slopes, good for any mode and as they are now."""
+import pytest
+import torch
+
+import flash_attention_v100 as fa
+
+SLOPES = torch.tensor([0.5, 0.0625])
+
+
+def _layer(**kw):
+    torch.manual_seed(1)
+    return fa.EnhancedMultiHeadAttention(128, 2, rotary_base=1e4, score_cap=20.0, distance_slopes=SLOPES, **kw)
+
+
+def test_tables_made_in_inference_mode_serve_training():
+    layer = _layer()
+    with torch.inference_mode():
+        built_there = _layer()
+        for n in ("frequencies", "slopes"):
+            for x in (layer, built_there):
+                assert not x._table(n, torch.device("cpu")).is_inference()
+    for n in ("frequencies", "slopes"):
+        assert not layer._table(n, torch.device("cpu")).is_inference()
+
+
+@pytest.mark.gpu
+def test_an_evaluation_before_training(device):
+    """The first pass under inference_mode, then a training step: as if there had been no first pass."""
+    x = torch.randn(2, 40, 128, generator=torch.Generator().manual_seed(0)).bfloat16().to(device)
+    r = fa.build_key_ranges(40, 40, causal=True, device=device)
+    grads = []
+    for first in (True, False):
+        layer = _layer().to(device).bfloat16()
+        if first:
+            with torch.inference_mode():
+                layer.eval()(x, key_ranges=r)
+            layer.train()
+        layer(x, key_ranges=r)[0].float().square().sum().backward()
+        grads.append([p.grad for p in layer.parameters()])
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
