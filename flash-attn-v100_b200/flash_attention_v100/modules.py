@@ -167,7 +167,7 @@ class EnhancedMultiHeadAttention(nn.Module):
         self.rotary = None if rotary_base is None else (rotary_dim or self.head_dim, float(rotary_base))
         self.distance_slopes = None if distance_slopes is None else distance_slopes.detach().float().clone()
         # frequencies (64 bits) and slopes (32) where they are used: as buffers a module's conversion to bf16 would round them
-        self._tables: Dict[Tuple[str, torch.device], torch.Tensor] = {}
+        self._tables: Dict[Tuple[str, torch.device], Tuple[Any, int, torch.Tensor]] = {}
         self.reset_parameters()
 
     def reset_parameters(self) -> None:
@@ -245,14 +245,17 @@ class EnhancedMultiHeadAttention(nn.Module):
         return out if self.batch_first else out.transpose(0, 1)
 
     def _table(self, name: str, device: torch.device) -> Optional[torch.Tensor]:
-        if name == "slopes" and self.distance_slopes is None:
+        source = self.rotary if name == "frequencies" else self.distance_slopes
+        if source is None:
             return None
-        if (name, device) not in self._tables:
+        version = source._version if isinstance(source, torch.Tensor) and not source.is_inference() else 0
+        kept = self._tables.get((name, device))
+        if kept is None or kept[0] is not source or kept[1] != version:          # (assigned or written anew since)
             # (kept for training steps too: an inference tensor could not be saved for their backwards)
             with torch.inference_mode(False):
-                table = rotary_frequencies(self.rotary[0], self.rotary[1], device=device)[0] if name == "frequencies" else self.distance_slopes.to(device)
-                self._tables[name, device] = table.clone() if table.is_inference() else table
-        return self._tables[name, device]
+                table = rotary_frequencies(*source, device=device)[0] if name == "frequencies" else source.to(device)
+                kept = self._tables[name, device] = (source, version, table.clone() if table.is_inference() else table)
+        return kept[2]
 
     def get_performance_stats(self) -> Optional[Dict[str, Any]]:
         """Reference :252-256.  Only the call count is kept here; time the layer with CUDA events."""

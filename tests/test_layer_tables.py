@@ -23,6 +23,37 @@ def test_tables_made_in_inference_mode_serve_training():
         assert not layer._table(n, torch.device("cpu")).is_inference()
 
 
+def test_tables_follow_what_they_were_made_of():
+    import copy
+    layer, cpu = _layer(), torch.device("cpu")
+    for x in (layer, copy.deepcopy(layer)):
+        t = x._table("frequencies", cpu)
+        assert torch.equal(x._table("slopes", cpu), SLOPES) and x._table("frequencies", cpu) is t
+        x.distance_slopes = torch.tensor([0.25, 0.125])
+        assert x._table("slopes", cpu).tolist() == [0.25, 0.125]
+        x.distance_slopes.mul_(2)
+        assert x._table("slopes", cpu).tolist() == [0.5, 0.25]
+        x.rotary = (32, 500.0)
+        assert torch.equal(x._table("frequencies", cpu), fa.rotary_frequencies(32, 500.0)[0])
+        x.distance_slopes = None
+        assert x._table("slopes", cpu) is None
+
+
+@pytest.mark.gpu
+def test_slopes_assigned_anew_are_seen(device):
+    x = torch.randn(1, 40, 128, generator=torch.Generator().manual_seed(0)).half().to(device)
+    new = torch.tensor([0.25, 0.125])
+    layer, fresh = _layer().to(device).half(), _layer().to(device).half()
+    with torch.no_grad():
+        before = layer(x, is_causal=True)[0]
+        layer.distance_slopes = new
+        fresh.distance_slopes = new.clone()
+        after = layer(x, is_causal=True)[0]
+        assert torch.equal(after, fresh(x, is_causal=True)[0]) and not torch.equal(after, before)
+        layer.distance_slopes.copy_(SLOPES)
+        assert torch.equal(layer(x, is_causal=True)[0], before)
+
+
 @pytest.mark.gpu
 def test_an_evaluation_before_training(device):
     """The first pass under inference_mode, then a training step: as if there had been no first pass."""
