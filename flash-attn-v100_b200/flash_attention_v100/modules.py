@@ -132,6 +132,11 @@ def _warn_no_weights() -> None:
 
 
 class EnhancedMultiHeadAttention(nn.Module):
+    # (a layer pickled whole before there were rules has none of them)
+    score_cap: Optional[float] = None
+    rotary: Optional[Tuple[int, float]] = None
+    distance_slopes: Optional[torch.Tensor] = None
+
     def __init__(self, embed_dim: int, num_heads: int, dropout: float = 0.0, bias: bool = True,
                  batch_first: bool = True, optimization_strategy: str = "balanced",
                  enable_multi_gpu: bool = True, enable_gradient_checkpointing: bool = False,

@@ -39,6 +39,19 @@ def test_tables_follow_what_they_were_made_of():
         assert x._table("slopes", cpu) is None
 
 
+def test_a_layer_pickled_before_there_were_rules():
+    import io
+    layer = fa.EnhancedMultiHeadAttention(128, 2)
+    for name in ("score_cap", "rotary", "distance_slopes", "_tables"):
+        del layer.__dict__[name]
+    f = io.BytesIO()
+    torch.save(layer, f)
+    f.seek(0)
+    old = torch.load(f, weights_only=False)
+    with pytest.raises(ValueError, match="CUDA"):            # (what any layer says on the CPU)
+        old(torch.zeros(1, 4, 128))
+
+
 @pytest.mark.gpu
 def test_slopes_assigned_anew_are_seen(device):
     x = torch.randn(1, 40, 128, generator=torch.Generator().manual_seed(0)).half().to(device)
