@@ -1725,7 +1725,8 @@ FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, int ru
     int64_t whole = (n_items + sms - 1) / sms * ((col + items - 1) / items);
     int64_t pair_most = (p.Nk + kBlockN - 1) / kBlockN;
     if (ruled) {
-        if (max_keys > 0 && (max_keys + 2 * kBlockM) / kBlockN + 1 < pair_most) pair_most = (max_keys + 2 * kBlockM) / kBlockN + 1;
+        const int64_t most = ((int64_t)max_keys + 2 * kBlockM) / kBlockN + 1;
+        if (max_keys > 0 && most < pair_most) pair_most = most;
         whole = (n_items * pair_most + sms - 1) / sms;
         if (whole < pair_most) whole = pair_most;
     }
@@ -1873,7 +1874,7 @@ int launch(const fa_b200_params& p, void* ws, size_t ws_bytes, const Rules* rule
             merge = fwd_decode_merge_kernel<D, BF16>;
             cfg.gridDim.y = (unsigned)(p.Nq * plan.pack);
             cfg.blockDim = dim3(128);
-        } else if (plan.ctas >= kManyParts * p.B * plan.heads * plan.n_pairs && !p.o_lo.ptr) {
+        } else if (plan.ctas >= (int64_t)kManyParts * p.B * plan.heads * plan.n_pairs && !p.o_lo.ptr) {
             merge = fwd_merge_many_kernel<D, BF16>;
             cfg.gridDim.z = D / 16;
         }
