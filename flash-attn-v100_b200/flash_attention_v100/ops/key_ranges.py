@@ -109,7 +109,9 @@ def build_key_ranges(seq_q: int, seq_k: int, *, batch: int = 1, causal: bool = F
                      out: Optional[KeyRanges] = None) -> KeyRanges:
     """Build a KeyRanges on the GPU.
 
-    Row i of batch entry b stands at position t = i + query_offsets[b] (an int: of every entry; default 0).
+    Row i of batch entry b stands at position t = i + query_offsets[b] (an int: of every entry; default 0).  Without documents
+    rows at t < 0 (more queries than a cache has keys) go by the same rules: under causal they see no key but a prefix, else the
+    keys of their window, or all.
 
     Args:
         seq_q, seq_k: rows and keys of the attention calls;  batch: entries, 1 serves any batch

@@ -325,11 +325,12 @@ int fa_b200_permute_rows(const void* src0, const void* src1, void* dst0, void* d
  *
  * Row i of batch entry b stands at position t = i + query_offset + query_offsets[b].
  *   document    the m with document_offsets[b][m] <= t < document_offsets[b][m + 1] (ascending; none: the row sees
- *               nothing); without documents one that starts at 0 and has no end
+ *               nothing); without documents one for all rows, those at t < 0 among them (more queries than a cache has
+ *               keys), whose start counts as 0 and which has no end
  *   first       the document's start, with a window at least t - window + 1
  *   end         the document's end, at most Nk and key_lengths[b]; causal: at most t + 1, or, where it is more, the
  *               document's start + prefix_lengths[b][m]; a window without causal: at most t + window
- *   position    t - the document's start (0 for a row of no document)
+ *   position    t - the document's start (0 for a row of no document; below 0 for t < 0 without documents)
  * A row with first >= end sees nothing and is stored as (0, 0).  With `rows` the intervals are given instead (clipped to
  * [0, Nk]), the fields above but query_offset(s), which count distances, are ignored, and positions are t.
  *

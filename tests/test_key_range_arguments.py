@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import flash_attention_v100 as fa
+from test_gpu_key_ranges import build, check
 
 
 @pytest.mark.parametrize("bad,error", [(3.0, TypeError), ("3", TypeError), ([3], TypeError), (2 ** 31, ValueError), (2 ** 32 + 5, ValueError),
@@ -31,3 +32,14 @@ def test_offsets_of_any_integer_type(device, offset):
     by_hand = fa.build_key_ranges(3, 50, rows=torch.tensor([[[0, 6], [0, 7], [0, 8]]], device=device), query_offsets=offset)
     for r, ends in ((first, [6, 7, 8]), (general, [6, 7, 7]), (anew, [6, 7, 8]), (by_hand, [6, 7, 8])):
         assert r.end.tolist() == [ends] and r.positions.tolist() == [[5, 6, 7]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mask", [dict(causal=True), dict(), dict(window=4), dict(window=40), dict(causal=True, window=4), dict(causal=True, prefixes=[3, 0, 50])], ids=str)
+def test_more_queries_than_a_cache_has_keys(device, mask):
+    """Rows before the first key: by the mask's rule as any other row, with positions below 0."""
+    lengths, Nq, Nk = [2, 20, 0], 20, 60
+    host = dict(mask, lengths=lengths, starts=[n - Nq for n in lengths])
+    r = build(Nq, Nk, 3, host, device)
+    check(r, Nq, Nk, 3, host)
+    assert r.positions.tolist() == [[n - Nq + i for i in range(Nq)] for n in lengths]
