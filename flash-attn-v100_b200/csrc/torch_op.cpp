@@ -422,7 +422,9 @@ py::object attention_rules(py::handle q_, py::handle k_, py::handle v_, py::hand
     const int device = q.device().index();
     if (device >= kMaxDevices || !g_status_word[device].load(std::memory_order_acquire)) return py::none();
     Ruled r{std::pow((double)q.size(3), -0.5), 0.0, batch, max_keys, {}, *pp};
-    if (q.size(1) != seq_q || k.size(1) != seq_k || (batch != 1 && batch != q.size(0)) || r.plan.device() != q.device()) return py::none();
+    if (q.size(1) != seq_q || k.size(1) != seq_k || (batch != 1 && batch != q.size(0)) || r.plan.device() != q.device() || r.plan.scalar_type() != at::kInt ||
+        !r.plan.is_contiguous() || (size_t)r.plan.numel() * 4 < fa_b200_key_ranges_bytes((int)batch, (int)seq_q, (int)seq_k))
+        return py::none();
     if (!scale_.is_none()) {
         if (!PyFloat_CheckExact(scale_.ptr())) return py::none();
         r.scale = PyFloat_AS_DOUBLE(scale_.ptr());

@@ -54,6 +54,14 @@ class KeyRanges:
         return self._column(1) if self._end is None else self._end
 
 
+def check_plan(r: KeyRanges) -> None:
+    """Raises where r cannot be what build_key_ranges made: the kernels read, and a build writes, as many bytes as its sizes say."""
+    need = _cabi.load().fa_b200_key_ranges_bytes(r.batch, r.seq_q, r.seq_k) // 4
+    if r.plan.dtype != torch.int32 or not r.plan.is_contiguous() or r.plan.numel() < need:
+        raise ValueError(f"a plan for batch {r.batch}, {r.seq_q} rows and {r.seq_k} keys is {need} dense int32, got "
+                         f"{r.plan.numel()} of {r.plan.dtype}: KeyRanges come from build_key_ranges")
+
+
 def _lengths(name: str, t: Optional[torch.Tensor], shapes, device: torch.device) -> Optional[torch.Tensor]:
     """Whole numbers on the device as dense int32."""
     if t is None:
@@ -173,6 +181,10 @@ def build_key_ranges(seq_q: int, seq_k: int, *, batch: int = 1, causal: bool = F
     else:
         if (out.batch, out.seq_q, out.seq_k) != (batch, seq_q, seq_k) or out.device != device:
             raise ValueError(f"out is for batch {out.batch}, {out.seq_q} rows and {out.seq_k} keys on {out.device}")
+        check_plan(out)
+        if tuple(out.positions.shape) != (batch, seq_q) or out.positions.dtype != torch.int32 or not out.positions.is_contiguous() or \
+                out.positions.device != device:
+            raise ValueError("out.positions are not build_key_ranges'")
         torch.autograd.graph.increment_version([out.plan, out.positions])
         out.max_keys = _most(causal, window)
     p = _cabi.RangesParams(

@@ -14,7 +14,7 @@ import torch
 from ..kernels import _cabi
 from .attention import _base_params, _tensor4, _variant_override
 from ..utils import _last_dim_contiguous, last_derivative
-from .key_ranges import KeyRanges
+from .key_ranges import KeyRanges, check_plan
 
 _RULES_BYTES = ctypes.sizeof(_cabi.RuleParams)
 
@@ -50,6 +50,7 @@ def check_rules(q: torch.Tensor, k: torch.Tensor, score_cap: Optional[float], sl
                              f"the call has batch {q.shape[0]}, {q.shape[1]} rows and {k.shape[1]} keys")
         if ranges.device != q.device:
             raise ValueError("key_ranges must be on the same device as input tensors")
+        check_plan(ranges)
     return cap, slopes
 
 

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import flash_attention_v100 as fa
+from flash_attention_v100.ops.rules import check_rules
 from test_gpu_key_ranges import build, check
 
 
@@ -19,6 +20,34 @@ def test_offsets_that_are_no_whole_numbers_of_32_bits(bad, error):
 def test_sizes_beyond_32_bits(sizes):
     with pytest.raises(ValueError, match="below 2"):
         fa.build_key_ranges(**sizes, device="cuda:0")
+
+
+def _by_hand(device, entries, dtype=torch.int32):
+    return fa.KeyRanges(torch.zeros(entries, dtype=dtype, device=device), torch.zeros(2, 300, dtype=torch.int32, device=device), 2, 300, 300)
+
+
+def test_a_plan_made_by_hand_is_measured():
+    q = torch.zeros(2, 300, 1, 8)
+    need = 2 * 384 * 2 + 2 * 3 * 4 + 2 * 24 * 2 + 2 * 3 * 2 + 2 * (3 + 2 + 3) + 4
+    check_rules(q, q, None, None, _by_hand("cpu", need))
+    for bad in (_by_hand("cpu", need - 1), _by_hand("cpu", 0), _by_hand("cpu", need, torch.int64)):
+        with pytest.raises(ValueError, match="come from build_key_ranges"):
+            check_rules(q, q, None, None, bad)
+
+
+@pytest.mark.gpu
+def test_a_plan_made_by_hand_is_refused(device):
+    """Both ways to use it: an attention call, in the native form first, and a build that would write it."""
+    q = torch.zeros(2, 300, 1, 64, device=device).half()
+    bad = _by_hand(device, 100)
+    with pytest.raises(ValueError, match="come from build_key_ranges"):
+        fa.flash_attention_v100_with_rules(q, q, q, key_ranges=bad)
+    with pytest.raises(ValueError, match="come from build_key_ranges"):
+        fa.build_key_ranges(300, 300, batch=2, device=device, out=bad)
+    good = fa.build_key_ranges(300, 300, batch=2, device=device)
+    good.positions = good.positions[:1]
+    with pytest.raises(ValueError, match="positions"):
+        fa.build_key_ranges(300, 300, batch=2, device=device, out=good)
 
 
 @pytest.mark.gpu
