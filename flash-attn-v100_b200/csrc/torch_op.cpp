@@ -432,7 +432,7 @@ py::object attention_rules(py::handle q_, py::handle k_, py::handle v_, py::hand
     if (!cap_.is_none()) {
         if (!PyFloat_CheckExact(cap_.ptr())) return py::none();
         r.cap = PyFloat_AS_DOUBLE(cap_.ptr());
-        if (!(r.cap > 0.0 && r.cap < 1e30)) return py::none();
+        if (!((float)r.cap > 0.f && r.cap < 1e30)) return py::none();
     }
     if (!slopes_.is_none()) {
         if (!plain(slopes_.ptr(), sp) || sp->scalar_type() != at::kFloat || sp->device() != q.device() || sp->dim() != 1 || sp->size(0) != q.size(2) ||

@@ -29,8 +29,8 @@ def check_rules(q: torch.Tensor, k: torch.Tensor, score_cap: Optional[float], sl
     cap = 0.0
     if score_cap is not None:
         cap = float(score_cap)
-        if not 0.0 < cap < 1e30:
-            raise ValueError(f"score_cap must be positive and finite, got {score_cap}")
+        if not 0.0 < cap < 1e30 or ctypes.c_float(cap).value == 0.0:        # (a 0 would mean none to the kernels)
+            raise ValueError(f"score_cap must be positive and finite in 32 bits, got {score_cap}")
     if slopes is not None:
         if not isinstance(slopes, torch.Tensor):
             raise TypeError("distance_slopes must be a torch.Tensor")
