@@ -166,7 +166,10 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, inv_f
         if tuple(positions.shape) not in ((N,), (1, N), (B, N)):
             raise ValueError(f"positions have shape {tuple(positions.shape)}, expected ({N},), (1, {N}) or ({B}, {N})")
     elif positions is not None:
-        offset, positions = int(positions), None
+        offset = int(positions)
+        if offset != positions or not -2 ** 63 <= offset < 2 ** 63:
+            raise ValueError(f"positions must be a tensor or a whole number of 64 bits, got {positions!r}")
+        positions = None
     wants = torch.is_grad_enabled() and any(x.requires_grad for x in xs)
     if inplace:
         if wants:
