@@ -6,8 +6,9 @@
 // H32 Hkv8 D128 bf16, cap and distances: 207 us, here 124 to 139 from one GPU to another, 106 at the copy rate).  So the
 // small matrix instruction instead: each of eight warps takes 16 keys of a 128-key block, S (16 x 16) = Q K^T with Q in
 // registers and K by ldmatrix from the tile TMA has brought, its own running maximum and sum, O (16 x D) += P V in registers.
-// A warp never waits for another one until a stretch ends, when the eight are put together through shared memory.  P is fp16,
-// or for bf16 calls a pair of bf16 hi + lo (two products), so that its rounding stays below the output's.
+// A warp never waits for another one until a stretch ends, when the eight are put together through shared memory.  P is
+// a pair of values of the call's type, hi + lo (two products), so that its rounding stays below the output's (as one value an
+// fp16 call was off by 2.9e-4 of its outputs where their own rounding is 2.1e-4; 32 requests 144 -> 147 us).
 // Sixteen warps (registers then spill: 202 us), 8-row registers (no change) and, at D 64, two blocks a warp at once (no
 // change) brought nothing; D 64 gets 62 % of D 128's rate out of a cache whose heads lie side by side, 128 bytes a head.
 #pragma once
@@ -210,8 +211,7 @@ fwd_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                         for (int y = 0; y < 2; ++y) {
                             const float p0 = ex2(sc[n][2 * y] + off[y]), p1 = ex2(sc[n][2 * y + 1] + off[y]);
                             l[y] += p0 + p1;
-                            if constexpr (BF16) pack2_pair<true>(p0, p1, ph_[2 * n + y], pl_[2 * n + y]);
-                            else ph_[2 * n + y] = pack2<false>(p0, p1);
+                            pack2_pair<BF16>(p0, p1, ph_[2 * n + y], pl_[2 * n + y]);
                         }
                 }
                 ok = ok && mbar_wait(&bars[Cfg::kFull + ST + s], ph, abort_flag);
@@ -233,10 +233,8 @@ fwd_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                         if (edge) { b[0] &= keep[0]; b[1] &= keep[1]; b[2] &= keep[0]; b[3] &= keep[1]; }
                         mma_16816<BF16>(acc[2 * n], ph_, b[0], b[1]);
                         mma_16816<BF16>(acc[2 * n + 1], ph_, b[2], b[3]);
-                        if constexpr (BF16) {
-                            mma_16816<BF16>(acc[2 * n], pl_, b[0], b[1]);
-                            mma_16816<BF16>(acc[2 * n + 1], pl_, b[2], b[3]);
-                        }
+                        mma_16816<BF16>(acc[2 * n], pl_, b[0], b[1]);
+                        mma_16816<BF16>(acc[2 * n + 1], pl_, b[2], b[3]);
                     }
                 }
                 mbar_arrive_warp(&bars[Cfg::kEmpty + s]);

@@ -36,3 +36,22 @@ def test_blocks_that_go_from_request_to_request(device, B, Nq, H, Hkv, D):
         for _ in range(50):
             again = call()
             assert torch.equal(again[0], o) and torch.equal(again[1], lse)
+
+
+@pytest.mark.parametrize("B,Nk,H,Hkv,D", [(6, 4096, 8, 8, 128), (4, 3000, 8, 2, 64), (3, 700, 4, 1, 80)])
+@pytest.mark.parametrize("cap", [None, 30.0])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+def test_outputs_are_rounded_once(device, dtype, B, Nk, H, Hkv, D, cap):
+    """Nearly every output is the formula's, rounded.  Before that rounding it is off by what scores (30 * 2^-22 under the cap) and
+    sums in 32 bits are: 1e-5 of it, a fiftieth of the least distance of two fp16 numbers, so that one in fifty may be the
+    neighbour.  (Probabilities rounded to 16 bits would be off by 2^-12 each, which moves one in three.)"""
+    g = torch.Generator().manual_seed(11)
+    q, k, v = (torch.randn(B, n, h, D, generator=g).to(dtype).to(device) for n, h in ((1, H), (Nk, Hkv), (Nk, Hkv)))
+    lengths = [Nk - 31 * b for b in range(B)]
+    counts = torch.tensor(lengths, dtype=torch.int32, device=device)
+    r = fa.build_key_ranges(1, Nk, batch=B, causal=True, key_lengths=counts, query_offsets=counts - 1)
+    see = torch.stack([visible(1, Nk, b, lengths=lengths) for b in range(B)])
+    want = attention64(q, k, v, see, torch.zeros(B, 1), D ** -0.5, cap)[0].to(dtype)
+    with torch.no_grad():
+        o = fa.flash_attention_v100_with_rules(q, k, v, score_cap=cap, key_ranges=r)
+    assert (o != want).float().mean().item() <= 0.05
