@@ -606,9 +606,9 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         prefetch_tensormap(&map_v);
     }
     if (FREE && warp == 11) find_range<SCHED, RULES>(a, lane, range);
-    if (RULED && FREE && warp == 10) {
-        // a packed tile's rows behind its last query, which no copy writes: their scores have a say in which of the tanh
-        // polynomials a warp takes, and what shared memory held before would come out as other roundings
+    if (FREE && warp == 10) {
+        // a packed tile's rows behind its last query, which no copy writes: their scores have a say in when a warp scales its sums
+        // anew, and what shared memory held before would come out as other roundings
         const int rows = a.pack * a.q_per_tile, pieces = (kBlockM - rows) * 8;
         for (int e = lane; e < Cfg::kQTiles * Cfg::kNBox * pieces; e += 32)
             *reinterpret_cast<uint4*>(sQ + e / pieces * kBoxBytes + rows * 128 + e % pieces * 16) = make_uint4(0u, 0u, 0u, 0u);
