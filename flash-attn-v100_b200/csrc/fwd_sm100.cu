@@ -1689,7 +1689,7 @@ constexpr int kDecodeRows = 16;        // rows of a K/V head that fwd_decode_ker
 // With rules whole pairs are dealt out as CTAs get done (Dealer), so a round-robin share is what the SMs have on average, one
 // pair at least, and a pair's keys are at most `max_keys` and its own 256 (0: not known).  Ranges cost more there, because a
 // packed tile's hull is read from memory wherever a walk comes to it: 700 queries on 8892 keys, H32 Hkv8 D128 bf16, whole ->
-// ranges, us: all keys 139 -> 133, with a cap 215 -> 172; window 4096 82 -> 90, 118 -> 111; window 1024 35 -> 57, 45 -> 68.
+// ranges, us: all keys 153 -> 136, with a cap 226 -> 181; window 4096 85 -> 93, 120 -> 118; window 1024 36 -> 58, 46 -> 69.
 // A block with a cap takes half as long again, so a merge is worth fewer of them.
 constexpr int kMergeUnitsRules = 16, kMergeUnitsCap = 8;
 FwdPlan plan_schedule(const fa_b200_params& p, int D, int sms, bool free, int rules = 0, int max_keys = 0) {

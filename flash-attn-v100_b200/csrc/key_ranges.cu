@@ -1,9 +1,10 @@
 // Which keys each query sees, as one interval a row (the definition is in fa_b200.h), with what the attention kernels
 // want to know of 16 and 128 rows and of 128 keys at once.
 //
-// A thread makes a row: a binary search of its document, a few minima and maxima.  What bounds it is latency, two
-// dependent launches and the search's chain of loads: 12 bytes a row are written, 1.5 MB at 8 rows of 16384 tokens, where a call
-// with 32 documents a row takes 14 us; one row for each of 64 requests 11.
+// A thread makes a row: a binary search of its document, a few minima and maxima.  What bounds it is latency: two dependent
+// launches (one for up to 128 rows, whose tiles need no order) and the search's chain of loads.  12 bytes a row are written, 1.5 MB at
+// 8 rows of 16384 tokens, where a call with 32 documents a row takes 14 us; one row for each of 64 requests 11, most of it the
+// host's, which makes a plan, positions and two views.
 #include "fa_common.cuh"
 #include "sm100_ptx.cuh"
 #include <limits.h>

@@ -472,7 +472,8 @@ def flash_attention_v100_with_rules(
     Args:
         q, k, v, scale, return_softmax_lse, enable_profiling: as flash_attention_v100's; grouped heads, every dtype and
             head size it takes.  fp16 and bf16 with a head size that is a multiple of 8 run on the tensor cores, others on
-            the CUDA cores
+            the CUDA cores.  On the tensor cores bf16 V (and in a training step q, k and v) become fp16 at every head size, as in plain
+            calls of head sizes 64 and 128: exact for 2^-17 <= |x| < 65520, saturating beyond
         score_cap: positive; None leaves the scores as they are
         distance_slopes: (num_heads,) floating point, no gradient.  A score x is rounded to 2^-24 |x|, as any 32-bit
             evaluation has it: 2^-24 slope times distance, where a query is far from all keys it sees
@@ -483,7 +484,8 @@ def flash_attention_v100_with_rules(
             of an entry); ranges for them are built by the call.  position_i is i, with the bottom-right alignment i + Nk - Nq
 
     Keys and values before the first and behind the last key that an entry's queries see may be unwritten memory in a call
-    without gradients; those between, and all in a training step, have to be numbers.  Gradients are bit-reproducible; a gradient of a
+    without gradients; those between, and all in a training step, have to be numbers.  A training step in fp16 or bf16 keeps one more
+    tensor of the output's size than the output, what its rounding dropped.  Gradients are bit-reproducible; a gradient of a
     gradient raises.  One GPU: that of the tensors.
     """
     manager = get_flash_attention_manager()

@@ -363,8 +363,12 @@ int fa_b200_key_ranges(const fa_b200_ranges_params* p);
  * with softmax, output, lse and gradients of x.  A row that sees nothing has an output of zeros, an lse of -inf and no
  * gradient.  Positions are those of the plan's query offsets.  In fa_b200_params causal, causal_shift, bias, kv_lengths,
  * d_scores, dropout_p and the rng_* fields have to be zero; the plan says what they would.
- * Keys and values before the first and behind the last key that rows of a call's batch entry see may hold anything in a
- * forward (an unwritten cache); those between, and all in a backward, have to be numbers.
+ * Keys and values before the first and behind the last key that rows of a call's batch entry see, and queries that see
+ * nothing, may hold anything in a forward (an unwritten cache) and change no bit of it; those between, and all in a
+ * backward, have to be numbers.
+ * fp16 and bf16 on the tensor cores: probabilities are one fp16 value (calls of up to 16 rows a K/V head with scratch: a
+ * hi + lo pair), dS one (fp16 results: a pair), and bf16 V and, in a backward, Q, K and dO become fp16 at every head size, exact
+ * for 2^-17 <= |x| < 65520 and saturating beyond (dO is normalised).
  * No counterpart in the reference.
  */
 typedef struct fa_b200_rules {

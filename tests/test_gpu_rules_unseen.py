@@ -28,7 +28,7 @@ RULES = {"cap": (6.0, False), "slopes": (None, True), "both": (6.0, True)}
 
 @pytest.mark.parametrize("rule", RULES)
 @pytest.mark.parametrize("Nq,H,Hkv,D", [(1, 4, 2, 64), (7, 4, 2, 128), (20, 2, 2, 64), (33, 3, 1, 128), (300, 2, 1, 64), (700, 4, 4, 128), (300, 4, 2, 80)])
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=["bf16", "fp16", "fp32"])
 def test_unwritten_ends_of_caches(device, dtype, Nq, H, Hkv, D, rule):
     """Scores of a tenth of the cap, so that what is behind a cache would change how the cap's tanh is taken, or when a row's
     sums are scaled anew."""
@@ -50,14 +50,15 @@ def test_unwritten_ends_of_caches(device, dtype, Nq, H, Hkv, D, rule):
 
 
 @pytest.mark.parametrize("rule", RULES)
-@pytest.mark.parametrize("N,D", [(40, 128), (300, 64), (1000, 128)])
-def test_queries_that_see_nothing(device, N, D, rule):
+@pytest.mark.parametrize("N,D", [(12, 64), (40, 128), (300, 64), (1000, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_queries_that_see_nothing(device, dtype, N, D, rule):
     """Padding behind the last document, between the rows of a tile's others: its queries, keys and values may be anything."""
     cap, slopes = RULES[rule]
     slopes = torch.linspace(0.01, 0.2, 2, device=device) if slopes else None
-    q, k, v = (_normal(2, N, 2, D, torch.bfloat16, device, s, x) for s, x in ((0, 0.3), (1, 1.0), (2, 1.0)))
+    q, k, v = (_normal(2, N, 2, D, dtype, device, s, x) for s, x in ((0, 0.3), (1, 1.0), (2, 1.0)))
     ends = [N - 9, N // 2 - 3]
-    r = fa.build_key_ranges(N, N, batch=2, causal=True, document_offsets=torch.tensor([[0, 11, e] for e in ends], dtype=torch.int32, device=device))
+    r = fa.build_key_ranges(N, N, batch=2, causal=True, document_offsets=torch.tensor([[0, min(11, e), e] for e in ends], dtype=torch.int32, device=device))
 
     def fill(x):
         for b, e in enumerate(ends):
