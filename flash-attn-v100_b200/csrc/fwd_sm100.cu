@@ -989,15 +989,15 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 [[maybe_unused]] int2 keys = make_int2(0, 0x7fffffff);
                 [[maybe_unused]] int at = 0, bend = 0, all_from = 0, all_to = 0;      // keys that all of my warp's rows see
                 [[maybe_unused]] float slope = 0.f;
-                [[maybe_unused]] bool live = false, ahead = false;                    // ahead: some row of my warp sees keys behind its position
+                [[maybe_unused]] bool ahead = false;                                   // ahead: some row of my warp sees keys behind its position
+                auto live = [&] { return keys.y != 0x7fffffff; };       // (no range ends there; kept apart it cost 1 % of a chunk)
                 if constexpr (RULED) {
                     if (row_ok()) {
                         const int2 x = a.rules.rows[st.b * a.rules.rows_b + i];
-                        live = x.x < x.y;
-                        if (live) keys = x;
+                        if (x.x < x.y) keys = x;
                         if (a.rules.slopes) slope = a.rules.slopes[h] * kLog2e;
                     }
-                    if (!live) m = INFINITY;                   // (which never grows)
+                    if (!live()) m = INFINITY;                   // (which never grows)
                     at = i + a.rules.origin[st.b * a.rules.origin_b];
                     if constexpr (DEALT) {
                         all_from = st.all[t].x;            // (nothing waits for the row's own range before a block has to be masked)
@@ -1006,7 +1006,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         all_from = __reduce_max_sync(0xffffffffu, keys.x);
                         all_to = __reduce_min_sync(0xffffffffu, keys.y);
                     }
-                    if (a.rules.slopes) ahead = __any_sync(0xffffffffu, live && at < keys.y - 1);
+                    if (a.rules.slopes) ahead = __any_sync(0xffffffffu, live() && at < keys.y - 1);
                 }
                 // my row of the bias (a row beyond Nq, whose results nobody keeps, reads the last one)
                 const float* brow = nullptr;
@@ -1109,7 +1109,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                                 }
                             }
                             const float top = decltype(form)::value ? kTanhLongMax : kTanhShortMax;
-                            return !__any_sync(0xffffffffu, live && fmaxf(z0, z1) > top * top);
+                            return !__any_sync(0xffffffffu, live() && fmaxf(z0, z1) > top * top);
                         };
                         auto again = [&] {
 #pragma unroll
@@ -1119,8 +1119,8 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         auto fails = [&](auto form) {
                             if (bent(form)) return false;
                             if (j == first || j == n - 1) {
-                                tmem_clear_32x(tS, 0, min((int)__reduce_min_sync(0xffffffffu, live ? keys.x : 0x7fffffff) - col0, kBlockN));
-                                tmem_clear_32x(tS, max((int)__reduce_max_sync(0xffffffffu, live ? keys.y : 0) - col0, 0), kBlockN);
+                                tmem_clear_32x(tS, 0, min((int)__reduce_min_sync(0xffffffffu, live() ? keys.x : 0x7fffffff) - col0, kBlockN));
+                                tmem_clear_32x(tS, max((int)__reduce_max_sync(0xffffffffu, live() ? keys.y : 0) - col0, 0), kBlockN);
                                 tmem_wait_st();
                                 again();
                                 if (bent(form)) return false;
@@ -1340,7 +1340,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
                 if (!ok) break;
 
-                if (RULED && !live) { m = -INFINITY; l = 0.f; }
+                if (RULED && !live()) { m = -INFINITY; l = 0.f; }
                 // ---- epilogue: O_t / l -> 16 bit -> global, straight from registers
                 if constexpr (FREE) {
                     wl.again(a, st);
@@ -1401,7 +1401,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     } else {
                         tmem_wait_ld();
                     }
-                    if (RULED && !live) {              // (0 times what it has summed may be no zero)
+                    if (RULED && !live()) {              // (0 times what it has summed may be no zero)
 #pragma unroll
                         for (int c = 0; c < 32; ++c) orr[c] = 0u;
                     }
